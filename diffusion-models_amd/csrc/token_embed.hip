@@ -1,0 +1,349 @@
+// Rows of an embedding table by token, scaled, and the table's gradient.
+//
+//   out[i]     = scale * table[token_i]
+//   dtable[t] += scale * sum of dout[i] over the i with token_i = t, in ascending order of i inside chunks of the sorted
+//                tokens, chunk by chunk (never by float atomics: the same bits every time)
+//
+// Both directions only move data: forward reads a row and writes a row per token, the gradient reads dout once and writes every
+// row that some token names. The gradient sorts the (token, i) pairs by token (stable radix sort, 8 bits a pass), so
+// that a row's terms are neighbours, and cuts the SORTED order into equal chunks: a token that makes up half of the
+// batch costs no more than as many rare ones.
+#include "dm_common.h"
+
+namespace {
+
+constexpr int TILE = 2048;      // keys a workgroup sorts at a time: 4 waves x 8 rounds x 64 lanes
+constexpr int RADIX = 256;
+
+// number of threads that share a row of `vecs` vectors: a power of two, so that a workgroup holds whole rows
+int threads_per_row(int vecs) {
+  int t = 1;
+  while (t < 256 && t < vecs) t <<= 1;
+  return t;
+}
+
+template <typename T, int V> struct Vec;
+template <> struct Vec<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float* f) { *(f32x4_t*)f = *(const f32x4_t*)p; }
+  static __device__ __forceinline__ void store(float* p, const float* f) { *(f32x4_t*)p = *(const f32x4_t*)f; }
+};
+template <> struct Vec<float, 1> {
+  static __device__ __forceinline__ void load(const float* p, float* f) { *f = *p; }
+  static __device__ __forceinline__ void store(float* p, const float* f) { *p = *f; }
+};
+template <> struct Vec<bf16_t, 4> {
+  static __device__ __forceinline__ void load(const bf16_t* p, float* f) {
+    const bf16x4_t v = *(const bf16x4_t*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (float)v[e];
+  }
+  static __device__ __forceinline__ void store(bf16_t* p, const float* f) {
+    bf16x4_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (bf16_t)f[e];
+    *(bf16x4_t*)p = v;
+  }
+};
+template <> struct Vec<bf16_t, 1> {
+  static __device__ __forceinline__ void load(const bf16_t* p, float* f) { *f = (float)*p; }
+  static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *p = (bf16_t)*f; }
+};
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void token_embed_kernel(const float* __restrict__ table, const int64_t* __restrict__ tokens,
+                                                          T* __restrict__ out, long n, long rows, int width, float scale, int tpr) {
+  const long i = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+  if (i >= n) return;
+  const int64_t t = tokens[i];
+  const bool live = t >= 0 && t < rows;
+  const float* src = table + (live ? t : 0) * (long)width;
+  for (int e = (threadIdx.x & (tpr - 1)) * V; e < width; e += tpr * V) {
+    float f[V];
+    Vec<float, V>::load(src + e, f);
+#pragma unroll
+    for (int x = 0; x < V; ++x) f[x] = live ? f[x] * scale : 0.f;
+    Vec<T, V>::store(out + i * (long)width + e, f);
+  }
+}
+
+// A token's sort key: the token itself, or `rows` (sorted behind every token) where it has no gradient
+__device__ __forceinline__ unsigned key_of(const int64_t* tokens, long i, long rows, long padding) {
+  const int64_t t = tokens[i];
+  return t < 0 || t >= rows || t == padding ? (unsigned)rows : (unsigned)t;
+}
+
+// counts of the first digit in every tile; the later passes' counts are cleared (the pass before fills them)
+__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ tokens, unsigned* __restrict__ counts, long n,
+                                                         long rows, long padding, int tiles, int passes) {
+  __shared__ unsigned c[RADIX];
+  const int t = blockIdx.x, tid = threadIdx.x;
+  c[tid] = 0;
+  __syncthreads();
+  for (int u = 0; u < TILE / 256; ++u) {
+    const long i = (long)t * TILE + u * 256 + tid;
+    if (i < n) atomicAdd(&c[key_of(tokens, i, rows, padding) & (RADIX - 1)], 1u);
+  }
+  __syncthreads();
+  counts[(long)t * RADIX + tid] = c[tid];
+  for (int p = 1; p < passes; ++p) counts[((long)p * tiles + t) * RADIX + tid] = 0;
+}
+
+// One stable pass: a key's place is (keys of smaller digits) + (keys of its digit in earlier tiles, waves and lanes).
+// Inside a wave the lanes of one digit find each other with 8 ballots.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restrict__ tokens, const unsigned* __restrict__ key_in,
+                                                        const unsigned* __restrict__ idx_in, unsigned* __restrict__ key_out,
+                                                        unsigned* __restrict__ idx_out, const unsigned* __restrict__ counts,
+                                                        unsigned* __restrict__ next, long n, long rows, long padding, int tiles, int shift) {
+  __shared__ unsigned base[RADIX], wcount[4][RADIX];
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) wcount[w][tid] = 0;
+  unsigned before = 0, total = 0;
+#pragma unroll 8
+  for (int x = 0; x < tiles; ++x) {
+    const unsigned c = counts[(long)x * RADIX + tid];
+    total += c;
+    before += x < t ? c : 0;
+  }
+  base[tid] = total;
+  __syncthreads();
+  for (int o = 1; o < RADIX; o <<= 1) {   // inclusive sums over the digits
+    const unsigned v = tid >= o ? base[tid - o] : 0;
+    __syncthreads();
+    base[tid] += v;
+    __syncthreads();
+  }
+  const unsigned start = base[tid] - total + before;
+  constexpr int ROUNDS = TILE / 256;
+  unsigned key[ROUNDS], idx[ROUNDS], rank[ROUNDS];
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const long i = (long)t * TILE + wave * (TILE / 4) + u * 64 + lane;
+    const bool in = i < n;
+    if constexpr (FIRST) {
+      key[u] = in ? key_of(tokens, i, rows, padding) : 0;
+      idx[u] = (unsigned)i;
+    } else {
+      key[u] = in ? key_in[i] : 0;
+      idx[u] = in ? idx_in[i] : 0;
+    }
+    const unsigned d = (key[u] >> shift) & (RADIX - 1);
+    unsigned long long same = __ballot(in);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const bool one = (d >> bit) & 1;
+      const unsigned long long m = __ballot(one);
+      same &= one ? m : ~m;
+    }
+    const int lower = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+    const unsigned have = wcount[wave][d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // every lane has read before one of them writes, and the next round reads that
+    rank[u] = have + lower;
+    if (in && lower == 0) wcount[wave][d] = have + __builtin_popcountll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  {   // the wave counts become places
+    unsigned s = start;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const unsigned c = wcount[w][tid];
+      wcount[w][tid] = s;
+      s += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const long i = (long)t * TILE + wave * (TILE / 4) + u * 64 + lane;
+    if (i >= n) continue;
+    const unsigned to = wcount[wave][(key[u] >> shift) & (RADIX - 1)] + rank[u];
+    key_out[to] = key[u];
+    idx_out[to] = idx[u];
+    if (next) atomicAdd(&next[(long)(to / TILE) * RADIX + ((key[u] >> (shift + 8)) & (RADIX - 1))], 1u);
+  }
+}
+
+// Sums of runs of equal keys inside one chunk of the sorted order. A run that lies inside the chunk goes to its row; the
+// part of a run that began before the chunk, and the part of one that goes on behind it, are left in part[chunk][0 / 1].
+template <typename T, int V>
+__global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout, const unsigned* __restrict__ key,
+                                                      const unsigned* __restrict__ idx, float* __restrict__ dtable, float* __restrict__ part,
+                                                      long n, unsigned rows, int width, float scale, int tpr, int chunk) {
+  const long c = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+  const int e = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * V;
+  const long p0 = c * chunk, p1 = min(p0 + chunk, n);
+  if (p0 >= n || e >= width) return;
+  constexpr int U = 8;
+  float s[V];
+#pragma unroll
+  for (int x = 0; x < V; ++x) s[x] = 0.f;
+  bool began = p0 == 0 || key[p0 - 1] != key[p0];   // the current run began in this chunk
+  for (long p = p0; p < p1; p += U) {
+    float f[U][V];
+    unsigned k[U + 1];
+#pragma unroll
+    for (int u = 0; u <= U; ++u) k[u] = p + u < n ? key[p + u] : 0xffffffffu;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = p + u < p1 && k[u] < rows;
+      if (on) Vec<T, V>::load(dout + (long)idx[p + u] * width + e, f[u]);
+      else
+#pragma unroll
+        for (int x = 0; x < V; ++x) f[u][x] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p + u >= p1 || k[u] >= rows) break;
+#pragma unroll
+      for (int x = 0; x < V; ++x) s[x] += f[u][x];
+      const bool last = p + u + 1 >= p1, ends = k[u + 1] != k[u];
+      if (ends || last) {
+        if (began && ends) {
+          float* to = dtable + (long)k[u] * width + e;
+          float g[V];
+          Vec<float, V>::load(to, g);
+#pragma unroll
+          for (int x = 0; x < V; ++x) g[x] += s[x] * scale;
+          Vec<float, V>::store(to, g);
+        } else {
+          Vec<float, V>::store(part + (c * 2 + (began ? 1 : 0)) * (long)width + e, s);
+        }
+#pragma unroll
+        for (int x = 0; x < V; ++x) s[x] = 0.f;
+        began = true;
+      }
+    }
+  }
+}
+
+// A run that goes on behind the chunk it began in: its parts, chunk by chunk
+template <int V>
+__global__ __launch_bounds__(256) void run_join_kernel(const unsigned* __restrict__ key, const float* __restrict__ part,
+                                                       float* __restrict__ dtable, long n, unsigned rows, int width, float scale, int tpr,
+                                                       int chunk) {
+  const long c = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+  const int e = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * V;
+  const long p0 = c * chunk, p1 = p0 + chunk;
+  if (p1 >= n || e >= width) return;
+  const unsigned k = key[p1 - 1];
+  if (k >= rows || key[p1] != k) return;
+  if (key[p0] == k && p0 > 0 && key[p0 - 1] == k) return;   // began before this chunk
+  float s[V];
+  Vec<float, V>::load(part + (c * 2 + 1) * (long)width + e, s);
+  for (long x = c + 1; x * chunk < n && key[x * chunk] == k; ++x) {
+    float f[V];
+    Vec<float, V>::load(part + x * 2 * (long)width + e, f);
+#pragma unroll
+    for (int y = 0; y < V; ++y) s[y] += f[y];
+  }
+  float* to = dtable + (long)k * width + e;
+  float g[V];
+  Vec<float, V>::load(to, g);
+#pragma unroll
+  for (int x = 0; x < V; ++x) g[x] += s[x] * scale;
+  Vec<float, V>::store(to, g);
+}
+
+int chunk_of(long n) { return n >= 65536 ? 64 : 16; }
+
+struct Plan {   // parts of the workspace, in bytes
+  long tiles, chunks;
+  int passes;
+  size_t key[2], idx[2], counts, part, total;
+};
+Plan plan_of(long n, long rows, int width) {
+  Plan p;
+  p.tiles = (n + TILE - 1) / TILE;
+  const int chunk = chunk_of(n);
+  p.chunks = (n + chunk - 1) / chunk;
+  p.passes = 1;
+  while (p.passes < 4 && (rows >> (8 * p.passes)) != 0) ++p.passes;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+  for (int i = 0; i < 2; ++i) { p.key[i] = take(n * 4); p.idx[i] = take(n * 4); }
+  p.counts = take((size_t)p.passes * p.tiles * RADIX * 4);
+  p.part = take((size_t)p.chunks * 2 * width * 4);
+  p.total = at;
+  return p;
+}
+
+int check_embed(const char* who, long n, long rows, int width) {
+  DM_REQUIRE(n >= 0 && n < 0x7fffffffL, DM_ERR_SHAPE, "%s: %ld tokens (up to 2^31-2)", who, n);
+  DM_REQUIRE(rows > 0 && rows < 0x7fffffffL, DM_ERR_SHAPE, "%s: %ld rows (1 to 2^31-2)", who, rows);
+  DM_REQUIRE(width > 0 && width <= 65536, DM_ERR_SHAPE, "%s: width %d (1 to 65536)", who, width);
+  return DM_OK;
+}
+bool vectors(int width, const void* a, const void* b) {
+  return width % 4 == 0 && (((uintptr_t)a | (uintptr_t)b) & 15) == 0;
+}
+
+}  // namespace
+
+extern "C" int dm_token_embed(const float* table, const int64_t* tokens, void* out, int out_bf16, long n, long rows, int width,
+                              float scale, void* stream) {
+  const char* who = "dm_token_embed";
+  int rc = check_embed(who, n, rows, width);
+  if (rc) return rc;
+  if (n == 0) return DM_OK;
+  DM_REQUIRE(table && tokens && out, DM_ERR_ARG, "%s: null pointer", who);
+  const bool vec = vectors(width, table, out);
+  const int tpr = threads_per_row(vec ? width / 4 : width);
+  const dim3 grid(dm_cdiv(n, 256 / tpr)), block(256);
+  hipStream_t st = (hipStream_t)stream;
+#define GO(T, V) hipLaunchKernelGGL((token_embed_kernel<T, V>), grid, block, 0, st, table, tokens, (T*)out, n, rows, width, scale, tpr)
+  if (out_bf16) { if (vec) GO(bf16_t, 4); else GO(bf16_t, 1); }
+  else { if (vec) GO(float, 4); else GO(float, 1); }
+#undef GO
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
+
+extern "C" size_t dm_token_embed_bwd_ws_bytes(long n, long rows, int width) {
+  if (check_embed("dm_token_embed_bwd_ws_bytes", n, rows, width)) return 0;
+  return plan_of(n, rows, width).total;
+}
+
+extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t* tokens, float* dtable, long n, long rows, int width,
+                                  float scale, long padding, void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "dm_token_embed_bwd";
+  int rc = check_embed(who, n, rows, width);
+  if (rc) return rc;
+  if (n == 0) return DM_OK;
+  DM_REQUIRE(dout && tokens && dtable, DM_ERR_ARG, "%s: null pointer", who);
+  const Plan p = plan_of(n, rows, width);
+  DM_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= p.total, DM_ERR_ARG, "%s: workspace of %zu bytes is too small or misaligned (%zu)", who, ws_bytes, p.total);
+  char* w = (char*)ws;
+  unsigned *key[2] = {(unsigned*)(w + p.key[0]), (unsigned*)(w + p.key[1])}, *idx[2] = {(unsigned*)(w + p.idx[0]), (unsigned*)(w + p.idx[1])};
+  unsigned* counts = (unsigned*)(w + p.counts);
+  float* part = (float*)(w + p.part);
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 block(256), tiles(p.tiles);
+  hipLaunchKernelGGL(sort_count_kernel, tiles, block, 0, st, tokens, counts, n, rows, padding, (int)p.tiles, p.passes);
+  DM_CHECK_LAUNCH();
+  for (int i = 0; i < p.passes; ++i) {
+    unsigned* now = counts + (long)i * p.tiles * RADIX;
+    unsigned* next = i + 1 < p.passes ? now + p.tiles * RADIX : nullptr;
+    if (i == 0)
+      hipLaunchKernelGGL((sort_pass_kernel<true>), tiles, block, 0, st, tokens, nullptr, nullptr, key[0], idx[0], now, next, n, rows, padding, (int)p.tiles, 0);
+    else
+      hipLaunchKernelGGL((sort_pass_kernel<false>), tiles, block, 0, st, tokens, key[(i - 1) & 1], idx[(i - 1) & 1], key[i & 1], idx[i & 1], now, next, n, rows, padding, (int)p.tiles, 8 * i);
+    DM_CHECK_LAUNCH();
+  }
+  const unsigned *sk = key[(p.passes - 1) & 1], *si = idx[(p.passes - 1) & 1];
+  const bool vec = vectors(width, dout, dtable);
+  const int vecs = vec ? width / 4 : width, tpr = threads_per_row(vecs), chunk = chunk_of(n);
+  const dim3 grid(dm_cdiv(p.chunks, 256 / tpr), dm_cdiv(vecs, tpr));
+#define GO(T, V) hipLaunchKernelGGL((run_sum_kernel<T, V>), grid, block, 0, st, (const T*)dout, sk, si, dtable, part, n, (unsigned)rows, width, scale, tpr, chunk)
+  if (dout_bf16) { if (vec) GO(bf16_t, 4); else GO(bf16_t, 1); }
+  else { if (vec) GO(float, 4); else GO(float, 1); }
+#undef GO
+  DM_CHECK_LAUNCH();
+  if (p.chunks > 1) {
+    if (vec) hipLaunchKernelGGL((run_join_kernel<4>), grid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, tpr, chunk);
+    else hipLaunchKernelGGL((run_join_kernel<1>), grid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, tpr, chunk);
+    DM_CHECK_LAUNCH();
+  }
+  return DM_OK;
+}

@@ -57,6 +57,12 @@ class WtItem(ctypes.Structure):
     _fields_ = [("offset", c_long), ("Cout", c_int), ("T", c_int), ("Cin", c_int), ("tile_begin", c_int)]
 
 
+class BlockDesc(ctypes.Structure):
+    """dm_block_desc: attention over chosen key blocks."""
+    _fields_ = [(n, c_int) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top")] + [("scale", c_float)] + \
+        [(n, c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "dq_stride", "dk_stride", "dv_stride")]
+
+
 P = c_void_p
 _SIGNATURES = {
     "dm_abi_version": (c_int, []),
@@ -93,6 +99,15 @@ _SIGNATURES = {
     "dm_groupnorm_param_grads": (c_int, [ctypes.POINTER(GnDesc)] + [P] * 6),
     "dm_attention_fwd": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_float, P]),
     "dm_attention_bwd": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, P]),
+    "dm_block_keys": (c_int, [P] * 5),
+    "dm_block_select": (c_int, [P] * 6),
+    "dm_block_attention_mask_bytes": (ctypes.c_size_t, [P, c_int]),
+    "dm_block_attention_fwd": (c_int, [P] * 11),
+    "dm_block_attention_bwd_ws_bytes": (ctypes.c_size_t, [P]),
+    "dm_block_attention_bwd": (c_int, [P] * 15 + [ctypes.c_size_t, P]),
+    "dm_token_embed": (c_int, [P, P, P, c_int, c_long, c_long, c_int, c_float, P]),
+    "dm_token_embed_bwd_ws_bytes": (ctypes.c_size_t, [c_long, c_long, c_int]),
+    "dm_token_embed_bwd": (c_int, [P, c_int, P, P, c_long, c_long, c_int, c_float, c_long, P, ctypes.c_size_t, P]),
     "dm_timestep_embed": (c_int, [P, P, P, c_int, c_int, P]),
     "dm_linear_fwd": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, P]),
     "dm_linear_bwd": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, P]),

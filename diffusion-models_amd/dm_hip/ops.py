@@ -4,13 +4,15 @@ Activations travel between operators as bf16 tensors of logical shape [B, C, H, 
 format, i.e. physically pixel-major [B][H][W][C] as the kernels expect; token tensors [B, L, C] are the same
 memory. Parameters stay fp32 in the reference's shapes. Every function here needs a HIP device tensor.
 """
+import contextlib
 import ctypes
 import os
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
-from . import ConvDesc, ConvProj, GnDesc, LinearItem, SumItem, WgradItem, check, lib
+from . import BlockDesc, ConvDesc, ConvProj, GnDesc, LinearItem, SumItem, WgradItem, check, lib
 
 BF16 = torch.bfloat16
 CL = torch.channels_last
@@ -836,6 +838,300 @@ class _AttentionFn(Function):
 
 def attention(qkv, n_heads, head_dim, scale=None):
     return _AttentionFn.apply(qkv, n_heads, head_dim, float(head_dim ** -0.5 if scale is None else scale))
+
+
+# ------------------------------------------------------------------------------------------------------------
+# Attention of each query over key blocks chosen for it, for sequences too long for `attention` above. Tensors are
+# [B, positions, heads, head_dim] (the parts of a packed qkv are read in place); BLOCK keys make a block.
+BLOCK = 64
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context in which launches and scratch go to `device` (torch's current device may be another one)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _tokens4(t, name, who):
+    """A bf16 [B, L, H, D] tensor whose rows of D can be read 16 bytes at a time; copied only if it is not one."""
+    _require_device(t, who)
+    if t.dim() != 4:
+        raise RuntimeError(f"{who}: {name} must be [batch, positions, heads, head_dim], got {tuple(t.shape)}")
+    if t.shape[3] not in (8, 16, 32, 64):
+        raise RuntimeError(f"{who}: head dims 8, 16, 32 and 64 are covered; {name} has {t.shape[3]}")
+    if t.dtype != BF16:
+        t = t.to(BF16)
+    s = t.stride()
+    if (s[3] != 1 and t.numel()) or (s[0] | s[1] | s[2] | (t.data_ptr() >> 1)) & 7:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _lengths(k_len, B, device, who):
+    if k_len is None:
+        return None
+    if k_len.shape != (B,) or k_len.is_floating_point() or k_len.is_complex():
+        raise RuntimeError(f"{who}: k_len must hold {B} whole numbers, one a sample; got {tuple(k_len.shape)} {k_len.dtype}")
+    if k_len.device != device:
+        raise RuntimeError(f"{who}: k_len is on {k_len.device}, the keys on {device}")
+    if k_len.dtype != torch.int32:   # (64-bit lengths clamp instead of wrapping)
+        k_len = k_len.clamp(0, 2 ** 31 - 1).to(torch.int32) if k_len.dtype == torch.int64 else k_len.to(torch.int32)
+    return k_len.contiguous()
+
+
+def _block_desc(B, Lq, Lk, Hq, Hkv, D, top, scale=1.0, q=None, k=None, v=None):
+    d = BlockDesc(B, Lq, Lk, Hq, Hkv, D, top, scale)
+    for t, to in ((q, d.q_stride), (k, d.k_stride), (v, d.v_stride)):
+        if t is not None:
+            to[:] = t.stride()[:3]
+    return d
+
+
+def _check_top(top, who):
+    if not 1 <= int(top) <= 64:
+        raise RuntimeError(f"{who}: 1 to 64 blocks a query, not {top}")
+    return int(top)
+
+
+def _check_heads(q, k, who):
+    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[-1] or q.device != k.device:
+        raise RuntimeError(f"{who}: queries {tuple(q.shape)} on {q.device} do not go with keys {tuple(k.shape)} on {k.device}")
+
+
+def block_keys(k, k_len=None):
+    """One summary a block, the mean of its valid keys: [B, key heads, ceil(Lk / 64), head_dim] bf16. k_len: [B] whole numbers,
+    the valid keys of each sample (None: all). Not differentiable: a summary only ranks blocks. Keys that do not change from
+    call to call (a text, the past of a sequence) need it once."""
+    k = _tokens4(k.detach(), "k", "block_keys")
+    B, Lk, H, D = k.shape
+    k_len = _lengths(k_len, B, k.device, "block_keys")
+    with _on(k.device):
+        keys = torch.empty((B, H, -(-Lk // BLOCK), D), dtype=BF16, device=k.device)
+        if keys.numel():
+            d = _block_desc(B, 1, Lk, H, H, D, 1, k=k)
+            check(lib.dm_block_keys(ctypes.byref(d), k.data_ptr(), _p(k_len), keys.data_ptr(), _stream()))
+    return keys
+
+
+def block_select(q, keys, top, k_len=None):
+    """The `top` blocks (1 to 64) of the highest q . keys for every query: int32 [B, query heads, Lq, top], ascending, -1 behind
+    the last where a sample has fewer. keys: block_keys of the keys; their heads may be shared by groups of query heads. Compared
+    in 64 bits; ties go to the lower block, NaN counts as -infinity. Not differentiable."""
+    top = _check_top(top, "block_select")
+    q = _tokens4(q.detach(), "q", "block_select")
+    B, Lq, Hq, D = q.shape
+    _require_device(keys, "block_select")
+    if keys.dim() != 4 or keys.shape[1] == 0 or Hq % keys.shape[1]:
+        raise RuntimeError(f"block_select: keys {tuple(keys.shape)} are not summaries for {Hq} query heads")
+    _check_heads(q, keys, "block_select")
+    keys = keys.detach().to(BF16).contiguous()
+    if keys.data_ptr() & 15:
+        keys = keys.clone()
+    n = keys.shape[2]
+    k_len = _lengths(k_len, B, q.device, "block_select")
+    with _on(q.device):
+        blocks = torch.empty((B, Hq, Lq, top), dtype=torch.int32, device=q.device)
+        if n == 0:
+            return blocks.fill_(-1)
+        if blocks.numel():
+            d = _block_desc(B, Lq, n * BLOCK, Hq, keys.shape[1], D, top, q=q)
+            check(lib.dm_block_select(ctypes.byref(d), q.data_ptr(), keys.data_ptr(), _p(k_len), blocks.data_ptr(), _stream()))
+    return blocks
+
+
+def _block_forward(d, q, k, v, blocks, k_len, training):
+    dev = q.device
+    out = torch.empty((d.B, d.Lq, d.Hq, d.D), dtype=BF16, device=dev)
+    out_lo = torch.empty_like(out) if training else None
+    lse = torch.empty((d.B, d.Hq, d.Lq), dtype=torch.float32, device=dev) if training else None
+    n = lib.dm_block_attention_mask_bytes(ctypes.byref(d), int(training))
+    mask = torch.empty(n // 8, dtype=torch.int64, device=dev) if n else None
+    check(lib.dm_block_attention_fwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
+                                     out.data_ptr(), _p(out_lo), _p(lse), _p(mask), _stream()))
+    return out, (mask, out_lo, lse)
+
+
+def _block_backward(d, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
+    mask, out_lo, lse = kept
+    for t, to in ((dq, d.dq_stride), (dk, d.dk_stride), (dv, d.dv_stride)):
+        to[:] = t.stride()[:3]
+    n = lib.dm_block_attention_bwd_ws_bytes(ctypes.byref(d))
+    ws = _scratch(q.device, (n + 3) // 4)
+    check(lib.dm_block_attention_bwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
+                                     mask.data_ptr(), out.data_ptr(), out_lo.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream()))
+
+
+class _BlockAttentionFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, blocks, k_len, d):
+        with _on(q.device):
+            out, kept = _block_forward(d, q, k, v, blocks, k_len, True)
+        ctx.save_for_backward(q, k, v, blocks, k_len, out, *kept)
+        ctx.d = d
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, blocks, k_len, out, *kept = ctx.saved_tensors
+        with _on(q.device):
+            dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k, v))
+            d = _block_desc(*(getattr(ctx.d, n) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top", "scale")), q, k, v)
+            _block_backward(d, q, k, v, blocks, k_len, out, kept, _aligned(dout), dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+def _aligned(t):
+    """bf16, contiguous and 16-byte aligned"""
+    t = t.to(BF16).contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def block_attention(q, k, v, blocks, scale=None, k_len=None):
+    """softmax(scale * q k^T) v of every query over the keys of its own blocks, and the gradients of q, k and v.
+
+    q [B, Lq, Hq, D], k and v [B, Lk, Hkv, D] (Hq a multiple of Hkv: neighbouring query heads share a key head; D 8, 16, 32 or
+    64; any strides with contiguous rows of D that start at multiples of 16 bytes, others are copied); blocks int32
+    [B, Hq, Lq, n], n up to 64, as block_select gives them: any order, a repeated block counts once, numbers outside
+    0 .. ceil(Lk / 64) - 1 name none. k_len as in block_keys; what lies behind the valid keys is never used. A query
+    without a key gives zeros and has no gradient. Returns bf16 [B, Lq, Hq, D]."""
+    who = "block_attention"
+    q, k, v = _tokens4(q, "q", who), _tokens4(k, "k", who), _tokens4(v, "v", who)
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1:3]
+    if k.shape != v.shape or k.device != v.device:
+        raise RuntimeError(f"{who}: keys {tuple(k.shape)} on {k.device} and values {tuple(v.shape)} on {v.device} differ")
+    _check_heads(q, k, who)
+    if Hkv == 0 or Hq % Hkv:
+        raise RuntimeError(f"{who}: {Hq} query heads do not share {Hkv} key heads evenly")
+    if blocks.dim() != 4 or blocks.shape[:3] != (B, Hq, Lq) or blocks.dtype != torch.int32 or blocks.device != q.device:
+        raise RuntimeError(f"{who}: blocks must be int32 {(B, Hq, Lq)} + (n,) on {q.device}, got {blocks.dtype} "
+                           f"{tuple(blocks.shape)} on {blocks.device}")
+    top = _check_top(blocks.shape[3], who)
+    k_len = _lengths(k_len, B, q.device, who)
+    if B * Lq * Hq * Lk == 0:   # nothing to attend: zeros, tied to the inputs so that their gradients are zeros too
+        nothing = q.masked_fill(torch.ones((), dtype=torch.bool, device=q.device), 0.0)
+        return nothing + 0.0 * (k.sum() + v.sum())   # (either k and v are empty or q is)
+    d = _block_desc(B, Lq, Lk, Hq, Hkv, D, top, float(D ** -0.5 if scale is None else scale), q, k, v)
+    blocks = blocks.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _BlockAttentionFn.apply(q, k, v, blocks, k_len, d)
+    with _on(q.device):
+        return _block_forward(d, q, k, v, blocks, k_len, False)[0]
+
+
+class _SparseAttentionFn(Function):
+    """The packed form: q, k and v are read in place and their gradients written into one packed tensor."""
+
+    @staticmethod
+    def forward(ctx, qkv, H, D, top, scale, training):
+        B, L, _ = qkv.shape
+        q, k, v = qkv.view(B, L, 3, H, D).unbind(2)
+        d = _block_desc(B, L, L, H, H, D, top, scale, q, k, v)
+        with _on(qkv.device):
+            blocks = block_select(q, block_keys(k), top)
+            out, kept = _block_forward(d, q, k, v, blocks, None, training)
+        if training:
+            ctx.save_for_backward(qkv, blocks, out, *kept)
+            ctx.cfg = (B, L, H, D, top, scale)
+        return out.view(B, L, H * D)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, blocks, out, *kept = ctx.saved_tensors
+        B, L, H, D, top, scale = ctx.cfg
+        q, k, v = qkv.view(B, L, 3, H, D).unbind(2)
+        with _on(qkv.device):
+            dqkv = torch.empty_like(qkv)
+            d = _block_desc(B, L, L, H, H, D, top, scale, q, k, v)
+            _block_backward(d, q, k, v, blocks, None, out, kept, _aligned(dout), *dqkv.view(B, L, 3, H, D).unbind(2))
+        return dqkv, None, None, None, None, None
+
+
+def sparse_attention(qkv, n_heads, head_dim, top, scale=None):
+    """Self-attention on a packed qkv [B, L, 3 * n_heads * head_dim] like `attention`, but every query attends only to the
+    `top` blocks of 64 positions whose mean key it scores highest (block_keys, block_select, block_attention in one call).
+    top >= L / 64 attends everywhere. The choice itself has no gradient."""
+    _require_device(qkv, "sparse_attention")
+    top = _check_top(top, "sparse_attention")
+    if qkv.dim() != 3 or qkv.shape[2] != 3 * n_heads * head_dim:
+        raise RuntimeError(f"sparse_attention: packed qkv is {tuple(qkv.shape)}, expected [batch, positions, 3*{n_heads}*{head_dim}]")
+    if head_dim not in (8, 16, 32, 64):
+        raise RuntimeError(f"sparse_attention: head dims 8, 16, 32 and 64 are covered, not {head_dim}")
+    qkv = _aligned(qkv)
+    scale = float(head_dim ** -0.5 if scale is None else scale)
+    if qkv.numel() == 0:
+        return qkv[..., :n_heads * head_dim] * 1.0
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _SparseAttentionFn.apply(qkv, n_heads, head_dim, top, scale, True)
+    return _SparseAttentionFn.forward(None, qkv, n_heads, head_dim, top, scale, False)
+
+
+# ------------------------------------------------------------------------------------------------------------
+def _embed_rows(tokens, table, scale, dtype):
+    with _on(table.device):
+        out = torch.empty(tokens.shape + table.shape[1:], dtype=dtype, device=table.device)
+        if out.numel():
+            check(lib.dm_token_embed(table.data_ptr(), tokens.data_ptr(), out.data_ptr(), int(dtype == BF16), tokens.numel(),
+                                     table.shape[0], table.shape[1], scale, _stream()))
+    return out
+
+
+class _TokenEmbedFn(Function):
+    @staticmethod
+    def forward(ctx, table, tokens, scale, padding, dtype):
+        ctx.save_for_backward(tokens)
+        ctx.param = table
+        ctx.cfg = (tuple(table.shape), table.dtype, scale, padding)
+        return _embed_rows(tokens, f32c(table.detach()), scale, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (tokens,) = ctx.saved_tensors
+        (rows, width), dtype, scale, padding = ctx.cfg
+        if dout.dtype not in (BF16, torch.float32):
+            dout = dout.float()
+        dout = dout.contiguous()
+        sink = _grad_sink(ctx.param)
+        with _on(dout.device):
+            dtable = sink if sink is not None else torch.zeros((rows, width), dtype=torch.float32, device=dout.device)
+            n = tokens.numel()
+            if n and width:
+                need = lib.dm_token_embed_bwd_ws_bytes(n, rows, width)
+                ws = _scratch(dout.device, (need + 3) // 4)
+                check(lib.dm_token_embed_bwd(dout.data_ptr(), int(dout.dtype == BF16), tokens.data_ptr(), dtable.data_ptr(), n, rows,
+                                             width, scale, padding, ws.data_ptr(), need, _stream()))
+        if sink is not None:
+            _grad_done(ctx.param)
+            return None, None, None, None, None
+        return dtable.to(dtype), None, None, None, None
+
+
+def token_embed(tokens, table, scale=1.0, padding_idx=None, dtype=BF16):
+    """scale * table[tokens], and the table's gradient by sorted tokens (fixed order of sums: bitwise reproducible).
+
+    tokens: whole numbers of any shape; table [rows, width] fp32; the result is tokens.shape + (width,) in `dtype` (bf16,
+    or fp32 for the embedding path). Tokens equal to padding_idx (negative: from the end) have no gradient; tokens outside
+    0 .. rows-1 give zeros and have none."""
+    _require_device(table, "token_embed")
+    if table.dim() != 2 or table.shape[0] == 0:
+        raise RuntimeError(f"token_embed: the table must be [rows, width], got {tuple(table.shape)}")
+    if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool or tokens.device != table.device:
+        raise RuntimeError(f"token_embed: tokens must be whole numbers on {table.device}, got {tokens.dtype} on {tokens.device}")
+    if dtype not in (BF16, torch.float32):
+        raise RuntimeError(f"token_embed: results are bf16 or fp32, not {dtype}")
+    rows = table.shape[0]
+    padding = -1 if padding_idx is None else int(padding_idx) + (rows if padding_idx < 0 else 0)
+    if padding_idx is not None and not 0 <= padding < rows:
+        raise RuntimeError(f"token_embed: padding_idx {padding_idx} is outside the table of {rows} rows")
+    if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+        tokens = tokens.to(torch.int64).contiguous()
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _TokenEmbedFn.apply(table, tokens, float(scale), padding, dtype)
+    return _embed_rows(tokens, f32c(table.detach()), float(scale), dtype)
 
 
 # ------------------------------------------------------------------------------------------------------------

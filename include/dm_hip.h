@@ -290,6 +290,58 @@ int dm_attention_bwd(const void* qkv, const void* out, const void* dout, const f
                      int H, int D, float scale, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
+ * Attention of each query over key blocks chosen for it (64 keys to a block), for sequences whose dense attention
+ * (above) is too long; the reference has no counterpart. Everything is bf16 but the fp32 statistics.
+ *   q [B][Lq][Hq][D], k, v [B][Lk][Hkv][D] by element strides {batch, position, head} (multiples of 8; D contiguous; the
+ *   parts of a packed qkv are such tensors), Hq a multiple of Hkv: query head h reads key head h / (Hq / Hkv);
+ *   D in {8, 16, 32, 64}; k_len: int [B], the valid keys of each sample (clamped to 0 .. Lk), or null: all Lk.
+ *   What lies behind the valid keys is never used, whatever it holds.
+ * nblk = ceil(Lk / 64) below; the last block of a sample may be partly valid.
+ * Results are bitwise reproducible and do not depend on the batch a sample is in. */
+typedef struct dm_block_desc {
+  int B, Lq, Lk, Hq, Hkv, D;
+  int top;      /* blocks a query names, 1 .. 64 */
+  float scale;  /* of q . k */
+  long q_stride[3], k_stride[3], v_stride[3];
+  long dq_stride[3], dk_stride[3], dv_stride[3];   /* backward only */
+} dm_block_desc;
+
+/* keys bf16 [B][Hkv][nblk][D]: the mean of each block's valid keys (zero where it has none), summed in 64 bits */
+int dm_block_keys(const dm_block_desc* d, const void* k, const int* k_len, void* keys, void* stream);
+/* blocks int [B][Hq][Lq][top]: the `top` blocks with a valid key of the highest q . keys, in ascending order, -1 behind
+ * the last where there are fewer. The scores are compared as 64-bit sums of the bf16 products; ties go to the lower
+ * block, NaN counts as -infinity. */
+int dm_block_select(const dm_block_desc* d, const void* q, const void* keys, const int* k_len, int* blocks, void* stream);
+/* out bf16 [B][Lq][Hq][D] = softmax over the valid keys of the blocks that `blocks` names for a query (any order; a
+ * repeated block counts once, numbers outside 0 .. nblk-1 name none), times v. A query without a key gets zeros.
+ * For the backward call: out_lo bf16, what the rounding of out lost; lse fp32 [B][Hq][Lq] (natural log; -infinity without
+ * a key); mask, the list as bits. out_lo and lse may be null. mask: dm_block_attention_mask_bytes(d, whether a backward call will read it), 16-byte aligned;
+ * null where that is 0. */
+size_t dm_block_attention_mask_bytes(const dm_block_desc* d, int for_backward);
+int dm_block_attention_fwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
+                           const int* k_len, void* out, void* out_lo, float* lse, void* mask, void* stream);
+/* dq, dk, dv bf16 by their strides, written (keys that no query attended get zeros), from what the forward call was
+ * given and wrote. ws: dm_block_attention_bwd_ws_bytes, 16-byte aligned, contents irrelevant. */
+size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d);
+int dm_block_attention_bwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
+                           const int* k_len, const void* mask, const void* out, const void* out_lo, const float* lse,
+                           const void* dout, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Rows of an embedding table by token: out[i] = scale * table[tokens[i]], i < n (the general form of the class table
+ * below: any number of tokens and rows). table fp32 [rows][width]; out fp32, or bf16 with out_bf16. A token outside
+ * 0 .. rows-1 gives zeros. Pointers need their element's alignment only (16-byte aligned ones and widths that are
+ * multiples of 4 run faster). */
+int dm_token_embed(const float* table, const int64_t* tokens, void* out, int out_bf16, long n, long rows, int width,
+                   float scale, void* stream);
+/* dtable[t] += scale * sum of dout[i] over tokens[i] == t (ACCUMULATES; fp32 sums of neighbours in a sorted order, no float
+ * atomics: bitwise reproducible). Tokens equal to `padding` (-1: none) or outside 0 .. rows-1 have no gradient.
+ * ws: dm_token_embed_bwd_ws_bytes, 16-byte aligned, contents irrelevant. */
+size_t dm_token_embed_bwd_ws_bytes(long n, long rows, int width);
+int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t* tokens, float* dtable, long n, long rows,
+                       int width, float scale, long padding, void* ws, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
  * Embedding path (fp32, tiny): modeling/embeddings.py:24-27 (sinusoidal encoding), :43-47 (MLP),
  * modeling/blocks.py:56-57 (emb_proj of SiLU(embedding)), modeling/unet.py:138-145 (class embedding add).
  */

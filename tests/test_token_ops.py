@@ -1,0 +1,472 @@
+"""Embedding rows by token (ops.token_embed) and attention over chosen key blocks (ops.block_keys, block_select,
+block_attention, sparse_attention), each against the definition in 64 bits.
+
+Tolerances count roundings. bf16 rounds by at most 2^-8 of a value (half a step), fp32 by 2^-24. An attention weight p is
+exact to 2^-12 (fp32 scores of at most 64 products, whose size the inputs here keep below 2^6, the fast exponential) and is
+rounded to bf16 where the matrix cores take it as an operand; so is ds. With sums of absolute terms in the reference:
+  out  2^-8 |out| + (2^-8 + 2^-12) sum p |v|
+  dv   2^-8 |dv|  + (2^-8 + 2^-12) sum p |do|
+  dq   2^-8 |dq|  + (2^-8 + 2^-11) sum |ds| |k| + scale * sum p |k| * E    (dk: the same over queries, with q)
+  E    the error of do . v - delta: 2^-15 |do| . |out| (delta's operand is a pair of bf16 numbers) + 2^-17 max |do| . |v|
+The table's gradient is an fp32 sum of n terms: n 2^-24 sum |terms|, at least two roundings."""
+import ctypes
+
+import pytest
+import torch
+
+from tests.parity import rel_err  # noqa: F401  (one place for the tests' path set-up)
+
+gpu = pytest.mark.gpu
+H = 2.0 ** -8
+BLOCK = 64
+
+
+def ops():
+    from dm_hip import ops as o
+    return o
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(torch.bfloat16)
+
+
+# -------------------------------------------------------------------------------------------------- references
+def lengths(k_len, B, L):
+    return torch.full((B,), L, device="cuda") if k_len is None else k_len.clamp(0, L)
+
+
+def ref_keys(k, k_len):
+    B, L, Hk, D = k.shape
+    n = -(-L // BLOCK)
+    out = torch.zeros(B, Hk, n, D, dtype=torch.float64, device="cuda")
+    for b, have in enumerate(lengths(k_len, B, L).tolist()):
+        for j in range(-(-have // BLOCK)):
+            out[b, :, j] = k[b, j * BLOCK:min(have, (j + 1) * BLOCK)].double().mean(0)
+    return out
+
+
+def ref_select(q, keys, top, k_len, L):
+    """the best blocks by (score, -block), one query after another as sorted lists"""
+    B, Lq, Hq, D = q.shape
+    score = torch.einsum("bihd,bhjd->bhij", q.double(), keys.double().repeat_interleave(Hq // keys.shape[1], 1))
+    score = torch.nan_to_num(score, nan=-float("inf"), posinf=float("inf"), neginf=-float("inf")).cpu()
+    out = torch.full((B, Hq, Lq, top), -1, dtype=torch.int32)
+    for b, have in enumerate(lengths(k_len, B, L).tolist()):
+        n = -(-have // BLOCK)
+        for h in range(Hq):
+            for i in range(Lq):
+                row = score[b, h, i, :n].tolist()
+                best = sorted(sorted(range(n), key=lambda j: (-row[j], j))[:top])
+                out[b, h, i, :len(best)] = torch.tensor(best, dtype=torch.int32)
+    return out.cuda()
+
+
+def ref_attention(q, k, v, blocks, scale, k_len, dout):
+    """(out, dq, dk, dv) in 64 bits and the bound of each, as in the module's text"""
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1:3]
+    G, n = Hq // Hkv, -(-Lk // BLOCK)
+    t = lambda x: x.double().transpose(1, 2)                                     # noqa: E731
+    have = lengths(k_len, B, Lk)
+    pos = torch.arange(Lk, device="cuda")
+    ok = (pos < have[:, None])[:, None, :, None]
+    qs, do = t(q), t(dout)
+    ks, vs = (torch.where(ok, t(x), 0.0).repeat_interleave(G, 1) for x in (k, v))
+    seen = torch.zeros(B, Hq, Lq, n, dtype=torch.bool, device="cuda")
+    for c in range(blocks.shape[3]):
+        j = blocks[..., c].long()
+        good = (j >= 0) & (j < n)
+        seen |= good[..., None] & (torch.arange(n, device="cuda") == j[..., None])
+    seen = seen.repeat_interleave(BLOCK, 3)[..., :Lk] & ok.transpose(2, 3)
+    s = torch.where(seen, torch.matmul(qs, ks.transpose(2, 3)) * scale, -float("inf"))
+    p = torch.where(seen.any(-1, keepdim=True), torch.softmax(s, -1), 0.0)
+    out = torch.matmul(p, vs)
+    dp = torch.matmul(do, vs.transpose(2, 3))
+    ds = p * (dp - (do * out).sum(-1, keepdim=True)) * scale
+    back = lambda x: x.transpose(1, 2)                                           # noqa: E731
+    keys = lambda x: x.view(B, Hkv, G, Lk, D).sum(2).transpose(1, 2)             # noqa: E731
+    T = lambda x: x.transpose(2, 3)                                              # noqa: E731
+    dq, dk, dv = torch.matmul(ds, ks), torch.matmul(T(ds), qs), torch.matmul(T(p), do)
+    E = 2.0 ** -15 * (do.abs() * out.abs()).sum(-1, keepdim=True) + 2.0 ** -17 * torch.where(seen, torch.matmul(do.abs(), T(vs.abs())), 0.0).amax(-1, keepdim=True)
+    w, e = ds.abs() * (H + 2.0 ** -11), scale * p * E
+    tiny = 1e-30
+    return ((back(out), back(H * out.abs() + (H + 2.0 ** -12) * torch.matmul(p, vs.abs()) + tiny)),
+            (back(dq), back(H * dq.abs() + torch.matmul(w + e, ks.abs()) + tiny)),
+            (keys(dk), H * keys(dk).abs() + keys(torch.matmul(T(w + e), qs.abs())) + tiny),
+            (keys(dv), H * keys(dv).abs() + (H + 2.0 ** -12) * keys(torch.matmul(T(p), do.abs())) + tiny))
+
+
+def within(name, got, want, bound):
+    over = (got.double() - want).abs() / bound
+    assert bool(torch.isfinite(got.double()).all()), f"{name}: not finite"
+    assert float(over.max()) <= 1.0, f"{name}: {float(over.max()):.3g} of the bound at {int(over.argmax())}"
+
+
+def some_blocks(g, B, Hq, Lq, n, top):
+    """any list a caller may hand over: repeats, -1 and numbers that are no block among them"""
+    b = torch.randint(-1, n + 1, (B, Hq, Lq, top), generator=g, device="cuda", dtype=torch.int32)
+    b[torch.rand(B, Hq, Lq, generator=g, device="cuda") < 0.1] = -1   # queries without a block
+    return b
+
+
+# -------------------------------------------------------------------------------------------------- choice of blocks
+@gpu
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", [
+    (1, 1, 1, 1, 1, 8, 1, False),
+    (2, 5, 63, 2, 1, 16, 3, False),
+    (2, 7, 64, 4, 4, 8, 2, False),
+    (3, 70, 65, 2, 2, 32, 1, True),
+    (3, 65, 1000, 6, 3, 64, 5, True),
+    (1, 130, 4200, 2, 1, 64, 16, False),     # more than 64 blocks
+    (2, 33, 9000, 2, 2, 8, 64, True),
+    (1, 3, 300, 40, 40, 16, 9, False),       # more heads than one workgroup's 64 vectors hold; top above the block count
+])
+def test_block_choice(B, Lq, Lk, Hq, Hkv, D, top, ragged):
+    g = gen(1)
+    q, k = randn(g, B, Lq, Hq, D), randn(g, B, Lk, Hkv, D)
+    k_len = torch.tensor([Lk // 2, 0, Lk + 5], dtype=torch.int32, device="cuda")[:B] if ragged else None
+    if ragged:
+        for b in range(B):
+            k[b, min(int(k_len[b]), Lk):] = float("nan")   # padding is never read as a value
+    keys = ops().block_keys(k, k_len)
+    want = ref_keys(k, k_len)
+    assert bool(((keys.double() - want).abs() <= H * want.abs()).all())
+    assert torch.equal(ops().block_select(q, keys, top, k_len), ref_select(q, keys, top, k_len, Lk))
+
+
+@gpu
+def test_block_choice_ties_and_values_that_are_no_numbers():
+    g = gen(2)
+    q, k = randn(g, 1, 40, 1, 16), randn(g, 1, 640, 1, 16)
+    k[:, 128:192] = k[:, 448:512]            # two equal blocks
+    k[:, 256:320] = 0
+    k[:, 576:] = 0
+    k[0, 200, 0, 3] = float("inf")
+    k[0, 330, 0, 3] = float("nan")
+    q[0, 0] = 0                              # every score is equal (or no number)
+    q[0, 1, 0, 2] = float("nan")
+    q[0, 2, 0, 3] = float("-inf")
+    q[0, 3] = 1e38
+    q[0, 4] *= 1e-30
+    for top in (1, 2, 5, 10):
+        keys = ops().block_keys(k)
+        assert torch.equal(ops().block_select(q, keys, top), ref_select(q, keys, top, None, 640))
+
+
+@gpu
+def test_block_choice_decides_differences_that_32_bits_cannot_hold():
+    # scores that differ by one part in 2^30: a large common product and a small one that differs
+    q = torch.zeros(1, 3, 1, 8, device="cuda", dtype=torch.bfloat16)
+    q[..., 0], q[..., 1] = 1024.0, 1.0
+    keys = torch.zeros(1, 1, 100, 8, device="cuda", dtype=torch.bfloat16)
+    keys[..., 0] = 1024.0
+    keys[0, 0, :, 1] = 2.0 ** -10 * torch.arange(100, device="cuda") * torch.where(torch.arange(100, device="cuda") % 2 == 0, 1, -1)
+    got = ops().block_select(q, keys, 3)
+    assert got[0, 0].tolist() == [[94, 96, 98]] * 3
+
+
+# -------------------------------------------------------------------------------------------------- attention
+CASES = [
+    # B, Lq, Lk, Hq, Hkv, D, top, ragged
+    (1, 1, 1, 1, 1, 8, 1, False),
+    (2, 1, 200, 4, 2, 64, 3, True),
+    (1, 3, 64, 1, 1, 32, 1, False),
+    (2, 63, 63, 2, 2, 16, 2, False),
+    (3, 65, 129, 4, 2, 8, 2, True),
+    (2, 200, 777, 6, 2, 16, 4, True),
+    (1, 513, 1025, 2, 2, 32, 5, False),
+    (2, 700, 1500, 4, 1, 64, 6, True),
+    (1, 1100, 640, 3, 3, 64, 10, False),
+    (1, 140, 5000, 2, 1, 64, 20, False),
+    (4, 16, 320, 16, 16, 8, 3, False),
+]
+
+
+@gpu
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", CASES)
+def test_block_attention(B, Lq, Lk, Hq, Hkv, D, top, ragged):
+    g = gen(3)
+    q, k, v, do = randn(g, B, Lq, Hq, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lq, Hq, D)
+    k_len = torch.tensor([Lk - 1, 0, Lk // 3], dtype=torch.int32, device="cuda")[:B] if ragged else None
+    if ragged:
+        for b in range(B):
+            k[b, int(k_len[b]):], v[b, int(k_len[b]):] = float("nan"), float("inf")
+    blocks = some_blocks(g, B, Hq, Lq, -(-Lk // BLOCK), top)
+    scale = 1.3 * D ** -0.5
+    ref = ref_attention(q, k, v, blocks, scale, k_len, do)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = ops().block_attention(*leaves, blocks, scale, k_len)
+    grads = torch.autograd.grad(out, leaves, do)
+    for name, got, (want, bound) in zip(("out", "dq", "dk", "dv"), (out, *grads), ref):
+        within(name, got, want, bound)
+    within("out without gradients", ops().block_attention(q, k, v, blocks, scale, k_len), *ref[0])
+
+
+@gpu
+def test_block_attention_of_one_sharp_weight():
+    """One key takes (almost) all the weight: ds is a small difference of large numbers."""
+    g = gen(4)
+    q, k, v, do = (randn(g, 1, 300, 2, 16) for _ in range(4))
+    q *= 12
+    blocks = torch.randint(0, 5, (1, 2, 300, 2), generator=g, device="cuda", dtype=torch.int32)
+    ref = ref_attention(q, k, v, blocks, 0.25, None, do)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = ops().block_attention(*leaves, blocks, 0.25)
+    for name, got, (want, bound) in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do)), ref):
+        within(name, got, want, bound)
+
+
+@gpu
+def test_block_attention_gradient_against_differences():
+    g = gen(5)
+    q, k, v, do = randn(g, 1, 70, 2, 16), randn(g, 1, 150, 1, 16), randn(g, 1, 150, 1, 16), randn(g, 1, 70, 2, 16)
+    blocks = some_blocks(g, 1, 2, 70, 3, 2)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    grads = torch.autograd.grad(ops().block_attention(*leaves, blocks, 0.25), leaves, do)
+    # central differences of the 64-bit definition along random directions, h^2 error below 2^-12 of the slope
+    for x, got in enumerate(grads):
+        u = torch.randn(leaves[x].shape, generator=g, device="cuda", dtype=torch.float64)
+        h = 2.0 ** -9
+        side = []
+        for sign in (1, -1):
+            moved = [t.double() for t in (q, k, v)]
+            moved[x] = moved[x] + sign * h * u
+            side.append((ref_attention(*moved, blocks, 0.25, None, do)[0][0] * do.double()).sum())
+        slope = float((side[0] - side[1]) / (2 * h))
+        bound = ref_attention(q, k, v, blocks, 0.25, None, do)[x + 1][1]
+        assert abs(float((got.double() * u).sum()) - slope) <= float((bound * u.abs()).sum()) + 2.0 ** -10 * abs(slope)
+
+
+@gpu
+def test_block_attention_reads_strided_tensors_in_place_and_copies_others():
+    g = gen(6)
+    B, L, Hh, D = 2, 150, 3, 16
+    qkv = randn(g, B, L, 3, Hh, D)
+    q, k, v = qkv.unbind(2)
+    blocks = some_blocks(g, B, Hh, L, 3, 2)
+    want = ops().block_attention(q.contiguous(), k.contiguous(), v.contiguous(), blocks)
+    assert torch.equal(ops().block_attention(q, k, v, blocks), want)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    assert torch.equal(ops().block_attention(*heads_first, blocks), want)
+    odd = torch.empty(B * L * Hh * D + 1, device="cuda", dtype=torch.bfloat16)[1:].view(B, L, Hh, D)   # rows off 16 bytes
+    assert torch.equal(ops().block_attention(q, odd.copy_(k), v, blocks), want)
+    assert torch.equal(ops().block_attention(q.float(), k.float(), v.float(), blocks), want)
+    # one value for every head and position: its gradient is the sum over both
+    one = randn(g, B, 1, 1, D).requires_grad_(True)
+    full = one.detach().expand(B, L, Hh, D).clone().requires_grad_(True)
+    do = randn(g, B, L, Hh, D)
+    a, = torch.autograd.grad(ops().block_attention(q, k, one.expand(B, L, Hh, D), blocks), one, do)
+    b, = torch.autograd.grad(ops().block_attention(q, k, full, blocks), full, do)
+    assert torch.equal(a, b.sum((1, 2), keepdim=True)) or rel_err(a.float().cpu(), b.float().sum((1, 2), keepdim=True).cpu()) < 2 * H
+
+
+@gpu
+@pytest.mark.parametrize("B,Lq,Lk", [(0, 3, 70), (2, 0, 70), (2, 3, 0)])
+def test_block_attention_of_nothing(B, Lq, Lk):
+    mk = lambda L: torch.full((B, L, 2, 16), float("nan"), device="cuda", dtype=torch.bfloat16, requires_grad=True)  # noqa: E731
+    q, k, v = mk(Lq), mk(Lk), mk(Lk)
+    blocks = torch.zeros(B, 2, Lq, 3, dtype=torch.int32, device="cuda")
+    out = ops().block_attention(q, k, v, blocks)
+    assert out.shape == q.shape and not bool(out.any())
+    for g_, x in zip(torch.autograd.grad(out, (q, k, v), torch.ones_like(out)), (q, k, v)):
+        assert g_.shape == x.shape and not bool(g_.any())
+    keys = ops().block_keys(k)
+    assert keys.shape == (B, 2, -(-Lk // 64), 16)
+    picked = ops().block_select(q, keys, 3)
+    assert picked.shape == (B, 2, Lq, 3) and bool((picked == -1).all() or Lk)
+
+
+@gpu
+@pytest.mark.parametrize("B,L,Hh,D,top", [(2, 130, 4, 8, 1), (1, 1024, 2, 64, 4), (3, 64, 5, 16, 2), (2, 1, 2, 32, 1)])
+def test_sparse_attention_packed(B, L, Hh, D, top):
+    g = gen(7)
+    qkv = randn(g, B, L, 3 * Hh * D)
+    do = randn(g, B, L, Hh * D)
+    q, k, v = qkv.view(B, L, 3, Hh, D).unbind(2)
+    blocks = ops().block_select(q, ops().block_keys(k), top)
+    assert torch.equal(blocks, ref_select(q, ops().block_keys(k), top, None, L))
+    leaf = qkv.clone().requires_grad_(True)
+    out = ops().sparse_attention(leaf, Hh, D, top)
+    (dqkv,) = torch.autograd.grad(out, leaf, do)
+    ref = ref_attention(q, k, v, blocks, D ** -0.5, None, do.view(B, L, Hh, D))
+    parts = dqkv.view(B, L, 3, Hh, D).unbind(2)
+    for name, got, (want, bound) in zip(("out", "dq", "dk", "dv"), (out.view(B, L, Hh, D), *parts), ref):
+        within(name, got, want, bound)
+    if top * 64 >= L:   # every block: the dense operator's result, both rounded
+        dense = ops().attention(qkv, Hh, D).view(B, L, Hh, D)
+        within("dense", dense, *(ref[0][0], 2 * ref[0][1]))
+
+
+@gpu
+def test_block_attention_same_bits_whatever_the_batch():
+    g = gen(8)
+    q, k, v, do = (randn(g, 3, 600, 4, 64) for _ in range(4))
+    blocks = some_blocks(g, 3, 4, 600, 10, 3)
+
+    def run(sl):
+        leaves = [x[sl].clone().requires_grad_(True) for x in (q, k, v)]
+        out = ops().block_attention(*leaves, blocks[sl])
+        return [out.detach(), *torch.autograd.grad(out, leaves, do[sl])]
+    whole = run(slice(0, 3))
+    for a, b in zip(whole, run(slice(0, 3))):
+        assert torch.equal(a, b)
+    for a, b in zip(whole, run(slice(1, 2))):
+        assert torch.equal(a[1:2], b)
+
+
+# -------------------------------------------------------------------------------------------------- embedding
+@gpu
+@pytest.mark.parametrize("n,rows,width,padding,out,scale", [
+    (1, 1, 1, None, "float32", 1.0),
+    (3, 5, 7, 4, "bfloat16", 3.0),
+    (256, 11, 512, 10, "float32", 1.0),
+    (1000, 300, 33, -1, "float32", 0.5),
+    (2048, 256, 20, None, "bfloat16", 1.0),
+    (2049, 257, 64, 0, "float32", -2.0),
+    (5000, 70000, 12, 3, "bfloat16", 1.0),      # three sort passes
+    (30000, 2, 8, None, "float32", 1.0),        # two runs over nearly every chunk
+    (70000, 900, 260, 1, "bfloat16", 22.0),     # the longer chunks of large calls
+    (400, 50, 1500, None, "float32", 1.0),      # more features than one workgroup takes
+])
+def test_token_embed(n, rows, width, padding, out, scale):
+    g = gen(9)
+    dtype = getattr(torch, out)
+    table = torch.randn(rows, width, generator=g, device="cuda")
+    tokens = (torch.rand(n, generator=g, device="cuda", dtype=torch.float64) ** 3 * rows).long().clamp(max=rows - 1)
+    if n > 100:
+        tokens[::17] = -1          # no tokens of the table
+        tokens[5::29] = rows
+        tokens[7] = 2 ** 40
+    ok = (tokens >= 0) & (tokens < rows)
+    leaf = table.clone().requires_grad_(True)
+    got = ops().token_embed(tokens, leaf, scale, padding, dtype)
+    half = H if dtype == torch.bfloat16 else 2.0 ** -24
+    want = torch.where(ok[:, None], table.double()[tokens.clamp(0, rows - 1)] * scale, 0.0)
+    assert got.dtype == dtype and bool(((got.double() - want).abs() <= 2 * 2.0 ** -24 * want.abs() + half * want.abs()).all())
+    assert torch.equal(got, ops().token_embed(tokens, table, scale, padding, dtype))
+    dout = torch.randn(n, width, generator=g, device="cuda").to(dtype)
+    (grad,) = torch.autograd.grad(got, leaf, dout)
+    pad = None if padding is None else padding % rows
+    keep = ok if pad is None else ok & (tokens != pad)
+    term = dout.double()[keep] * scale
+    ref = torch.zeros(rows, width, dtype=torch.float64, device="cuda").index_add_(0, tokens[keep], term)
+    size = torch.zeros_like(ref).index_add_(0, tokens[keep], term.abs())
+    count = torch.zeros(rows, dtype=torch.float64, device="cuda").index_add_(0, tokens[keep], torch.ones_like(tokens[keep], dtype=torch.float64))
+    assert bool(((grad.double() - ref).abs() <= (count[:, None] + 2) * 2.0 ** -24 * size).all())
+    (again,) = torch.autograd.grad(ops().token_embed(tokens, leaf, scale, padding, dtype), leaf, dout)
+    assert torch.equal(grad, again)
+
+
+@gpu
+def test_token_embed_shapes_types_and_an_empty_call():
+    g = gen(10)
+    table = torch.randn(9, 6, generator=g, device="cuda", requires_grad=True)
+    t = torch.randint(0, 9, (4, 5), generator=g, device="cuda", dtype=torch.int32)
+    out = ops().token_embed(t.t(), table, dtype=torch.float32)
+    assert torch.equal(out, table.detach()[t.t().long()])
+    out.backward(torch.ones_like(out))
+    assert torch.equal(table.grad.sum(1), 6.0 * torch.bincount(t.flatten().long(), minlength=9))
+    none = ops().token_embed(torch.empty(0, 3, dtype=torch.int64, device="cuda"), table)
+    assert none.shape == (0, 3, 6) and not bool(torch.autograd.grad(none, table, torch.empty_like(none))[0].any())
+    half = table.detach().to(torch.bfloat16).requires_grad_(True)
+    (gr,) = torch.autograd.grad(ops().token_embed(t, half), half, torch.ones(4, 5, 6, device="cuda", dtype=torch.bfloat16))
+    assert gr.dtype == torch.bfloat16
+    at_odd = torch.randn(9 * 6 + 1, generator=g, device="cuda")[1:].view(9, 6)   # 4-byte aligned rows
+    assert torch.equal(ops().token_embed(t, at_odd, dtype=torch.float32), at_odd[t.long()])
+
+
+@gpu
+def test_token_embed_gradient_accumulates_into_the_arena():
+    o = ops()
+    g = gen(11)
+    table = torch.nn.Parameter(torch.randn(20, 8, generator=g, device="cuda"))
+    t = torch.randint(0, 20, (100,), generator=g, device="cuda")
+    dout = torch.randn(100, 8, generator=g, device="cuda")
+    (want,) = torch.autograd.grad(o.token_embed(t, table, dtype=torch.float32), table, dout)
+    table.grad = torch.ones_like(table)
+    ready = []
+    o.DIRECT_GRADS, o.GRAD_READY = True, ready.append
+    try:
+        o.token_embed(t, table, dtype=torch.float32).backward(dout)
+    finally:
+        o.DIRECT_GRADS, o.GRAD_READY = False, None
+    assert len(ready) == 1 and ready[0] is table
+    assert bool(((table.grad - 1 - want).abs() <= 2.0 ** -23 * (1 + want.abs())).all())
+
+
+# -------------------------------------------------------------------------------------------------- refusals (no GPU needed)
+def test_refusals_of_tensors_on_the_cpu():
+    o = ops()
+    x, t = torch.zeros(1, 2, 1, 8, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    for call in (lambda: o.block_keys(x), lambda: o.block_select(x, x, 1), lambda: o.sparse_attention(x[:, :, 0], 1, 8, 1),
+                 lambda: o.block_attention(x, x, x, torch.zeros(1, 1, 2, 1, dtype=torch.int32)), lambda: o.token_embed(t, torch.zeros(3, 4))):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+def test_refusals_of_the_c_abi():
+    """Argument checks come before anything touches the device, and report through dm_last_error."""
+    from dm_hip import BlockDesc, lib
+    p = ctypes.c_void_p(4096)
+
+    def desc(**kw):
+        d = BlockDesc(1, 64, 64, 2, 1, 16, 4, 1.0)
+        for s in ("q_stride", "k_stride", "v_stride", "dq_stride", "dk_stride", "dv_stride"):
+            getattr(d, s)[:] = [2048, 32, 16]
+        for k, v in kw.items():
+            if isinstance(v, list):
+                getattr(d, k)[:] = v
+            else:
+                setattr(d, k, v)
+        return ctypes.byref(d)
+
+    for kw, code, text in [(dict(D=24), 2, "head dim"), (dict(D=128), 2, "head dim"), (dict(top=0), 2, "top"), (dict(top=65), 2, "top"),
+                           (dict(Hq=3, Hkv=2), 2, "evenly"), (dict(Lk=0), 2, "positive"), (dict(B=-1), 2, "positive"),
+                           (dict(B=70000), 2, "65535"), (dict(k_stride=[2048, 36, 16]), 1, "multiples of 8")]:
+        assert lib.dm_block_keys(desc(**kw), p, None, p, None) == code
+        assert text in lib.dm_last_error().decode()
+    assert lib.dm_block_keys(None, p, None, p, None) == 1
+    assert lib.dm_block_keys(desc(), None, None, p, None) == 1
+    assert lib.dm_block_keys(desc(), ctypes.c_void_p(4100), None, p, None) == 1
+    assert lib.dm_block_select(desc(q_stride=[2048, 33, 16]), p, p, None, p, None) == 1
+    assert lib.dm_block_select(desc(), p, p, None, None, None) == 1
+    assert lib.dm_block_attention_fwd(desc(), p, p, p, None, None, p, None, None, None, None) == 1
+    assert lib.dm_block_attention_bwd(desc(), p, p, p, p, None, p, p, p, p, p, p, p, p, p, 8, None) == 1
+    assert "workspace" in lib.dm_last_error().decode()
+    assert lib.dm_block_attention_mask_bytes(desc(D=3), 1) == 0
+    assert lib.dm_token_embed(p, p, p, 0, 5, 0, 4, 1.0, None) == 2
+    assert lib.dm_token_embed(p, p, p, 0, 2 ** 31, 9, 4, 1.0, None) == 2
+    assert lib.dm_token_embed(p, p, p, 0, 5, 9, 0, 1.0, None) == 2
+    assert lib.dm_token_embed(p, None, p, 0, 5, 9, 4, 1.0, None) == 1
+    assert lib.dm_token_embed(None, None, None, 0, 0, 9, 4, 1.0, None) == 0
+    assert lib.dm_token_embed_bwd(p, 0, p, p, 5, 9, 4, 1.0, -1, p, 16, None) == 1
+    assert lib.dm_token_embed_bwd_ws_bytes(5, 9, -1) == 0
+
+
+@gpu
+def test_refusals():
+    o = ops()
+    z = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.bfloat16)          # noqa: E731
+    i = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.int32)             # noqa: E731
+    q, k = z(2, 5, 4, 16), z(2, 70, 2, 16)
+    good = i(2, 4, 5, 3)
+    o.block_attention(q, k, k, good)
+    for bad in [lambda: o.block_attention(q[0], k, k, good), lambda: o.block_attention(z(2, 5, 4, 24), z(2, 70, 2, 24), z(2, 70, 2, 24), good),
+                lambda: o.block_attention(q, z(1, 70, 2, 16), z(1, 70, 2, 16), good), lambda: o.block_attention(q, k, z(2, 71, 2, 16), good),
+                lambda: o.block_attention(q, z(2, 70, 3, 16), z(2, 70, 3, 16), good), lambda: o.block_attention(q, k, k, good.long()),
+                lambda: o.block_attention(q, k, k, i(2, 5, 4, 3)), lambda: o.block_attention(q, k, k, i(2, 4, 5, 65)),
+                lambda: o.block_attention(q, k, k, i(2, 4, 5, 0)), lambda: o.block_attention(q, k, k, good.cpu()),
+                lambda: o.block_attention(q, k, k, good, k_len=torch.ones(2, device="cuda")),
+                lambda: o.block_attention(q, k, k, good, k_len=i(3)), lambda: o.block_attention(q, k, k, good, k_len=torch.ones(2, dtype=torch.int32)),
+                lambda: o.block_select(q, z(2, 3, 2, 16), 2), lambda: o.block_select(q, z(2, 2, 2, 8), 2), lambda: o.block_select(q, o.block_keys(k), 0),
+                lambda: o.sparse_attention(z(2, 5, 48), 2, 16, 1), lambda: o.sparse_attention(z(2, 5, 72), 1, 24, 1),
+                lambda: o.sparse_attention(z(2, 5, 48), 1, 16, 65),
+                lambda: o.token_embed(torch.zeros(3, device="cuda"), torch.zeros(3, 4, device="cuda")),
+                lambda: o.token_embed(i(3), torch.zeros(12, device="cuda")), lambda: o.token_embed(i(3), torch.zeros(3, 4, device="cuda"), dtype=torch.float16),
+                lambda: o.token_embed(i(3), torch.zeros(3, 4, device="cuda"), padding_idx=3), lambda: o.token_embed(i(3).cpu(), torch.zeros(3, 4, device="cuda"))]:
+        with pytest.raises(RuntimeError):
+            bad()
