@@ -13,6 +13,8 @@
 // few keys, ds is a small difference of do . v and delta, and the rounding of out alone would be as large. No kernel adds with float atomics: results do not depend on scheduling.
 #include "dm_common.h"
 
+extern int g_dm_block_pool;
+
 namespace {
 
 constexpr int BLK = 64;
@@ -333,87 +335,616 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
   if (lane < LPR) *(bf16x8_t*)(a.dq + b * a.dqb + i * a.dql + h * a.dqh + c) = dm_pack8(dq);
 }
 
-// dk and dv of one block a workgroup: its keys and values stay in registers, the rows that chose it are dealt to the
-// waves, whose sums are added in wave order
+// ---------------------------------------------------------------------------------------------------------------
+// The matrix-core form. A workgroup owns a POOL of P rows of one (sample, key head) and walks the blocks that any of
+// them chose, in order. A block's keys and values are staged in LDS once for the pool; the pool's rows that chose it
+// are packed into tiles of 16, so that a matrix instruction works on 16 rows that all want the block however the choices are
+// scattered (16 neighbouring rows would share few blocks: with 8 of 64 chosen at random a tile of neighbours has to
+// visit 56). A tile is dealt to a wave; what a row accumulates (its output, maximum and sum, or its dq) lives in LDS in fp32, because
+// the next block packs it into another tile. Rows of one block are disjoint and blocks are separated by barriers, so
+// a row's sums run in block order: the same bits every time.
+//
+// Products are formed transposed, S^T = K Q^T: a lane then holds 4 keys x 4 tiles of ONE row (lane & 15), the row's
+// maximum and sum are two lane swaps away, and exp(S^T) is in the register layout that the second product takes as its
+// right operand (its left operand, V^T or K^T, is read by transposing LDS reads in the same order of keys).
 template <int D>
-__global__ __launch_bounds__(256) void dkv_row_kernel(Args a, int ngroups) {
-  constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
-  __shared__ float acc[2][BLK][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  const int n0 = valid_keys(a.k_len, b, a.Lk) - j * BLK;
-  const int c = (lane % LPR) * 8, key = lane / LPR;
-  const float sc = a.scale * LOG2E;
-  const bf16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + (long)j * BLK * a.k.sl + c;
-  const bf16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + (long)j * BLK * a.v.sl + c;
-  const bf16x8_t none = {};
-  bf16x8_t kk[NI], vv[NI];
-  float dk[NI][8], dv[NI][8];
+struct Geo {
+  static constexpr int DV = D < 16 ? 16 : D;           // features of a row in LDS, zeros behind D
+  static constexpr int ROWB = DV * 2, KV_BYTES = BLK * ROWB;
+  static constexpr int KS = D <= 16 ? 1 : D / 32;      // matrix instructions (of 16 or 32 features) to a score
+  static constexpr int DT = DV / 16;                   // 16-feature tiles of a row
+  static constexpr int OC = DV / 4;                    // 16-byte pieces of an fp32 row
+};
+// Byte offset of 16-byte piece c of bf16 row r: 32-byte units are exchanged by row such that both the 16-byte reads (16
+// rows, one piece) and the transposing reads (4 groups of 4 rows, one unit) meet every bank equally often.
+template <int D>
+__device__ __forceinline__ int lds_at(int r, int c) {
+  if constexpr (D == 64) return r * 128 + (((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) << 4);
+  else if constexpr (D == 32) return r * 64 + (((((c >> 1) ^ ((r >> 1) & 1)) << 1) | (c & 1)) << 4);
+  else return r * 32 + (c << 4);
+}
+// float offset of 4-feature piece c of fp32 row r
+template <int D>
+__device__ __forceinline__ int acc_at(int r, int c) {
+  if constexpr (D == 64) return r * 64 + ((c ^ (r & 15)) << 2);
+  else if constexpr (D == 32) return r * 32 + ((c ^ (r & 7)) << 2);
+  else return r * 16 + (c << 2);
+}
+
+// 4 consecutive rows (row0 + 4 (lane >> 4) ...) of one feature (16 dt + (lane & 15)) for every lane
+template <int D>
+__device__ __forceinline__ bf16x4_t read_tr(const char* base, int row0, int dt, int lane) {
+  typedef __attribute__((address_space(3))) bf16x4_t* lds_ptr;
+  const int i = lane & 15, row = row0 + 4 * (lane >> 4) + (i >> 2);
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_ptr)(base + lds_at<D>(row, dt * 2 + ((i >> 1) & 1)) + (i & 1) * 8));
+}
+__device__ __forceinline__ bf16x8_t join4(bf16x4_t a, bf16x4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// operand of a product over features: the row's KS pieces of 8 (or, up to 16 features, its piece of 4)
+template <int D>
+struct Frag {
+  bf16x8_t x[Geo<D>::KS];
+  // p: the row, g = lane >> 4
+  __device__ __forceinline__ void load(const bf16_t* p, int g) {
+    if constexpr (D <= 16) {
+      const bf16x4_t z = {}, v = D == 16 || g < 2 ? *(const bf16x4_t*)(p + g * 4) : z;
+      x[0] = join4(v, z);
+    } else {
 #pragma unroll
-  for (int u = 0; u < NI; ++u) {
-    const int pos = u * KPI + key;
-    kk[u] = pos < n0 ? *(const bf16x8_t*)(kp + pos * a.k.sl) : none;
-    vv[u] = pos < n0 ? *(const bf16x8_t*)(vp + pos * a.v.sl) : none;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dk[u][e] = dv[u][e] = 0.f;
+      for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const bf16x8_t*)(p + s * 32 + g * 8);
+    }
   }
-  for (int rg = wave; rg < ngroups; rg += 4) {
-    const unsigned long long w = a.mask[((long)bh * ngroups + rg) * a.nblk + j];
-    unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)w), hi = __builtin_amdgcn_readfirstlane((unsigned)(w >> 32));
-    unsigned long long bits = ((unsigned long long)hi << 32) | lo;
-    if (n0 <= 0) bits = 0;
-    while (bits) {
-      const long r = (long)rg * 64 + __builtin_ctzll(bits);
-      bits &= bits - 1;
-      const long i = r / a.G;
-      const int h = hk * a.G + (int)(r - i * a.G);
-      const long row = ((long)b * a.Hq + h) * a.Lq + i;
-      const float lse = a.lse[row], ls = lse * LOG2E, delta = a.delta[row];
-      if (lse == -INFINITY) continue;
-      float q[8], go[8];
-      dm_unpack8(*(const bf16x8_t*)(a.q.p + b * a.q.sb + i * a.q.sl + h * a.q.sh + c), q);
-      dm_unpack8(*(const bf16x8_t*)(a.go + (((long)b * a.Lq + i) * a.Hq + h) * D + c), go);
+  __device__ __forceinline__ void zero() {
+    const bf16x8_t z = {};
 #pragma unroll
-      for (int u = 0; u < NI; ++u) {
-        float x[8], y[8], s = 0.f, dp = 0.f;
-        dm_unpack8(kk[u], x);
-        dm_unpack8(vv[u], y);
+    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = z;
+  }
+  __device__ __forceinline__ void from_lds(const char* base, int row, int g) {
+    if constexpr (D <= 16) {
+      const bf16x4_t z = {};
+      x[0] = join4(*(const bf16x4_t*)(base + lds_at<D>(row, g >> 1) + (g & 1) * 8), z);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { s += q[e] * x[e]; dp += go[e] * y[e]; }
-        s = group_sum<LPR>(s) * sc;
-        dp = group_sum<LPR>(dp);
-        const float p = __builtin_amdgcn_exp2f(s - ls), ds = p * (dp - delta) * a.scale;
+      for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const bf16x8_t*)(base + lds_at<D>(row, s * 4 + g));
+    }
+  }
+};
+template <int D>
+__device__ __forceinline__ f32x4_t dot_frag(const Frag<D>& a, const Frag<D>& b) {
+  f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (D <= 16) {
+    typedef __attribute__((ext_vector_type(4))) short half_t;
+    const bf16x4_t a4 = __builtin_shufflevector(a.x[0], a.x[0], 0, 1, 2, 3), b4 = __builtin_shufflevector(b.x[0], b.x[0], 0, 1, 2, 3);
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(half_t, a4), __builtin_bit_cast(half_t, b4), c, 0, 0, 0);
+  } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { dk[u][e] += ds * q[e]; dv[u][e] += p * go[e]; }
+    for (int s = 0; s < Geo<D>::KS; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.x[s], b.x[s], c, 0, 0, 0);
+    return c;
+  }
+}
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48 (the lanes that hold one row)
+__device__ __forceinline__ float row_max(float x) {
+  unsigned u = __builtin_bit_cast(unsigned, x);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__builtin_bit_cast(float, (unsigned)a[0]), __builtin_bit_cast(float, (unsigned)a[1]));
+  u = __builtin_bit_cast(unsigned, x);
+  a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)a[0]), __builtin_bit_cast(float, (unsigned)a[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  unsigned u = __builtin_bit_cast(unsigned, x);
+  auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
+  u = __builtin_bit_cast(unsigned, x);
+  a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
+}
+
+// The walk over a pool's blocks: which come next, the rows that chose each (packed into `list`, one wave a group of 64
+// rows), and the staging of keys and values.
+template <int D, int P>
+struct Walk {
+  static constexpr int NG = P / 64;                 // groups of 64 rows = waves
+  static constexpr int PIECES = 2 * BLK * D / 8;    // 16-byte pieces of a block's keys and values
+  static constexpr int PER = (PIECES + P - 1) / P;
+  const Args& a;
+  const int bh, b, hk, rg0, ngroups, tid, lane, wave, n, nb;
+  unsigned short (*list)[P];
+  unsigned long long bits = 0, mine = 0;
+  int base = 0, next0 = 0, pre = 0, tot = 0;
+  bf16x8_t kv[PER];
+  struct Hit { int j, n; };
+
+  __device__ __forceinline__ Walk(const Args& a_, int bh_, int tile, int ngroups_, unsigned short (*l)[P])
+      : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), rg0(tile * NG), ngroups(ngroups_), tid(threadIdx.x),
+        lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
+        nb((n + BLK - 1) / BLK), list(l) {}
+
+  // The next block that a row of the pool chose (j < 0: none) and its rows, into list[buf]. Lane x looks at block base + x.
+  __device__ __forceinline__ Hit advance(int buf) {
+    while (!bits) {
+      if (next0 >= nb) return Hit{-1, 0};
+      base = next0;
+      next0 += 64;
+      pre = tot = 0;
+      mine = 0;
+      const int j = base + lane;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const unsigned long long w = j < nb && rg0 + x < ngroups ? a.mask[((long)bh * ngroups + rg0 + x) * a.nblk + j] : 0;
+        if (x == wave) { mine = w; pre = tot; }
+        tot += __builtin_popcountll(w);
+      }
+      bits = __ballot(tot > 0);
+    }
+    const int x = __builtin_ctzll(bits);
+    bits &= bits - 1;
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)mine, x), hi = __builtin_amdgcn_readlane((unsigned)(mine >> 32), x);
+    const int first = __builtin_amdgcn_readlane(pre, x);
+    const int rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+    if (((lane < 32 ? lo : hi) >> (lane & 31)) & 1) list[buf][first + rank] = (unsigned short)(wave * 64 + lane);
+    return Hit{base + x, __builtin_amdgcn_readlane(tot, x)};
+  }
+
+  __device__ __forceinline__ long row_index(int row) const { return (long)rg0 * 64 + row; }
+  // position and head of a row
+  __device__ __forceinline__ void place(int row, long& i, int& h) const {
+    const unsigned r = (unsigned)row_index(row);
+    if (a.G == 1) { i = r; h = hk; }
+    else { const unsigned q = r / (unsigned)a.G; i = q; h = hk * a.G + (int)(r - q * a.G); }
+  }
+
+  __device__ __forceinline__ void fetch(int j) {   // block j's keys and values into registers
+    const bf16x8_t none = {};
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * P + tid, half = e >= PIECES / 2 ? 1 : 0, p = e - half * (PIECES / 2);
+      const int t = p / (D / 8), c = (p % (D / 8)) * 8;
+      const Rows& s = half ? a.v : a.k;
+      const long pos = (long)j * BLK + t;
+      kv[u] = e < PIECES && pos < n ? *(const bf16x8_t*)(s.p + b * s.sb + pos * s.sl + hk * s.sh + c) : none;
+    }
+  }
+  __device__ __forceinline__ void stage(char* kbuf, char* vbuf) const {
+    const bf16x8_t none = {};
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * P + tid, half = e >= PIECES / 2 ? 1 : 0, p = e - half * (PIECES / 2);
+      if (e >= PIECES) continue;
+      const int t = p / (D / 8), c = p % (D / 8);
+      char* to = half ? vbuf : kbuf;
+      *(bf16x8_t*)(to + lds_at<D>(t, c)) = kv[u];
+      if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+    }
+  }
+};
+
+__device__ __forceinline__ bool pool_of(int nbh, int ntiles, int& bh, int& tile) {
+  if ((nbh & 7) == 0) dm_xcd_tile(blockIdx.x, ntiles, bh, tile);   // one head's pools on one XCD: its keys and values stay in that L2
+  else { bh = blockIdx.x / ntiles; tile = blockIdx.x % ntiles; }
+  return bh < nbh;
+}
+
+template <int D, int P>
+__global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int ntiles) {
+  using GE = Geo<D>;
+  __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
+  __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
+  __shared__ float sm[P], sl[P], sr[P];   // maximum, sum of the weights, sum of the weights as rounded
+  __shared__ unsigned short list[3][P];
+  int bh, tile;
+  if (!pool_of(a.B * a.Hkv, ntiles, bh, tile)) return;
+  Walk<D, P> w(a, bh, tile, ngroups, list);
+  const int lane = w.lane, g = lane >> 4;
+  const float sc = a.scale * LOG2E;
+  auto cur = w.advance(0);
+  typename Walk<D, P>::Hit nxt{-1, 0};
+  if (cur.j >= 0) {
+    nxt = w.advance(1);
+    w.fetch(cur.j);
+    w.stage(kbuf, vbuf);
+  }
+  const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
+  const bf16_t one = (bf16_t)1.f;
+  const bf16x8_t ones = {one, one, one, one, one, one, one, one};
+  for (int e = w.tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
+  sm[w.tid] = -INFINITY;
+  sl[w.tid] = sr[w.tid] = 0.f;
+  __syncthreads();
+
+  auto load_q = [&](Frag<D>& f, const unsigned short* ls, int t, int count) {
+    const int li = t * 16 + (lane & 15);
+    long i;
+    int h;
+    w.place(ls[li < count ? li : t * 16], i, h);
+    f.load(a.q.p + w.b * a.q.sb + i * a.q.sl + h * a.q.sh, g);
+  };
+  Frag<D> qf, qn;
+  qf.zero();
+  qn.zero();
+  if (cur.j >= 0 && w.wave * 16 < cur.n) load_q(qf, list[0], w.wave, cur.n);
+  int buf = 0;
+  while (cur.j >= 0) {
+    const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+    typename Walk<D, P>::Hit nn{-1, 0};
+    if (nxt.j >= 0) {
+      w.fetch(nxt.j);
+      nn = w.advance(b2);
+      if (w.wave * 16 < nxt.n) load_q(qn, list[b1], w.wave, nxt.n);
+    }
+    const int n0 = w.n - cur.j * BLK;   // valid keys from this block on
+    for (int t = w.wave; t * 16 < cur.n; t += P / 64) {
+      if (t != w.wave) load_q(qf, list[buf], t, cur.n);
+      const int li = t * 16 + (lane & 15);
+      const bool live = li < cur.n;
+      const int row = list[buf][live ? li : t * 16];
+      float s[16];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        Frag<D> kf;
+        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
+        const f32x4_t c = dot_frag<D>(kf, qf);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kt * 4 + e] = c[e] * sc;
+      }
+      if (n0 < BLK) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) s[e] = -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+      const float m_old = sm[row], m_new = fmaxf(m_old, row_max(mx)), at = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m_old - at);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(s[e] - at);
+        sum += s[e];
+      }
+      sum = row_sum(sum);
+      // The weights are rounded to bf16 as the matrix instruction's operand. The output is divided by the sum of the
+      // ROUNDED weights (one more product, with ones), so that it stays an average of values: a rounding then counts only
+      // with the value's distance from the output. The saved statistic is of the unrounded ones.
+      bf16x8_t p[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) p[u] = dm_pack8(s + u * 8);
+      const float r_old = sr[row] * alpha;
+      f32x4_t rs = {r_old, r_old, r_old, r_old};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
+      if (live && g == 0) {
+        sl[row] = sl[row] * alpha + sum;
+        sr[row] = rs[0];
+        sm[row] = m_new;
+      }
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        float* at_o = acc + acc_at<D>(row, dt * 4 + g);
+        f32x4_t c = *(const f32x4_t*)at_o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(read_tr<D>(vbuf, u * 32, dt, lane), read_tr<D>(vbuf, u * 32 + 16, dt, lane)), p[u], c, 0, 0, 0);
+        if (live) *(f32x4_t*)at_o = c;
       }
     }
+    __syncthreads();
+    if (nxt.j >= 0) w.stage(kbuf, vbuf);
+    __syncthreads();
+    cur = nxt;
+    nxt = nn;
+    qf = qn;
+    buf = b1;
   }
-  for (int w = 0; w < 4; ++w) {
-    if (wave == w) {
+  constexpr int PC = D / 8;
+  for (int e = w.tid; e < P * PC; e += P) {
+    const int row = e / PC, c = e % PC;
+    if (w.row_index(row) >= (long)a.Lq * a.G) break;
+    long i;
+    int h;
+    w.place(row, i, h);
+    const float l = sl[row], inv = 1.0f / sr[row];
+    float f[8], lo[8];
+    *(f32x4_t*)f = *(const f32x4_t*)(acc + acc_at<D>(row, c * 2));
+    *(f32x4_t*)(f + 4) = *(const f32x4_t*)(acc + acc_at<D>(row, c * 2 + 1));
 #pragma unroll
-      for (int u = 0; u < NI; ++u)
+    for (int x = 0; x < 8; ++x) f[x] = l == 0.f ? 0.f : f[x] * inv;
+    const bf16x8_t y = dm_pack8(f);
+    const long at = (((long)w.b * a.Lq + i) * a.Hq + h) * D + c * 8;
+    *(bf16x8_t*)(a.out + at) = y;
+    if (a.out_lo) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float* pk = &acc[0][u * KPI + key][c + e];
-          float* pv = &acc[1][u * KPI + key][c + e];
-          *pk = (w ? *pk : 0.f) + dk[u][e];
-          *pv = (w ? *pv : 0.f) + dv[u][e];
-        }
+      for (int x = 0; x < 8; ++x) lo[x] = f[x] - (float)y[x];
+      *(bf16x8_t*)(a.out_lo + at) = dm_pack8(lo);
+    }
+    if (a.lse && c == 0) a.lse[((long)w.b * a.Hq + h) * a.Lq + i] = l == 0.f ? -INFINITY : sm[row] * LN2 + logf(l);
+  }
+}
+
+// dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end.
+template <int D, int P>
+__global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int ntiles) {
+  using GE = Geo<D>;
+  __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
+  __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
+  __shared__ float s_lse[P], s_delta[P];
+  __shared__ unsigned short list[3][P];
+  int bh, tile;
+  if (!pool_of(a.B * a.Hkv, ntiles, bh, tile)) return;
+  Walk<D, P> w(a, bh, tile, ngroups, list);
+  const int lane = w.lane, g = lane >> 4;
+  const float sc = a.scale * LOG2E;
+  auto cur = w.advance(0);
+  typename Walk<D, P>::Hit nxt{-1, 0};
+  if (cur.j >= 0) {
+    nxt = w.advance(1);
+    w.fetch(cur.j);
+    w.stage(kbuf, vbuf);
+  }
+  const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
+  for (int e = w.tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
+  constexpr int PC = D / 8;
+  for (int e = w.tid; e < P * PC; e += P) {   // (a row's PC lanes are neighbours: P is a multiple of PC)
+    const int row = e / PC, c = e % PC;
+    const bool in = w.row_index(row) < (long)a.Lq * a.G;
+    long i = 0;
+    int h = 0;
+    if (in) w.place(row, i, h);
+    const long at = (((long)w.b * a.Lq + i) * a.Hq + h) * D + c * 8, lrow = ((long)w.b * a.Hq + h) * a.Lq + i;
+    float go[8], o[8], lo[8], delta = 0.f;
+    if (in) {
+      dm_unpack8(*(const bf16x8_t*)(a.go + at), go);
+      dm_unpack8(*(const bf16x8_t*)(a.o + at), o);
+      dm_unpack8(*(const bf16x8_t*)(a.o_lo + at), lo);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) delta += go[x] * (o[x] + lo[x]);
+    }
+    delta = group_sum<PC>(delta);
+    if (c == 0) {
+      const float lse = in ? a.lse[lrow] : 0.f;
+      s_delta[row] = delta;
+      s_lse[row] = lse == -INFINITY ? INFINITY : lse * LOG2E;   // no key: every weight becomes zero
+      if (in) a.delta[lrow] = delta;
+    }
+  }
+  __syncthreads();
+
+  auto load_rows = [&](Frag<D>& fq, Frag<D>& fo, const unsigned short* ls, int t, int count) {
+    const int li = t * 16 + (lane & 15);
+    long i;
+    int h;
+    w.place(ls[li < count ? li : t * 16], i, h);
+    fq.load(a.q.p + w.b * a.q.sb + i * a.q.sl + h * a.q.sh, g);
+    fo.load(a.go + (((long)w.b * a.Lq + i) * a.Hq + h) * D, g);
+  };
+  Frag<D> qf, qn, of, on;
+  qf.zero(); qn.zero(); of.zero(); on.zero();
+  if (cur.j >= 0 && w.wave * 16 < cur.n) load_rows(qf, of, list[0], w.wave, cur.n);
+  int buf = 0;
+  while (cur.j >= 0) {
+    const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+    typename Walk<D, P>::Hit nn{-1, 0};
+    if (nxt.j >= 0) {
+      w.fetch(nxt.j);
+      nn = w.advance(b2);
+      if (w.wave * 16 < nxt.n) load_rows(qn, on, list[b1], w.wave, nxt.n);
+    }
+    const int n0 = w.n - cur.j * BLK;
+    for (int t = w.wave; t * 16 < cur.n; t += P / 64) {
+      if (t != w.wave) load_rows(qf, of, list[buf], t, cur.n);
+      const int li = t * 16 + (lane & 15);
+      const bool live = li < cur.n;
+      const int row = list[buf][live ? li : t * 16];
+      const float lse = s_lse[row], delta = s_delta[row];
+      float ds[16];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        Frag<D> kf, vf;
+        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
+        vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
+        const f32x4_t s = dot_frag<D>(kf, qf), dp = dot_frag<D>(vf, of);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - lse) * (dp[e] - delta);
+      }
+      if (n0 < BLK) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) ds[e] = 0.f;
+      }
+      bf16x8_t p[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) p[u] = dm_pack8(ds + u * 8);
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        float* at_o = acc + acc_at<D>(row, dt * 4 + g);
+        f32x4_t c = *(const f32x4_t*)at_o;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(read_tr<D>(kbuf, u * 32, dt, lane), read_tr<D>(kbuf, u * 32 + 16, dt, lane)), p[u], c, 0, 0, 0);
+        if (live) *(f32x4_t*)at_o = c;
+      }
     }
     __syncthreads();
+    if (nxt.j >= 0) w.stage(kbuf, vbuf);
+    __syncthreads();
+    cur = nxt;
+    nxt = nn;
+    qf = qn;
+    of = on;
+    buf = b1;
   }
+  for (int e = w.tid; e < P * PC; e += P) {
+    const int row = e / PC, c = e % PC;
+    if (w.row_index(row) >= (long)a.Lq * a.G) break;
+    long i;
+    int h;
+    w.place(row, i, h);
+    float f[8];
+    *(f32x4_t*)f = *(const f32x4_t*)(acc + acc_at<D>(row, c * 2));
+    *(f32x4_t*)(f + 4) = *(const f32x4_t*)(acc + acc_at<D>(row, c * 2 + 1));
+#pragma unroll
+    for (int x = 0; x < 8; ++x) f[x] *= a.scale;
+    *(bf16x8_t*)(a.dq + w.b * a.dqb + i * a.dql + h * a.dqh + c * 8) = dm_pack8(f);
+  }
+}
+
+// dk and dv of one block, four waves. The rows that chose it are packed into a list, 4096 rows at a time, and dealt to the
+// waves in tiles of 32; every wave sums all 64 keys over its own rows in registers, and the four sums are added in wave
+// order. Scores are formed as S = Q K^T here: a lane holds 4 rows x 2 tiles of ONE key, which is the layout that dv =
+// P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
+constexpr int LIST = 4096;
+template <int D>
+__global__ __launch_bounds__(256, 2) void dkv_kernel(Args a, int ngroups) {
+  using GE = Geo<D>;
+  constexpr int TILE_BYTES = 32 * GE::ROWB;
+  __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
+  __shared__ __attribute__((aligned(16))) char rows[4][2][TILE_BYTES];    // q and do of a wave's tile; at the end the sums
+  __shared__ __attribute__((aligned(16))) float stat[4][2][32];           // lse, delta
+  __shared__ unsigned short list[LIST];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+  const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int n0 = valid_keys(a.k_len, b, a.Lk) - j * BLK;
+  const float sc = a.scale * LOG2E;
+  const bf16x8_t none = {};
+  if (n0 > 0) {
+    for (int e = tid; e < 2 * BLK * D / 8; e += 256) {
+      const int half = e >= BLK * D / 8 ? 1 : 0, p = e - half * (BLK * D / 8), t = p / (D / 8), c = p % (D / 8);
+      const Rows& s = half ? a.v : a.k;
+      char* to = half ? vbuf : kbuf;
+      *(bf16x8_t*)(to + lds_at<D>(t, c)) = t < n0 ? *(const bf16x8_t*)(s.p + b * s.sb + ((long)j * BLK + t) * s.sl + hk * s.sh + c * 8) : none;
+      if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+    }
+  }
+  f32x4_t dk[4][GE::DT], dv[4][GE::DT];
+#pragma unroll
+  for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+    for (int dt = 0; dt < GE::DT; ++dt) dk[kt][dt] = dv[kt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  char *qb = rows[wave][0], *ob = rows[wave][1];
+  float *st_lse = stat[wave][0], *st_delta = stat[wave][1];
+  for (int rg0 = 0; rg0 < ngroups && n0 > 0; rg0 += LIST / 64) {
+    const unsigned long long word = rg0 + lane < ngroups ? a.mask[((long)bh * ngroups + rg0 + lane) * a.nblk + j] : 0;
+    int inc = __builtin_popcountll(word);
+    const int own = inc;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += up;
+    }
+    const int count = __builtin_amdgcn_readlane(inc, 63), before = inc - own;
+    __syncthreads();   // the list's last use is over
+    for (int x = wave; x < LIST / 64; x += 4) {
+      const unsigned lo = __builtin_amdgcn_readlane((unsigned)word, x), hi = __builtin_amdgcn_readlane((unsigned)(word >> 32), x);
+      const int first = __builtin_amdgcn_readlane(before, x);
+      const int rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+      if (((lane < 32 ? lo : hi) >> (lane & 31)) & 1) list[first + rank] = (unsigned short)(x * 64 + lane);
+    }
+    __syncthreads();
+    for (int t = wave; t * 32 < count; t += 4) {
+      // a lane's two rows: 16 mt + (lane & 15)
+      Frag<D> qf[2], of[2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const int li = t * 32 + mt * 16 + (lane & 15);
+        qf[mt].zero();
+        of[mt].zero();
+        float lse = INFINITY, delta = 0.f;
+        if (li < count) {
+          const unsigned r = (unsigned)(rg0 * 64 + list[li]);
+          const unsigned i = a.G == 1 ? r : r / (unsigned)a.G;
+          const int h = hk * a.G + (int)(r - i * a.G);
+          const long lrow = ((long)b * a.Hq + h) * a.Lq + i;
+          qf[mt].load(a.q.p + b * a.q.sb + (long)i * a.q.sl + h * a.q.sh, g);
+          of[mt].load(a.go + (((long)b * a.Lq + i) * a.Hq + h) * D, g);
+          lse = a.lse[lrow];
+          lse = lse == -INFINITY ? INFINITY : lse * LOG2E;
+          delta = a.delta[lrow];
+        }
+        const int row = mt * 16 + (lane & 15);
+        if (g == 0) { st_lse[row] = lse; st_delta[row] = delta; }
+        if constexpr (D <= 16) {
+          *(bf16x4_t*)(qb + lds_at<D>(row, g >> 1) + (g & 1) * 8) = __builtin_shufflevector(qf[mt].x[0], qf[mt].x[0], 0, 1, 2, 3);
+          *(bf16x4_t*)(ob + lds_at<D>(row, g >> 1) + (g & 1) * 8) = __builtin_shufflevector(of[mt].x[0], of[mt].x[0], 0, 1, 2, 3);
+        } else {
+#pragma unroll
+          for (int s = 0; s < GE::KS; ++s) {
+            *(bf16x8_t*)(qb + lds_at<D>(row, s * 4 + g)) = qf[mt].x[s];
+            *(bf16x8_t*)(ob + lds_at<D>(row, s * 4 + g)) = of[mt].x[s];
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes, read by its other lanes
+      bf16x8_t qt[GE::DT], ot[GE::DT];
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        qt[dt] = join4(read_tr<D>(qb, 0, dt, lane), read_tr<D>(qb, 16, dt, lane));
+        ot[dt] = join4(read_tr<D>(ob, 0, dt, lane), read_tr<D>(ob, 16, dt, lane));
+      }
+      f32x4_t lse4[2], delta4[2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        lse4[mt] = *(const f32x4_t*)(st_lse + mt * 16 + g * 4);
+        delta4[mt] = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
+      }
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        Frag<D> kf, vf;
+        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
+        vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
+        float p[8], ds[8];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - lse4[mt][e]);
+            ds[mt * 4 + e] = p[mt * 4 + e] * (dp[e] - delta4[mt][e]);
+          }
+        }
+        const bf16x8_t pt = dm_pack8(p), dst = dm_pack8(ds);
+#pragma unroll
+        for (int dt = 0; dt < GE::DT; ++dt) {
+          dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pt, ot[dt], dv[kt][dt], 0, 0, 0);
+          dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dst, qt[dt], dk[kt][dt], 0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+  // the four waves' sums, in wave order: [key][feature] fp32 in the tiles' memory (4 x 2 x 32 rows hold 64 rows twice)
+  float* sum = (float*)&rows[0][0][0];
+  constexpr int HALF = BLK * GE::DV;
+  for (int x = 0; x < 4; ++x) {
+    __syncthreads();
+    if (wave == x) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int dt = 0; dt < GE::DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = (kt * 16 + g * 4 + e) * GE::DV + dt * 16 + (lane & 15);
+            sum[at] = (x ? sum[at] : 0.f) + dk[kt][dt][e];
+            sum[HALF + at] = (x ? sum[HALF + at] : 0.f) + dv[kt][dt][e];
+          }
+    }
+  }
+  __syncthreads();
   const int in = min(BLK, a.Lk - j * BLK);
-  for (int e = threadIdx.x; e < BLK * D / 8; e += 256) {
-    const int t = e / LPR, d = (e % LPR) * 8;
+  for (int e = tid; e < BLK * D / 8; e += 256) {
+    const int t = e / (D / 8), d = (e % (D / 8)) * 8;
     if (t >= in) break;
     const long pos = (long)j * BLK + t;
     const bool live = t < n0;   // positions behind the last valid key: zero
     float f[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? acc[0][t][d + x] : 0.f;
+    for (int x = 0; x < 8; ++x) f[x] = live ? sum[t * GE::DV + d + x] * a.scale : 0.f;
     *(bf16x8_t*)(a.dk + b * a.dkb + pos * a.dkl + hk * a.dkh + d) = dm_pack8(f);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? acc[1][t][d + x] : 0.f;
+    for (int x = 0; x < 8; ++x) f[x] = live ? sum[HALF + t * GE::DV + d + x] : 0.f;
     *(bf16x8_t*)(a.dv + b * a.dvb + pos * a.dvl + hk * a.dvh + d) = dm_pack8(f);
   }
 }
@@ -436,6 +967,14 @@ int check_strides(const char* who, const char* name, const long* s) {
   return DM_OK;
 }
 int blocks_of(const dm_block_desc* d) { return (d->Lk + BLK - 1) / BLK; }
+// Rows of a pool (0: one query a workgroup). Large pools fill tiles better and read keys and values less often; small ones
+// give more workgroups where there are few rows.
+int pool_rows(const dm_block_desc* d) {
+  if (g_dm_block_pool) return g_dm_block_pool == 1 ? 0 : g_dm_block_pool;
+  const long rows = (long)d->Lq * (d->Hq / d->Hkv), heads = (long)d->B * d->Hkv;
+  if (rows < 16) return 0;
+  return heads * dm_cdiv(rows, 512) >= 256 ? 512 : 128;
+}
 int groups_of(const dm_block_desc* d) { return dm_cdiv((long)d->Lq * (d->Hq / d->Hkv), 64); }
 
 Rows rows_of(const void* p, const long* s) { return Rows{(const bf16_t*)p, s[0], s[1], s[2]}; }
@@ -489,7 +1028,7 @@ extern "C" int dm_block_select(const dm_block_desc* d, const void* q, const void
 }
 
 extern "C" size_t dm_block_attention_mask_bytes(const dm_block_desc* d, int for_backward) {
-  if (check_desc("dm_block_attention_mask_bytes", d) || !for_backward) return 0;
+  if (check_desc("dm_block_attention_mask_bytes", d) || (!for_backward && !pool_rows(d))) return 0;
   return (size_t)d->B * d->Hkv * groups_of(d) * blocks_of(d) * 8;
 }
 
@@ -504,15 +1043,23 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
     return rc;
   Args a = args_of(d);
   a.q = rows_of(q, d->q_stride); a.k = rows_of(k, d->k_stride); a.v = rows_of(v, d->v_stride);
-  a.blocks = blocks; a.k_len = k_len; a.out = (bf16_t*)out; a.out_lo = (bf16_t*)out_lo; a.lse = lse;
+  a.blocks = blocks; a.k_len = k_len; a.out = (bf16_t*)out; a.out_lo = (bf16_t*)out_lo; a.lse = lse; a.mask = (unsigned long long*)mask;
   hipStream_t st = (hipStream_t)stream;
+  const int pool = pool_rows(d), tiles = pool ? dm_cdiv((long)d->Lq * a.G, pool) : 0;
+  DM_REQUIRE(aligned(mask) || (!mask && !pool), DM_ERR_ARG, "%s: this shape needs a mask (dm_block_attention_mask_bytes), 16-byte aligned", who);
   if (mask) {
     hipLaunchKernelGGL(block_mask_kernel, dim3(groups_of(d), d->B * d->Hkv), dim3(256), 0, st, blocks, (unsigned long long*)mask, d->Lq,
                        d->Hq, a.G, d->top, a.nblk, groups_of(d));
     DM_CHECK_LAUNCH();
   }
   const long rows = (long)d->B * d->Hq * d->Lq;
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a));
+  const dim3 grid(d->B * d->Hkv * tiles);
+  switch (pool) {
+    case 0: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a)); break;
+    case 128: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 128>), grid, dim3(128), 0, st, a, groups_of(d), tiles)); break;
+    case 256: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 256>), grid, dim3(256), 0, st, a, groups_of(d), tiles)); break;
+    default: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 512>), grid, dim3(512), 0, st, a, groups_of(d), tiles)); break;
+  }
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -546,9 +1093,16 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   a.dvb = d->dv_stride[0]; a.dvl = d->dv_stride[1]; a.dvh = d->dv_stride[2];
   hipStream_t st = (hipStream_t)stream;
   const long rows = (long)d->B * d->Hq * d->Lq;
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows));
+  const int pool = pool_rows(d), tiles = pool ? dm_cdiv((long)d->Lq * a.G, pool) : 0;
+  const dim3 grid(d->B * d->Hkv * tiles);
+  switch (pool) {
+    case 0: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows)); break;
+    case 128: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 128>), grid, dim3(128), 0, st, a, groups_of(d), tiles)); break;
+    case 256: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 256>), grid, dim3(256), 0, st, a, groups_of(d), tiles)); break;
+    default: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 512>), grid, dim3(512), 0, st, a, groups_of(d), tiles)); break;
+  }
   DM_CHECK_LAUNCH();
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_row_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a, groups_of(d)));
+  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a, groups_of(d)));
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
