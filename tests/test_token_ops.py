@@ -127,6 +127,10 @@ def some_blocks(g, B, Hq, Lq, n, top):
     (1, 130, 4200, 2, 1, 64, 16, False),     # more than 64 blocks
     (2, 33, 9000, 2, 2, 8, 64, True),
     (1, 3, 300, 40, 40, 16, 9, False),       # more heads than one workgroup's 64 vectors hold; top above the block count
+    (1, 2, 70000, 1, 1, 8, 20, False),       # more blocks than are scored at a time, few queries
+    (1, 20, 70000, 1, 1, 8, 10, False),      # ... and more
+    (2, 9, 5000, 4, 2, 32, 30, True),
+    (1, 17, 5000, 2, 2, 16, 60, False),
 ])
 def test_block_choice(B, Lq, Lk, Hq, Hkv, D, top, ragged):
     g = gen(1)
@@ -161,15 +165,32 @@ def test_block_choice_ties_and_values_that_are_no_numbers():
 
 
 @gpu
-def test_block_choice_decides_differences_that_32_bits_cannot_hold():
+@pytest.mark.parametrize("scale_q,scale_k", [(1.0, 1.0), (2.0 ** 40, 2.0 ** -70), (2.0 ** -80, 2.0 ** -80), (2.0 ** 60, 2.0 ** 60)])
+@pytest.mark.parametrize("top", [1, 3, 8, 15, 25])
+def test_block_choice_among_near_ties(top, scale_q, scale_k):
+    """Summaries of few distinct values: many scores are equal, or differ by the last bits of a 32-bit sum."""
+    g = gen(12)
+    q = torch.randint(-3, 4, (1, 300, 2, 64), generator=g, device="cuda").to(torch.bfloat16) * scale_q
+    keys = torch.randint(-2, 3, (1, 2, 130, 64), generator=g, device="cuda").to(torch.bfloat16)
+    keys[:, :, ::3] += 2.0 ** -7 * torch.randint(-1, 2, (1, 2, 44, 64), generator=g, device="cuda").to(torch.bfloat16)
+    keys[:, :, 5:30] *= 0     # a run of equal ones
+    keys *= scale_k
+    want = ref_select(q, keys, top, None, 130 * 64)
+    assert torch.equal(ops().block_select(q, keys, top), want)
+    assert torch.equal(ops().block_select(q[:, :7], keys, top), want[:, :, :7])
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 40])   # fewer queries than a tile of 16 rows, and more
+def test_block_choice_decides_differences_that_32_bits_cannot_hold(n):
     # scores that differ by one part in 2^30: a large common product and a small one that differs
-    q = torch.zeros(1, 3, 1, 8, device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros(1, n, 1, 8, device="cuda", dtype=torch.bfloat16)
     q[..., 0], q[..., 1] = 1024.0, 1.0
     keys = torch.zeros(1, 1, 100, 8, device="cuda", dtype=torch.bfloat16)
     keys[..., 0] = 1024.0
     keys[0, 0, :, 1] = 2.0 ** -10 * torch.arange(100, device="cuda") * torch.where(torch.arange(100, device="cuda") % 2 == 0, 1, -1)
     got = ops().block_select(q, keys, 3)
-    assert got[0, 0].tolist() == [[94, 96, 98]] * 3
+    assert got[0, 0].tolist() == [[94, 96, 98]] * n
 
 
 # -------------------------------------------------------------------------------------------------- attention
