@@ -346,6 +346,16 @@ struct Frag {
       for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const bf16x8_t*)(p + s * 32 + g * 8);
     }
   }
+  // waits for the operand here and not behind younger loads (the compiler counts loads in order, and across branches all of them)
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int s = 0; s < Geo<D>::KS; ++s) asm volatile("" : "+v"(x[s]));
+  }
+  __device__ __forceinline__ void negate() {
+    typedef __attribute__((ext_vector_type(4))) unsigned bits_t;
+#pragma unroll
+    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = __builtin_bit_cast(bf16x8_t, __builtin_bit_cast(bits_t, x[s]) ^ 0x80008000u);
+  }
   __device__ __forceinline__ void zero() {
     const bf16x8_t z = {};
 #pragma unroll
@@ -615,12 +625,25 @@ struct Walk {
   unsigned long long bits = 0, mine = 0;
   int base = 0, next0 = 0, pre = 0, tot = 0;
   bf16x8_t kv[PER];
+  const bf16_t* src[PER];   // this thread's pieces of block 0, the distance of a block, their place in LDS
+  long step[PER];
+  int key[PER], to[PER];
   struct Hit { int j, n; };
 
   __device__ __forceinline__ Walk(const Args& a_, int bh_, int tile, int ngroups_, unsigned short (*l)[P])
       : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), rg0(tile * NG), ngroups(ngroups_), tid(threadIdx.x),
         lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
-        nb((n + BLK - 1) / BLK), list(l) {}
+        nb((n + BLK - 1) / BLK), list(l) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * P + tid, half = e >= PIECES / 2 ? 1 : 0, x = e - half * (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
+      const Rows& r = half ? a.v : a.k;
+      src[u] = r.p + b * r.sb + t * r.sl + hk * r.sh + c * 8;
+      step[u] = BLK * r.sl;
+      key[u] = e < PIECES ? t : 0x40000000;   // (no piece: behind every valid key)
+      to[u] = half * Geo<D>::KV_BYTES + lds_at<D>(t, c);
+    }
+  }
 
   // The next block that a row of the pool chose (j < 0: none) and its rows, into list[buf]. Lane x looks at block base + x.
   __device__ __forceinline__ Hit advance(int buf) {
@@ -648,6 +671,14 @@ struct Walk {
     return Hit{base + x, __builtin_amdgcn_readlane(tot, x)};
   }
 
+  // a row's place in a [..][positions][heads][D] tensor, in units of 8 features from the sample's first (0 behind the last row)
+  __device__ __forceinline__ unsigned offset(int row, long sl, long sh) const {
+    if (row_index(row) >= (long)a.Lq * a.G) return 0;
+    long i;
+    int h;
+    place(row, i, h);
+    return (unsigned)((i * sl + h * sh) >> 3);
+  }
   __device__ __forceinline__ long row_index(int row) const { return (long)rg0 * 64 + row; }
   // position and head of a row
   __device__ __forceinline__ void place(int row, long& i, int& h) const {
@@ -658,25 +689,17 @@ struct Walk {
 
   __device__ __forceinline__ void fetch(int j) {   // block j's keys and values into registers
     const bf16x8_t none = {};
+    const int left = n - j * BLK;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int e = u * P + tid, half = e >= PIECES / 2 ? 1 : 0, p = e - half * (PIECES / 2);
-      const int t = p / (D / 8), c = (p % (D / 8)) * 8;
-      const Rows& s = half ? a.v : a.k;
-      const long pos = (long)j * BLK + t;
-      kv[u] = e < PIECES && pos < n ? *(const bf16x8_t*)(s.p + b * s.sb + pos * s.sl + hk * s.sh + c) : none;
-    }
+    for (int u = 0; u < PER; ++u) kv[u] = key[u] < left ? *(const bf16x8_t*)(src[u] + j * step[u]) : none;
   }
-  __device__ __forceinline__ void stage(char* kbuf, char* vbuf) const {
+  __device__ __forceinline__ void stage(char* kvbuf) const {
     const bf16x8_t none = {};
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int e = u * P + tid, half = e >= PIECES / 2 ? 1 : 0, p = e - half * (PIECES / 2);
-      if (e >= PIECES) continue;
-      const int t = p / (D / 8), c = p % (D / 8);
-      char* to = half ? vbuf : kbuf;
-      *(bf16x8_t*)(to + lds_at<D>(t, c)) = kv[u];
-      if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+      if (PIECES < P * PER && key[u] >= 0x40000000) continue;
+      *(bf16x8_t*)(kvbuf + to[u]) = kv[u];
+      if constexpr (D == 8) *(bf16x8_t*)(kvbuf + to[u] + 16) = none;
     }
   }
 };
@@ -690,41 +713,44 @@ __device__ __forceinline__ bool pool_of(int nbh, int ntiles, int& bh, int& tile)
 template <int D, int P>
 __global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int ntiles) {
   using GE = Geo<D>;
-  __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
+  __shared__ __attribute__((aligned(16))) char kbuf[2 * GE::KV_BYTES];
+  char* const vbuf = kbuf + GE::KV_BYTES;
   __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
+  __shared__ unsigned rowoff[P];          // a row's place in q, in units of 8 features from the sample's first
   __shared__ float sm[P], sl[P], sr[P];   // maximum, sum of the weights, sum of the weights as rounded
   __shared__ unsigned short list[3][P];
   int bh, tile;
   if (!pool_of(a.B * a.Hkv, ntiles, bh, tile)) return;
   Walk<D, P> w(a, bh, tile, ngroups, list);
   const int lane = w.lane, g = lane >> 4;
-  const float sc = a.scale * LOG2E;
+  const float sc = a.scale * LOG2E, asc = fabsf(sc);   // (the sign of the scale goes to q: a maximum is scaled by the amount)
   auto cur = w.advance(0);
   typename Walk<D, P>::Hit nxt{-1, 0};
   if (cur.j >= 0) {
     nxt = w.advance(1);
     w.fetch(cur.j);
-    w.stage(kbuf, vbuf);
+    w.stage(kbuf);
   }
   const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
   const bf16_t one = (bf16_t)1.f;
   const bf16x8_t ones = {one, one, one, one, one, one, one, one};
   for (int e = w.tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
+  rowoff[w.tid] = w.offset(w.tid, a.q.sl, a.q.sh);
   sm[w.tid] = -INFINITY;
   sl[w.tid] = sr[w.tid] = 0.f;
   __syncthreads();
 
+  const bf16_t* const qbase = a.q.p + w.b * a.q.sb;
   auto load_q = [&](Frag<D>& f, const unsigned short* ls, int t, int count) {
     const int li = t * 16 + (lane & 15);
-    long i;
-    int h;
-    w.place(ls[li < count ? li : t * 16], i, h);
-    f.load(a.q.p + w.b * a.q.sb + i * a.q.sl + h * a.q.sh, g);
+    f.load(qbase + (size_t)rowoff[ls[li < count ? li : t * 16]] * 8, g);
+    if (sc < 0.f) f.negate();
   };
   Frag<D> qf, qn;
   qf.zero();
   qn.zero();
   if (cur.j >= 0 && w.wave * 16 < cur.n) load_q(qf, list[0], w.wave, cur.n);
+  qf.arrived();
   int buf = 0;
   while (cur.j >= 0) {
     const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
@@ -736,19 +762,32 @@ __global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int
     }
     const int n0 = w.n - cur.j * BLK;   // valid keys from this block on
     for (int t = w.wave; t * 16 < cur.n; t += P / 64) {
-      if (t != w.wave) load_q(qf, list[buf], t, cur.n);
+      if (t != w.wave) {
+        load_q(qf, list[buf], t, cur.n);
+        qf.arrived();
+      }
       const int li = t * 16 + (lane & 15);
       const bool live = li < cur.n;
       const int row = list[buf][live ? li : t * 16];
       float s[16];
+      {
+        Frag<D> kf[4];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        Frag<D> kf;
-        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
-        const f32x4_t c = dot_frag<D>(kf, qf);
+        for (int kt = 0; kt < 4; ++kt) kf[kt].from_lds(kbuf, kt * 16 + (lane & 15), g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[kt * 4 + e] = c[e] * sc;
+        for (int kt = 0; kt < 4; ++kt) *(f32x4_t*)(s + kt * 4) = dot_frag<D>(kf[kt], qf);
       }
+      // everything else that the tile reads from LDS is under way before the softmax
+      const float m_old = sm[row], l_old = sl[row], r_sum = sr[row];
+      f32x4_t o[GE::DT];
+      bf16x4_t vt[GE::DT][4];
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        o[dt] = *(const f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vt[dt][u] = read_tr<D>(vbuf, u * 16, dt, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       if (n0 < BLK) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -757,14 +796,18 @@ __global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int
       float mx = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-      const float m_old = sm[row], m_new = fmaxf(m_old, row_max(mx)), at = m_new == -INFINITY ? 0.f : m_new;
+      const float m_new = fmaxf(m_old, row_max(mx) * asc), at = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = __builtin_amdgcn_exp2f(m_old - at);
       float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(s[e] - at);
-        sum += s[e];
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * asc - at);
+      if (n0 < BLK) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) s[e] = 0.f;   // (a scale of zero times -infinity is no zero)
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum += s[e];
       sum = row_sum(sum);
       // The weights are rounded to bf16 as the matrix instruction's operand. The output is divided by the sum of the
       // ROUNDED weights (one more product, with ones), so that it stays an average of values: a rounding then counts only
@@ -772,33 +815,32 @@ __global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int
       bf16x8_t p[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) p[u] = dm_pack8(s + u * 8);
-      const float r_old = sr[row] * alpha;
+      const float r_old = r_sum * alpha;
       f32x4_t rs = {r_old, r_old, r_old, r_old};
 #pragma unroll
       for (int u = 0; u < 2; ++u) rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
       if (live && g == 0) {
-        sl[row] = sl[row] * alpha + sum;
+        sl[row] = l_old * alpha + sum;
         sr[row] = rs[0];
         sm[row] = m_new;
       }
 #pragma unroll
       for (int dt = 0; dt < GE::DT; ++dt) {
-        float* at_o = acc + acc_at<D>(row, dt * 4 + g);
-        f32x4_t c = *(const f32x4_t*)at_o;
+        f32x4_t c = o[dt];
 #pragma unroll
         for (int e = 0; e < 4; ++e) c[e] *= alpha;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(read_tr<D>(vbuf, u * 32, dt, lane), read_tr<D>(vbuf, u * 32 + 16, dt, lane)), p[u], c, 0, 0, 0);
-        if (live) *(f32x4_t*)at_o = c;
+        for (int u = 0; u < 2; ++u) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(vt[dt][2 * u], vt[dt][2 * u + 1]), p[u], c, 0, 0, 0);
+        if (live) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = c;
       }
     }
     __syncthreads();
-    if (nxt.j >= 0) w.stage(kbuf, vbuf);
+    if (nxt.j >= 0) w.stage(kbuf);
     __syncthreads();
     cur = nxt;
     nxt = nn;
     qf = qn;
+    qf.arrived();
     buf = b1;
   }
   constexpr int PC = D / 8;
@@ -830,8 +872,11 @@ __global__ __launch_bounds__(P) void attend_pool_kernel(Args a, int ngroups, int
 template <int D, int P>
 __global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int ntiles) {
   using GE = Geo<D>;
-  __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
+  __shared__ __attribute__((aligned(16))) char kbuf[2 * GE::KV_BYTES];
+  char* const vbuf = kbuf + GE::KV_BYTES;
   __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
+  __shared__ unsigned rowoff[P];          // a row's place in q, in units of 8 features from the sample's first
+  __shared__ unsigned gooff[P];           // ... and in the output's gradient
   __shared__ float s_lse[P], s_delta[P];
   __shared__ unsigned short list[3][P];
   int bh, tile;
@@ -844,10 +889,12 @@ __global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int nti
   if (cur.j >= 0) {
     nxt = w.advance(1);
     w.fetch(cur.j);
-    w.stage(kbuf, vbuf);
+    w.stage(kbuf);
   }
   const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
   for (int e = w.tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
+  rowoff[w.tid] = w.offset(w.tid, a.q.sl, a.q.sh);
+  gooff[w.tid] = w.offset(w.tid, (long)a.Hq * D, D);
   constexpr int PC = D / 8;
   for (int e = w.tid; e < P * PC; e += P) {   // (a row's PC lanes are neighbours: P is a multiple of PC)
     const int row = e / PC, c = e % PC;
@@ -874,17 +921,18 @@ __global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int nti
   }
   __syncthreads();
 
+  const bf16_t* const qbase = a.q.p + w.b * a.q.sb;
+  const bf16_t* const obase = a.go + (long)w.b * a.Lq * a.Hq * D;
   auto load_rows = [&](Frag<D>& fq, Frag<D>& fo, const unsigned short* ls, int t, int count) {
-    const int li = t * 16 + (lane & 15);
-    long i;
-    int h;
-    w.place(ls[li < count ? li : t * 16], i, h);
-    fq.load(a.q.p + w.b * a.q.sb + i * a.q.sl + h * a.q.sh, g);
-    fo.load(a.go + (((long)w.b * a.Lq + i) * a.Hq + h) * D, g);
+    const int li = t * 16 + (lane & 15), row = ls[li < count ? li : t * 16];
+    fq.load(qbase + (size_t)rowoff[row] * 8, g);
+    fo.load(obase + (size_t)gooff[row] * 8, g);
   };
   Frag<D> qf, qn, of, on;
   qf.zero(); qn.zero(); of.zero(); on.zero();
   if (cur.j >= 0 && w.wave * 16 < cur.n) load_rows(qf, of, list[0], w.wave, cur.n);
+  qf.arrived();
+  of.arrived();
   int buf = 0;
   while (cur.j >= 0) {
     const int b1 = buf == 2 ? 0 : buf + 1, b2 = b1 == 2 ? 0 : b1 + 1;
@@ -896,21 +944,41 @@ __global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int nti
     }
     const int n0 = w.n - cur.j * BLK;
     for (int t = w.wave; t * 16 < cur.n; t += P / 64) {
-      if (t != w.wave) load_rows(qf, of, list[buf], t, cur.n);
+      if (t != w.wave) {
+        load_rows(qf, of, list[buf], t, cur.n);
+        qf.arrived();
+        of.arrived();
+      }
       const int li = t * 16 + (lane & 15);
       const bool live = li < cur.n;
       const int row = list[buf][live ? li : t * 16];
       const float lse = s_lse[row], delta = s_delta[row];
       float ds[16];
+      Frag<D> kf[4], vf[4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
-        Frag<D> kf, vf;
-        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
-        vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
-        const f32x4_t s = dot_frag<D>(kf, qf), dp = dot_frag<D>(vf, of);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - lse) * (dp[e] - delta);
+        kf[kt].from_lds(kbuf, kt * 16 + (lane & 15), g);
+        vf[kt].from_lds(vbuf, kt * 16 + (lane & 15), g);
       }
+      f32x4_t s[4], dp[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        s[kt] = dot_frag<D>(kf[kt], qf);
+        dp[kt] = dot_frag<D>(vf[kt], of);
+      }
+      f32x4_t o[GE::DT];
+      bf16x4_t kt_[GE::DT][4];
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        o[dt] = *(const f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) kt_[dt][u] = read_tr<D>(kbuf, u * 16, dt, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[kt][e] * sc - lse) * (dp[kt][e] - delta);
       if (n0 < BLK) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -921,21 +989,21 @@ __global__ __launch_bounds__(P) void dq_pool_kernel(Args a, int ngroups, int nti
       for (int u = 0; u < 2; ++u) p[u] = dm_pack8(ds + u * 8);
 #pragma unroll
       for (int dt = 0; dt < GE::DT; ++dt) {
-        float* at_o = acc + acc_at<D>(row, dt * 4 + g);
-        f32x4_t c = *(const f32x4_t*)at_o;
+        f32x4_t c = o[dt];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(read_tr<D>(kbuf, u * 32, dt, lane), read_tr<D>(kbuf, u * 32 + 16, dt, lane)), p[u], c, 0, 0, 0);
-        if (live) *(f32x4_t*)at_o = c;
+        for (int u = 0; u < 2; ++u) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(kt_[dt][2 * u], kt_[dt][2 * u + 1]), p[u], c, 0, 0, 0);
+        if (live) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = c;
       }
     }
     __syncthreads();
-    if (nxt.j >= 0) w.stage(kbuf, vbuf);
+    if (nxt.j >= 0) w.stage(kbuf);
     __syncthreads();
     cur = nxt;
     nxt = nn;
     qf = qn;
     of = on;
+    qf.arrived();
+    of.arrived();
     buf = b1;
   }
   for (int e = w.tid; e < P * PC; e += P) {
@@ -1128,6 +1196,14 @@ int check_strides(const char* who, const char* name, const long* s) {
     DM_REQUIRE(s[i] % 8 == 0, DM_ERR_ARG, "%s: strides of %s must be multiples of 8 elements (rows are read 16 bytes at a time)", who, name);
   return DM_OK;
 }
+// rows are addressed inside a sample by 32-bit numbers of 8 features
+int check_span(const char* who, const dm_block_desc* d) {
+  const long* s = d->q_stride;
+  for (int i = 0; i < 3; ++i) DM_REQUIRE(s[i] >= 0, DM_ERR_ARG, "%s: negative stride of q", who);
+  DM_REQUIRE((d->Lq - 1) * s[1] + (d->Hq - 1) * s[2] < (1L << 35) && (long)d->Lq * d->Hq * d->D < (1L << 35), DM_ERR_SHAPE,
+             "%s: a sample of q spans more than 2^35 elements", who);
+  return DM_OK;
+}
 int blocks_of(const dm_block_desc* d) { return (d->Lk + BLK - 1) / BLK; }
 // Rows of a pool (0: one query a workgroup). Large pools fill tiles better and read keys and values less often; small ones
 // give more workgroups where there are few rows.
@@ -1210,7 +1286,7 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   if (rc) return rc;
   DM_REQUIRE(aligned(q) && aligned(k) && aligned(v) && aligned(out) && blocks, DM_ERR_ARG, "%s: null or misaligned pointer", who);
   if ((rc = check_strides(who, "q", d->q_stride)) || (rc = check_strides(who, "k", d->k_stride)) ||
-      (rc = check_strides(who, "v", d->v_stride)))
+      (rc = check_strides(who, "v", d->v_stride)) || (rc = check_span(who, d)))
     return rc;
   Args a = args_of(d);
   a.q = rows_of(q, d->q_stride); a.k = rows_of(k, d->k_stride); a.v = rows_of(v, d->v_stride);
@@ -1253,6 +1329,7 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
                                                           {"dq", d->dq_stride}, {"dk", d->dk_stride}, {"dv", d->dv_stride}};
   for (const auto& x : all)
     if ((rc = check_strides(who, x.n, x.s))) return rc;
+  if ((rc = check_span(who, d))) return rc;
   Args a = args_of(d);
   a.q = rows_of(q, d->q_stride); a.k = rows_of(k, d->k_stride); a.v = rows_of(v, d->v_stride);
   a.o = (const bf16_t*)out; a.o_lo = (const bf16_t*)out_lo; a.go = (const bf16_t*)dout;

@@ -94,8 +94,8 @@ def ref_attention(q, k, v, blocks, scale, k_len, dout):
     T = lambda x: x.transpose(2, 3)                                              # noqa: E731
     dq, dk, dv = torch.matmul(ds, ks), torch.matmul(T(ds), qs), torch.matmul(T(p), do)
     E = 2.0 ** -15 * (do.abs() * out.abs()).sum(-1, keepdim=True) + 2.0 ** -17 * torch.where(seen, torch.matmul(do.abs(), T(vs.abs())), 0.0).amax(-1, keepdim=True)
-    E = E + (H + 2.0 ** -12) * ds.abs().sum(-1, keepdim=True) / scale
-    w, e = ds.abs() * (H + 2.0 ** -11), scale * p * E
+    E = E + (H + 2.0 ** -12) * (p * (dp - (do * out).sum(-1, keepdim=True))).abs().sum(-1, keepdim=True)
+    w, e = ds.abs() * (H + 2.0 ** -11), abs(scale) * p * E
     tiny = 1e-30
     return ((back(out), back(H * out.abs() + (H + 2.0 ** -12) * torch.matmul(p, vs.abs()) + tiny)),
             (back(dq), back(H * dq.abs() + torch.matmul(w + e, ks.abs()) + tiny)),
@@ -250,6 +250,21 @@ def test_block_attention_of_one_sharp_weight(pool):
     ref = ref_attention(q, k, v, blocks, 0.25, None, do)
     leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
     out = ops().block_attention(*leaves, blocks, 0.25)
+    for name, got, (want, bound) in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do)), ref):
+        within(name, got, want, bound)
+
+
+@gpu
+@pytest.mark.parametrize("pool", [1, 128])
+@pytest.mark.parametrize("scale", [-0.4, 0.0])
+def test_block_attention_of_a_scale_that_is_not_positive(scale, pool):
+    rows_together(pool)
+    g = gen(13)
+    q, k, v, do = randn(g, 1, 90, 2, 16), randn(g, 1, 150, 1, 16), randn(g, 1, 150, 1, 16), randn(g, 1, 90, 2, 16)
+    blocks = some_blocks(g, 1, 2, 90, 3, 2)
+    ref = ref_attention(q, k, v, blocks, scale, None, do)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    out = ops().block_attention(*leaves, blocks, scale)
     for name, got, (want, bound) in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, leaves, do)), ref):
         within(name, got, want, bound)
 
