@@ -39,7 +39,6 @@ int g_dm_conv1x1_stream = 1;          // 1x1 stride-1 convolutions: streaming ke
 int g_dm_patch_direct = 1;           // 3x3 patch kernel: plain outputs leave the accumulator registers directly (0: through LDS, as the outputs with a GroupNorm epilogue do)
 int g_dm_gn_min_ppt = 4;             // single-pass GroupNorm: least pixels per thread (1, 2, 4, 8) where the image leaves 8 pixel lanes; 8x8 images: 128-thread workgroups of 4 pixels per thread instead of 512 x 1 (forward 10.0 -> 7.0 us, backward 14.1 -> 9.2 us at batch 128, 512 channels)
 int g_dm_gn_bwd16 = 1;               // 513..1024-pixel GroupNorm backward: 512 threads x 16 pixels (no spills) instead of 1024 x 8
-int g_dm_block_pool = 0;             // attention over chosen blocks: rows a workgroup works on together (128, 256, 512; 1: one query a workgroup; 0: by the shape)
 
 namespace {
 struct Switch { const char* key; int* value; int initial; };
@@ -52,7 +51,7 @@ const Switch kSwitches[] = {
   {"edge_mfma", &g_dm_edge_mfma, 1},             {"attn_mfma", &g_dm_attn_mfma, 1},
   {"timing_skip", &g_dm_timing_skip, 0},         {"timing_twice", &g_dm_timing_twice, 0},
   {"conv1x1_stream", &g_dm_conv1x1_stream, 1},   {"patch_direct", &g_dm_patch_direct, 1},
-  {"gn_min_ppt", &g_dm_gn_min_ppt, 4},           {"block_pool", &g_dm_block_pool, 0},
+  {"gn_min_ppt", &g_dm_gn_min_ppt, 4},
   {"gn_bwd16", &g_dm_gn_bwd16, 1},               {"conv_proj_fuse", &g_dm_conv_proj_fuse, 1},
 };
 const Switch* find_switch(const char* key) {
@@ -68,8 +67,6 @@ extern "C" int dm_config_set(const char* key, int value) {
   const Switch* s = find_switch(key);
   if (!s) return DM_ERR_ARG;
   if (s->value == &g_dm_wgrad_reduce_cap && value < 1) value = 1;
-  DM_REQUIRE(s->value != &g_dm_block_pool || value == 0 || value == 1 || value == 128 || value == 256 || value == 512, DM_ERR_ARG,
-             "dm_config_set: block_pool is 0, 1, 128, 256 or 512, not %d", value);
   *s->value = value;
   return DM_OK;
 }

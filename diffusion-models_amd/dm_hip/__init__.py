@@ -59,7 +59,7 @@ class WtItem(ctypes.Structure):
 
 class BlockDesc(ctypes.Structure):
     """dm_block_desc: attention over chosen key blocks."""
-    _fields_ = [(n, c_int) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top")] + [("scale", c_float)] + \
+    _fields_ = [(n, c_int) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top", "pool")] + [("scale", c_float)] + \
         [(n, c_long * 3) for n in ("q_stride", "k_stride", "v_stride", "dq_stride", "dk_stride", "dv_stride")]
 
 
@@ -101,7 +101,7 @@ _SIGNATURES = {
     "dm_attention_bwd": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, P]),
     "dm_block_keys": (c_int, [P] * 5),
     "dm_block_select": (c_int, [P] * 6),
-    "dm_block_attention_mask_bytes": (ctypes.c_size_t, [P, c_int]),
+    "dm_block_attention_plan_bytes": (ctypes.c_size_t, [P, c_int]),
     "dm_block_attention_fwd": (c_int, [P] * 11),
     "dm_block_attention_bwd_ws_bytes": (ctypes.c_size_t, [P]),
     "dm_block_attention_bwd": (c_int, [P] * 15 + [ctypes.c_size_t, P]),

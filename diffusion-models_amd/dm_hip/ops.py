@@ -844,6 +844,7 @@ def attention(qkv, n_heads, head_dim, scale=None):
 # Attention of each query over key blocks chosen for it, for sequences too long for `attention` above. Tensors are
 # [B, positions, heads, head_dim] (the parts of a packed qkv are read in place); BLOCK keys make a block.
 BLOCK = 64
+BLOCK_POOL = 0   # rows a workgroup works on together (dm_block_desc.pool); 0: by the shape
 _HERE = contextlib.nullcontext()
 
 
@@ -879,8 +880,8 @@ def _lengths(k_len, B, device, who):
     return k_len.contiguous()
 
 
-def _block_desc(B, Lq, Lk, Hq, Hkv, D, top, scale=1.0, q=None, k=None, v=None):
-    d = BlockDesc(B, Lq, Lk, Hq, Hkv, D, top, scale)
+def _block_desc(B, Lq, Lk, Hq, Hkv, D, top, scale=1.0, q=None, k=None, v=None, pool=None):
+    d = BlockDesc(B, Lq, Lk, Hq, Hkv, D, top, BLOCK_POOL if pool is None else pool, scale)
     for t, to in ((q, d.q_stride), (k, d.k_stride), (v, d.v_stride)):
         if t is not None:
             to[:] = t.stride()[:3]
@@ -944,21 +945,21 @@ def _block_forward(d, q, k, v, blocks, k_len, training):
     out = torch.empty((d.B, d.Lq, d.Hq, d.D), dtype=BF16, device=dev)
     out_lo = torch.empty_like(out) if training else None
     lse = torch.empty((d.B, d.Hq, d.Lq), dtype=torch.float32, device=dev) if training else None
-    n = lib.dm_block_attention_mask_bytes(ctypes.byref(d), int(training))
-    mask = torch.empty(n // 8, dtype=torch.int64, device=dev) if n else None
+    n = lib.dm_block_attention_plan_bytes(ctypes.byref(d), int(training))
+    plan = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     check(lib.dm_block_attention_fwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
-                                     out.data_ptr(), _p(out_lo), _p(lse), _p(mask), _stream()))
-    return out, (mask, out_lo, lse)
+                                     out.data_ptr(), _p(out_lo), _p(lse), _p(plan), _stream()))
+    return out, (plan, out_lo, lse)
 
 
 def _block_backward(d, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
-    mask, out_lo, lse = kept
+    plan, out_lo, lse = kept
     for t, to in ((dq, d.dq_stride), (dk, d.dk_stride), (dv, d.dv_stride)):
         to[:] = t.stride()[:3]
     n = lib.dm_block_attention_bwd_ws_bytes(ctypes.byref(d))
     ws = _scratch(q.device, (n + 3) // 4)
     check(lib.dm_block_attention_bwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
-                                     mask.data_ptr(), out.data_ptr(), out_lo.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                     plan.data_ptr(), out.data_ptr(), out_lo.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream()))
 
 
@@ -977,7 +978,7 @@ class _BlockAttentionFn(Function):
         q, k, v, blocks, k_len, out, *kept = ctx.saved_tensors
         with _on(q.device):
             dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k, v))
-            d = _block_desc(*(getattr(ctx.d, n) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top", "scale")), q, k, v)
+            d = _block_desc(*(getattr(ctx.d, n) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top", "scale")), q, k, v, ctx.d.pool)
             _block_backward(d, q, k, v, blocks, k_len, out, kept, _aligned(dout), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
@@ -1034,18 +1035,18 @@ class _SparseAttentionFn(Function):
             out, kept = _block_forward(d, q, k, v, blocks, None, training)
         if training:
             ctx.save_for_backward(qkv, blocks, out, *kept)
-            ctx.cfg = (B, L, H, D, top, scale)
+            ctx.cfg = (B, L, H, D, top, scale, d.pool)
         return out.view(B, L, H * D)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         qkv, blocks, out, *kept = ctx.saved_tensors
-        B, L, H, D, top, scale = ctx.cfg
+        B, L, H, D, top, scale, pool = ctx.cfg
         q, k, v = qkv.view(B, L, 3, H, D).unbind(2)
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            d = _block_desc(B, L, L, H, H, D, top, scale, q, k, v)
+            d = _block_desc(B, L, L, H, H, D, top, scale, q, k, v, pool)
             _block_backward(d, q, k, v, blocks, None, out, kept, _aligned(dout), *dqkv.view(B, L, 3, H, D).unbind(2))
         return dqkv, None, None, None, None, None
 

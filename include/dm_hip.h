@@ -71,8 +71,6 @@ int dm_abi_version(void);
  *   "wgrad_slab_overhead" (12), "wgrad_reduce_cap" (8192)   split-K planning of the weight-gradient kernels
  *   "gn_fused" (1), "gn_bwd16" (1)   single-pass GroupNorm kernels; 512 x 16-pixel form of the 1024-pixel backward
  *   "attn_mfma" (1), "edge_mfma" (1) matrix-core attention (head dims 8, 16) and edge convolutions
- *   "block_pool" (0)      attention over chosen blocks: rows a workgroup works on together (128, 256, 512; 1: one query a
- *                         workgroup; 0: by the shape)
  *   "timing_skip" (0)     TIMING EXPERIMENTS ONLY, results are wrong while non-zero: bit mask of kernel families whose
  *                         launches return without running (1: 1x1 convolutions, 2: weight-gradient slab sums, 4:
  *                         single-tap weight gradients, 8 / 16: GroupNorm backward / forward, 32: stride-2 convolutions,
@@ -303,6 +301,8 @@ int dm_attention_bwd(const void* qkv, const void* out, const void* dout, const f
 typedef struct dm_block_desc {
   int B, Lq, Lk, Hq, Hkv, D;
   int top;      /* blocks a query names, 1 .. 64 */
+  int pool;     /* attention: rows a workgroup works on together, 128, 256 or 512; 1: one query a workgroup; 0: by the
+                   shape. The same in the backward call as in its forward call */
   float scale;  /* of q . k */
   long q_stride[3], k_stride[3], v_stride[3];
   long dq_stride[3], dk_stride[3], dv_stride[3];   /* backward only */
@@ -317,16 +317,17 @@ int dm_block_select(const dm_block_desc* d, const void* q, const void* keys, con
 /* out bf16 [B][Lq][Hq][D] = softmax over the valid keys of the blocks that `blocks` names for a query (any order; a
  * repeated block counts once, numbers outside 0 .. nblk-1 name none), times v. A query without a key gets zeros.
  * For the backward call: out_lo bf16, what the rounding of out lost; lse fp32 [B][Hq][Lq] (natural log; -infinity without
- * a key); mask, the list as bits. out_lo and lse may be null. mask: dm_block_attention_mask_bytes(d, whether a backward call will read it), 16-byte aligned;
- * null where that is 0. */
-size_t dm_block_attention_mask_bytes(const dm_block_desc* d, int for_backward);
+ * a key); both may be null. plan: the rows of every block, written here and read by the backward call;
+ * dm_block_attention_plan_bytes(d, whether there will be one), 16-byte aligned, null where that is 0.
+ * A sample of q spans less than 2^35 elements. */
+size_t dm_block_attention_plan_bytes(const dm_block_desc* d, int for_backward);
 int dm_block_attention_fwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
-                           const int* k_len, void* out, void* out_lo, float* lse, void* mask, void* stream);
+                           const int* k_len, void* out, void* out_lo, float* lse, void* plan, void* stream);
 /* dq, dk, dv bf16 by their strides, written (keys that no query attended get zeros), from what the forward call was
  * given and wrote. ws: dm_block_attention_bwd_ws_bytes, 16-byte aligned, contents irrelevant. */
 size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d);
 int dm_block_attention_bwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
-                           const int* k_len, const void* mask, const void* out, const void* out_lo, const float* lse,
+                           const int* k_len, const void* plan, const void* out, const void* out_lo, const float* lse,
                            const void* dout, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------

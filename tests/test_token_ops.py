@@ -210,10 +210,16 @@ CASES = [
 ]
 
 
+@pytest.fixture(autouse=True)
+def _pool_by_shape():
+    yield
+    from dm_hip import ops as o
+    o.BLOCK_POOL = 0
+
+
 def rows_together(n):
     """how many rows a workgroup takes: by the shape (0), one query (1), or a pool on the matrix cores"""
-    from dm_hip import check, lib
-    check(lib.dm_config_set(b"block_pool", n))
+    ops().BLOCK_POOL = n
 
 
 @gpu
@@ -463,7 +469,7 @@ def test_refusals_of_the_c_abi():
     p = ctypes.c_void_p(4096)
 
     def desc(**kw):
-        d = BlockDesc(1, 64, 64, 2, 1, 16, 4, 1.0)
+        d = BlockDesc(1, 64, 64, 2, 1, 16, 4, 0, 1.0)
         for s in ("q_stride", "k_stride", "v_stride", "dq_stride", "dk_stride", "dv_stride"):
             getattr(d, s)[:] = [2048, 32, 16]
         for k, v in kw.items():
@@ -485,11 +491,12 @@ def test_refusals_of_the_c_abi():
     assert lib.dm_block_select(desc(), p, p, None, None, None) == 1
     assert lib.dm_block_attention_fwd(desc(), p, p, p, None, None, p, None, None, None, None) == 1
     assert lib.dm_block_attention_fwd(desc(), p, p, p, p, None, p, None, None, None, None) == 1
-    assert "mask" in lib.dm_last_error().decode()
+    assert "plan" in lib.dm_last_error().decode()
     assert lib.dm_block_attention_bwd(desc(), p, p, p, p, None, p, p, p, p, p, p, p, p, p, 8, None) == 1
     assert "workspace" in lib.dm_last_error().decode()
-    assert lib.dm_block_attention_mask_bytes(desc(D=3), 1) == 0
-    assert lib.dm_config_set(b"block_pool", 64) == 1
+    assert lib.dm_block_attention_plan_bytes(desc(D=3), 1) == 0
+    assert lib.dm_block_attention_plan_bytes(desc(pool=64), 1) == 0
+    assert lib.dm_block_attention_fwd(desc(q_stride=[0, 2 ** 32, 16]), p, p, p, p, None, p, None, None, p, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 5, 0, 4, 1.0, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 2 ** 31, 9, 4, 1.0, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 5, 9, 0, 1.0, None) == 2
