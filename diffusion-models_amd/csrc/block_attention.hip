@@ -193,63 +193,72 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 
 // offs[b][hkv][pool][0 .. nblk]: where the rows of a block begin in rows[b][hkv][pool][P top] (numbers inside the pool,
 // ascending). A set: a block that a query names twice counts once, numbers outside 0 .. nblk-1 name none.
-constexpr int PLAN_CHUNK = 256;
+// A thread is a row. It sets its bit in the words of its blocks; after the counts' prefix sums a row's place in a block's list is the
+// block's start + the bits of earlier words + those of earlier lanes.
+constexpr int PLAN_CHUNK = 256;   // blocks at a time
 template <int P>
-__global__ __launch_bounds__(256) void block_plan_kernel(const int* __restrict__ blocks, int* __restrict__ offs, unsigned short* __restrict__ rows,
-                                                         int Lq, int Hq, int G, int top, int nblk, int pools) {
-  constexpr int NG = P / 64;
-  __shared__ unsigned long long word[PLAN_CHUNK][NG];
-  __shared__ int place[PLAN_CHUNK], wsum[4];
+__global__ __launch_bounds__(P < 256 ? 256 : P) void block_plan_kernel(const int* __restrict__ blocks, int* __restrict__ offs,
+                                                                       unsigned short* __restrict__ rows, int Lq, int Hq, int G, int top,
+                                                                       int nblk, int pools) {
+  constexpr int NG = P / 64, NT = P < 256 ? 256 : P;
+  __shared__ unsigned long long word[NG][PLAN_CHUNK];
+  __shared__ int place[NG][PLAN_CHUNK], wsum[4];
   const int pool = blockIdx.x, bh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int Hkv = Hq / G, b = bh / Hkv, hk = bh - b * Hkv;
   const long r0 = (long)pool * P;
-  const int n_rows = (int)min((long)P, (long)Lq * G - r0);
+  const bool in = tid < P && r0 + tid < (long)Lq * G;
+  const unsigned r = (unsigned)(r0 + tid), i = G == 1 ? r : r / (unsigned)G;
+  const int* const named = blocks + (((long)b * Hq + hk * G + (int)(r - i * (unsigned)G)) * Lq + i) * top;
   int* const of = offs + ((long)bh * pools + pool) * (nblk + 1);
   unsigned short* const out = rows + ((long)bh * pools + pool) * ((long)P * top);
   int base = 0;
   for (int j0 = 0; j0 < nblk; j0 += PLAN_CHUNK) {
-    for (int e = tid; e < PLAN_CHUNK * NG; e += 256) (&word[0][0])[e] = 0;
+    const int n = min(PLAN_CHUNK, nblk - j0);
+    for (int e = tid; e < PLAN_CHUNK * NG; e += NT) (&word[0][0])[e] = 0;
     __syncthreads();
-    for (int e = tid; e < n_rows * top; e += 256) {
-      const int rr = e / top, t = e - rr * top;
-      const unsigned r = (unsigned)(r0 + rr), i = G == 1 ? r : r / (unsigned)G;
-      const int h = hk * G + (int)(r - i * (unsigned)G);
-      const int j = blocks[(((long)b * Hq + h) * Lq + i) * top + t] - j0;
-      if (j >= 0 && j < PLAN_CHUNK && j0 + j < nblk) atomicOr(&word[j][rr >> 6], 1ull << (rr & 63));
-    }
-    __syncthreads();
-    int count = 0;
-#pragma unroll
-    for (int x = 0; x < NG; ++x) count += __builtin_popcountll(word[tid][x]);
-    int inc = count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += up;
-    }
-    if (lane == 63) wsum[wave] = inc;
-    __syncthreads();
-    int before = base, all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      before += w < wave ? wsum[w] : 0;
-      all += wsum[w];
-    }
-    before += inc - count;
-    place[tid] = before;
-    if (j0 + tid < nblk) of[j0 + tid] = before;
-    __syncthreads();
-    for (int j = wave; j < min(PLAN_CHUNK, nblk - j0); j += 4) {
-      int at = place[j];
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const unsigned long long w = word[j][x];
-        const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(w >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)w, 0));
-        if ((w >> lane) & 1) out[at + rank] = (unsigned short)(x * 64 + lane);
-        at += __builtin_popcountll(w);
+    if (in) {
+#pragma unroll 8
+      for (int t = 0; t < top; ++t) {
+        const int j = named[t] - j0;
+        if (j >= 0 && j < n) atomicOr(&word[wave][j], 1ull << lane);
       }
     }
-    base += all;
+    __syncthreads();
+    int count = 0, before = 0;
+    if (tid < PLAN_CHUNK) {
+#pragma unroll
+      for (int x = 0; x < NG; ++x) count += __builtin_popcountll(word[x][tid]);
+      int inc = count;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 63) wsum[wave] = inc;
+      before = inc - count;
+    }
+    __syncthreads();
+    if (tid < PLAN_CHUNK) {
+      before += base;
+#pragma unroll
+      for (int w = 0; w < 3; ++w) before += w < wave ? wsum[w] : 0;
+      if (tid < n) of[j0 + tid] = before;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        place[x][tid] = before;
+        before += __builtin_popcountll(word[x][tid]);
+      }
+    }
+    base += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+    if (in) {
+#pragma unroll 8
+      for (int t = 0; t < top; ++t) {
+        const int j = named[t] - j0;
+        if (j >= 0 && j < n)   // (a block named twice: the same place and row again)
+          out[place[wave][j] + __builtin_popcountll(word[wave][j] & ((1ull << lane) - 1))] = (unsigned short)tid;
+      }
+    }
     __syncthreads();
   }
   if (tid == 0) of[nblk] = base;
@@ -885,7 +894,7 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
     unsigned short* rows = (unsigned short*)((char*)plan + p.offs);
     a.offs = offs; a.rows = rows;
     const dim3 grid(p.pools, d->B * d->Hkv);
-#define GO(P) hipLaunchKernelGGL((block_plan_kernel<P>), grid, dim3(256), 0, st, blocks, offs, rows, d->Lq, d->Hq, a.G, d->top, a.nblk, p.pools)
+#define GO(P) hipLaunchKernelGGL((block_plan_kernel<P>), grid, dim3(P < 256 ? 256 : P), 0, st, blocks, offs, rows, d->Lq, d->Hq, a.G, d->top, a.nblk, p.pools)
     if (p.pool == 128) GO(128); else if (p.pool == 256) GO(256); else GO(512);
 #undef GO
     DM_CHECK_LAUNCH();

@@ -1,0 +1,299 @@
+// The choice of key blocks: one summary per block of 64 keys, and for every query the blocks whose summaries it scores highest.
+//
+//   keys[b][h][j]   = mean of block j's valid keys              (dm_block_keys)
+//   blocks[b][h][i] = the `top` blocks of the highest q_i . keys_j (dm_block_select)
+//
+// Query heads share key heads (Hq = G Hkv). The ROWS of a (sample, key head) are its G Lq queries, r = i G + g.
+#include "block_common.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------
+// One summary per block: the mean of its valid keys. Summed in 64 bits (64 bf16 values of ordinary spread add up
+// exactly, so the order does not matter) and rounded to fp32 and then bf16: the summary is only a score's operand, and
+// as bf16 its products with q are exact in 64-bit sums too, which makes the choice of blocks independent of batch, tile and order.
+// A workgroup holds one block of up to 512 features (8 a lane) of all heads, its threads splitting the 64 keys.
+__global__ __launch_bounds__(256) void block_keys_kernel(Rows k, const int* __restrict__ k_len, bf16_t* __restrict__ keys, int Lk, int Hkv,
+                                                         int D, int nblk, int vt) {
+  __shared__ double part[256][8];
+  const int j = blockIdx.x, b = blockIdx.z, tid = threadIdx.x;
+  const int vl = tid & (vt - 1), phase = tid / vt, phases = 256 / vt;
+  const int f = (blockIdx.y * vt + vl) * 8;
+  const bool live = f < Hkv * D;
+  const int h = live ? f / D : 0, d = live ? f - h * D : 0;
+  const int n = min(valid_keys(k_len, b, Lk) - j * BLK, BLK);
+  double s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (live) {
+    const bf16_t* p = k.p + b * k.sb + (long)j * BLK * k.sl + h * k.sh + d;
+#pragma unroll 4
+    for (int t = phase; t < n; t += phases) {
+      const bf16x8_t x = *(const bf16x8_t*)(p + t * k.sl);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (double)(float)x[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[tid][e] = s[e];
+  __syncthreads();
+  if (phase == 0 && live) {
+    bf16x8_t y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      double t = part[vl][e];
+      for (int w = 1; w < phases; ++w) t += part[w * vt + vl][e];
+      y[e] = (bf16_t)(float)(n > 0 ? t / n : 0.0);
+    }
+    *(bf16x8_t*)(keys + (((long)b * Hkv + h) * nblk + j) * D + d) = y;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The choice of blocks. Scores are compared as 64-bit sums; two ways to get there:
+//
+// exact_top: one query a wave, all scores in 64 bits, EXACT_CHUNK blocks at a time beside the best of the earlier ones. A
+// score becomes an unsigned number of the same order (NaN: that of -infinity), 0 stands for a block already taken.
+constexpr int EXACT_CHUNK = 512;
+template <int O>
+__device__ __forceinline__ unsigned lane_xor_u(unsigned x) {   // as lane_xor, and O = 16, 32 (whole-wave reductions)
+  if constexpr (O == 16) { auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); return (threadIdx.x & 16) ? r[0] : r[1]; }
+  else if constexpr (O == 32) { auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); return (threadIdx.x & 32) ? r[0] : r[1]; }
+  else return __builtin_bit_cast(unsigned, lane_xor<O>(__builtin_bit_cast(float, x)));
+}
+template <int O>
+__device__ __forceinline__ void take_best(unsigned long long& key, int& j) {
+  const unsigned long long k = (unsigned long long)lane_xor_u<O>((unsigned)(key >> 32)) << 32 | lane_xor_u<O>((unsigned)key);
+  const int i = (int)lane_xor_u<O>((unsigned)j);
+  if (k > key || (k == key && i < j)) { key = k; j = i; }
+}
+constexpr int NO_BLOCK = 0x7fffffff;
+
+// lane t's return value: the t-th block taken, or NO_BLOCK
+template <int D>
+__device__ int exact_top(const bf16_t* qp, const bf16_t* kp, int have, int top, unsigned long long* buf, int lane) {
+  unsigned long long won = 0;    // lane t: the t-th best of the chunks so far
+  int won_j = NO_BLOCK;
+  for (int c0 = 0; c0 < have; c0 += EXACT_CHUNK) {
+    const int n = min(EXACT_CHUNK, have - c0);
+    for (int x = lane; x < n; x += 64) {
+      double s = 0;
+#pragma unroll 2
+      for (int d = 0; d < D; d += 8) {
+        const bf16x8_t a = *(const bf16x8_t*)(qp + d), b = *(const bf16x8_t*)(kp + (long)(c0 + x) * D + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)(float)a[e] * (double)(float)b[e];
+      }
+      s = s == s ? s + 0.0 : -INFINITY;   // (-0 and 0 are equal)
+      const unsigned long long u = __builtin_bit_cast(unsigned long long, s);
+      buf[x] = (u >> 63) ? ~u : u | 0x8000000000000000ull;
+    }
+    unsigned long long next = 0;
+    int next_j = NO_BLOCK;
+    for (int t = 0; t < top; ++t) {
+      unsigned long long key = won;
+      int j = won_j;
+      for (int x = lane; x < n; x += 64)
+        if (buf[x] > key) { key = buf[x]; j = c0 + x; }   // (earlier chunks have the lower numbers: ties stay with them)
+      take_best<1>(key, j);
+      take_best<2>(key, j);
+      take_best<4>(key, j);
+      take_best<8>(key, j);
+      take_best<16>(key, j);
+      take_best<32>(key, j);
+      if (!key) break;
+      if (lane == t) { next = key; next_j = j; }
+      if (won_j == j) won = 0;
+      if (j >= c0 && ((j - c0) & 63) == lane) buf[j - c0] = 0;   // (a lane reads only what it wrote)
+    }
+    won = next;
+    won_j = next_j;
+  }
+  return won_j;
+}
+// the blocks taken, in ascending order, -1 behind
+__device__ __forceinline__ void write_taken(int* to, int taken, int top, int lane) {
+  int rank = 0;
+  for (int t = 0; t < top; ++t) {
+    const int other = __builtin_amdgcn_readlane(taken, t);
+    rank += other < taken || (other == taken && t < lane);
+  }
+  if (lane < top) to[rank] = taken == NO_BLOCK ? -1 : taken;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void block_select_row_kernel(Rows q, const bf16_t* __restrict__ keys, const int* __restrict__ k_len,
+                                                               int* __restrict__ blocks, int Lq, int Lk, int Hq, int G, int top,
+                                                               int nblk, long rows) {
+  __shared__ unsigned long long buf[4][EXACT_CHUNK];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long row = (long)blockIdx.x * 4 + wave;
+  if (row >= rows) return;
+  const int i = row % Lq, h = (row / Lq) % Hq, b = row / ((long)Lq * Hq);
+  const int have = (valid_keys(k_len, b, Lk) + BLK - 1) / BLK;
+  const int taken = exact_top<D>(q.p + b * q.sb + i * q.sl + h * q.sh, keys + ((long)b * (Hq / G) + h / G) * nblk * (long)D, have, top, buf[wave], lane);
+  write_taken(blocks + row * top, taken, top, lane);
+}
+
+// The screening kernel: 16 rows a wave. Scores come from the matrix cores in fp32, off by at most
+//   eps = max(D, 16) 2^-23 |q| max |key| + 2^-118
+// (exact products, at most that many additions each off by one unit of the sum of absolute terms, which |q| |key| bounds; 2^-118, here and under
+// the roots, covers products too small for fp32; the factor 1.016 the roundings of the norms themselves). With T the (top)-th and U the (top + 1)-th best of them, T - U > 2 eps says that
+// the fp32 scores order these two as 64-bit ones would, and the choice is the scores above U. Rows where that fails, and waves
+// that meet an infinity or NaN, are decided by exact_top.
+//   Every lane keeps the K best of the blocks it sees (a row's blocks are dealt to 4 lanes, neighbouring blocks to
+// different ones), sorted, one v_med3 a place and score. K is about twice the fair share (top + 1) / 4: a lane that may have
+// dropped one that counts sends its row to exact_top as well. A second pass over the same scores writes the choice in order.
+template <int D, int K>
+__global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t* __restrict__ keys, const int* __restrict__ k_len,
+                                                           int* __restrict__ blocks, int Lq, int Lk, int Hkv, int G, int top, int nblk) {
+  constexpr int EXACT_FLOATS = EXACT_CHUNK * 2, LIST_FLOATS = 2 * K * 64;
+  __shared__ __attribute__((aligned(16))) float scratch[4][EXACT_FLOATS > LIST_FLOATS ? EXACT_FLOATS : LIST_FLOATS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, bh = blockIdx.y, b = bh / Hkv, hk = bh - b * Hkv;
+  const long rows = (long)Lq * G, r0 = ((long)blockIdx.x * 4 + wave) * 16;
+  if (r0 >= rows) return;   // (waves are independent: no barriers)
+  const long r = min(r0 + (lane & 15), rows - 1);
+  const bool in = r0 + (lane & 15) < rows;
+  const unsigned i = G == 1 ? (unsigned)r : (unsigned)r / (unsigned)G;
+  const int h = hk * G + (int)((unsigned)r - i * (unsigned)G), Hq = Hkv * G;
+  int* to = blocks + (((long)b * Hq + h) * Lq + i) * top;
+  const int have = (valid_keys(k_len, b, Lk) + BLK - 1) / BLK;
+  if (have <= top) {   // every block
+    if (in)
+      for (int t = g; t < top; t += 4) to[t] = t < have ? t : -1;
+    return;
+  }
+  const bf16_t* kp = keys + (long)bh * nblk * D;
+  const bf16_t* qp = q.p + b * q.sb + (long)i * q.sl + h * q.sh;
+  Frag<D> qf;
+  qf.load(qp, g);
+  float qq = 0.f;
+#pragma unroll
+  for (int s = 0; s < Geo<D>::KS; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qq += (float)qf.x[s][e] * (float)qf.x[s][e];
+  qq = row_sum(qq);
+  const int mine = 4 * (lane & 3) + ((lane & 15) >> 2);   // the block of a chunk of 16 that this lane fetches; it gets the scores of 4 e + g
+  float best[K];
+#pragma unroll
+  for (int x = 0; x < K; ++x) best[x] = -INFINITY;
+  unsigned kk = 0;   // the largest |key|^2, by its bits: a NaN is larger than any number
+  for (int c = 0; c < have; c += 16) {
+    Frag<D> kf;
+    kf.load(kp + (long)min(c + mine, have - 1) * D, g);
+    const f32x4_t s = dot_frag<D>(kf, qf), n = dot_frag<D>(kf, kf);
+    const float d01 = (lane & 1) ? n[1] : n[0], d23 = (lane & 1) ? n[3] : n[2], d = (lane & 2) ? d23 : d01;
+    if (g == ((lane & 15) >> 2)) kk = max(kk, __builtin_bit_cast(unsigned, d) & 0x7fffffffu);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = c + 4 * e + g < have ? s[e] : -INFINITY;
+#pragma unroll
+      for (int p = K - 1; p > 0; --p) best[p] = __builtin_amdgcn_fmed3f(best[p - 1], best[p], x);
+      best[0] = fmaxf(best[0], x);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) kk = max(kk, (unsigned)__shfl_xor((int)kk, o, 64));
+  // two lanes' lists become one of 2 K (values of the other lane in order: the j-th takes place j or a later one)
+  float two[2 * K];
+#pragma unroll
+  for (int x = 0; x < K; ++x) { two[x] = best[x]; two[K + x] = -INFINITY; }
+#pragma unroll
+  for (int x = 0; x < K; ++x) {
+    const float y = __builtin_bit_cast(float, lane_xor_u<16>(__builtin_bit_cast(unsigned, best[x])));
+#pragma unroll
+    for (int p = K + x; p > x; --p) two[p] = __builtin_amdgcn_fmed3f(two[p - 1], two[p], y);
+    two[x] = fmaxf(two[x], y);
+  }
+  // the m-th best of two sorted lists: max over i of min(a_i, b_(m - i)), counted from 1, a_0 = b_0 = infinity
+  float* lists = scratch[wave];
+#pragma unroll
+  for (int x = 0; x < 2 * K; ++x) lists[x * 64 + lane] = two[x];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  float T = -INFINITY, U = -INFINITY;
+#pragma unroll
+  for (int x = 0; x <= 2 * K; ++x) {
+    const float a = x == 0 ? INFINITY : two[x == 0 ? 0 : x - 1];
+    const int m = top - x;
+    auto other = [&](int y) { return y == 0 ? INFINITY : y > 0 && y <= 2 * K ? lists[(y - 1) * 64 + (lane ^ 32)] : -INFINITY; };
+    T = fmaxf(T, fminf(a, other(m)));
+    U = fmaxf(U, fminf(a, other(m + 1)));
+  }
+  const float eps2 = 2.f * ((D < 16 ? 16 : D) * 0x1.04p-23f * __builtin_sqrtf(qq + 0x1p-118f) * __builtin_sqrtf(__builtin_bit_cast(float, kk) + 0x1p-118f) + 0x1p-118f);
+  bool clear = T - U > eps2;                                            // (false if anything is NaN or infinite)
+  if (K < top + 1) {
+    const float last = best[K - 1], l16 = fmaxf(last, __builtin_bit_cast(float, lane_xor_u<16>(__builtin_bit_cast(unsigned, last))));
+    const float l32 = fmaxf(l16, __builtin_bit_cast(float, lane_xor_u<32>(__builtin_bit_cast(unsigned, l16))));
+    clear = clear && (l32 == -INFINITY || U > l32);                     // what a lane dropped is not above its last
+  }
+  clear = clear && kk < 0x7f800000u && qq < INFINITY;
+  int count = 0;
+  for (int c = 0; c < have; c += 16) {
+    Frag<D> kf;
+    kf.load(kp + (long)min(c + mine, have - 1) * D, g);
+    const f32x4_t s = dot_frag<D>(kf, qf);
+    unsigned bits = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + 4 * e + g < have && s[e] > U) bits |= 1u << (4 * e + g);
+    unsigned all = bits | lane_xor_u<16>(bits);
+    all |= lane_xor_u<32>(all);
+    if (clear && in) {
+      while (bits) {
+        const int x = __builtin_ctz(bits);
+        bits &= bits - 1;
+        to[count + __builtin_popcount(all & ((1u << x) - 1))] = c + x;
+      }
+    }
+    count += __builtin_popcount(all);
+  }
+  unsigned long long open = __ballot(!clear && in && g == 0);
+  while (open) {   // rows that 32 bits cannot decide
+    const int x = __builtin_ctzll(open);
+    open &= open - 1;
+    const unsigned ri = __builtin_amdgcn_readlane(i, x);
+    const int rh = __builtin_amdgcn_readlane(h, x);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int taken = exact_top<D>(q.p + b * q.sb + (long)ri * q.sl + rh * q.sh, kp, have, top, (unsigned long long*)scratch[wave], lane);
+    write_taken(blocks + (((long)b * Hq + rh) * Lq + ri) * top, taken, top, lane);
+  }
+}
+
+}  // namespace
+
+extern "C" int dm_block_keys(const dm_block_desc* d, const void* k, const int* k_len, void* keys, void* stream) {
+  const char* who = "dm_block_keys";
+  int rc = check_desc(who, d);
+  if (rc) return rc;
+  DM_REQUIRE(aligned(k) && aligned(keys), DM_ERR_ARG, "%s: null or misaligned pointer", who);
+  if ((rc = check_strides(who, "k", d->k_stride))) return rc;
+  const int vecs = d->Hkv * d->D / 8;
+  DM_REQUIRE(d->B <= 65535 && dm_cdiv(vecs, 64) <= 65535, DM_ERR_SHAPE, "%s: batch or heads too large", who);
+  int vt = 1;
+  while (vt < 64 && vt < vecs) vt <<= 1;
+  hipLaunchKernelGGL(block_keys_kernel, dim3(blocks_of(d), dm_cdiv(vecs, vt), d->B), dim3(256), 0, (hipStream_t)stream,
+                     rows_of(k, d->k_stride), k_len, (bf16_t*)keys, d->Lk, d->Hkv, d->D, blocks_of(d), vt);
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
+
+extern "C" int dm_block_select(const dm_block_desc* d, const void* q, const void* keys, const int* k_len, int* blocks, void* stream) {
+  const char* who = "dm_block_select";
+  int rc = check_desc(who, d);
+  if (rc) return rc;
+  DM_REQUIRE(aligned(q) && aligned(keys) && blocks, DM_ERR_ARG, "%s: null or misaligned pointer", who);
+  if ((rc = check_strides(who, "q", d->q_stride))) return rc;
+  const int G = d->Hq / d->Hkv, n = blocks_of(d), top = d->top;
+  const long rows = (long)d->B * d->Hq * d->Lq, shared = (long)d->Lq * G;
+  hipStream_t st = (hipStream_t)stream;
+  if (shared < 16) {
+    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
+                                         (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows));
+  } else {
+    const dim3 grid(dm_cdiv(shared, 64), d->B * d->Hkv);
+#define GO(K) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_kernel<HD, K>), grid, dim3(256), 0, st, rows_of(q, d->q_stride), \
+                                                   (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hkv, G, top, n))
+    if (top <= 4) GO(5) else if (top <= 11) GO(8) else if (top <= 19) GO(12) else if (top <= 35) GO(20) else GO(36)
+#undef GO
+  }
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
