@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The matrix-core form. A workgroup owns a POOL of P rows of one (sample, key head) and visits the blocks that any of
+// The matrix-core form. A workgroup owns a POOL of 512 rows of one (sample, key head) and visits the blocks that any of
 // them chose, in order. The pool's rows that chose a block are packed into tiles of 16, so that a matrix instruction works on 16
 // rows that all want the block however the choices are scattered (16 neighbouring rows would share few blocks: with 8 of 64
 // chosen at random a tile of neighbours has to visit 56). What a row accumulates (its output and statistics, or its dq) lives in LDS in
@@ -191,22 +191,23 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 // maximum and sum are two lane swaps away, and exp(S^T) is in the register layout that the second product takes as its
 // right operand (its left operand, V^T or K^T, is read by transposing LDS reads in the same order of keys).
 
-// offs[b][hkv][pool][0 .. nblk]: where the rows of a block begin in rows[b][hkv][pool][P top] (numbers inside the pool,
+constexpr int POOL = 512;
+
+// offs[b][hkv][pool][0 .. nblk]: where the rows of a block begin in rows[b][hkv][pool][512 top] (numbers inside the pool,
 // ascending). A set: a block that a query names twice counts once, numbers outside 0 .. nblk-1 name none.
 // A thread is a row. It sets its bit in the words of its blocks; after the counts' prefix sums a row's place in a block's list is the
 // block's start + the bits of earlier words + those of earlier lanes.
 constexpr int PLAN_CHUNK = 256;   // blocks at a time
-template <int P>
-__global__ __launch_bounds__(P < 256 ? 256 : P) void block_plan_kernel(const int* __restrict__ blocks, int* __restrict__ offs,
-                                                                       unsigned short* __restrict__ rows, int Lq, int Hq, int G, int top,
-                                                                       int nblk, int pools) {
-  constexpr int NG = P / 64, NT = P < 256 ? 256 : P;
+__global__ __launch_bounds__(POOL) void block_plan_kernel(const int* __restrict__ blocks, int* __restrict__ offs,
+                                                          unsigned short* __restrict__ rows, int Lq, int Hq, int G, int top, int nblk,
+                                                          int pools) {
+  constexpr int P = POOL, NG = P / 64;
   __shared__ unsigned long long word[NG][PLAN_CHUNK];
   __shared__ int place[NG][PLAN_CHUNK], wsum[4];
   const int pool = blockIdx.x, bh = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int Hkv = Hq / G, b = bh / Hkv, hk = bh - b * Hkv;
   const long r0 = (long)pool * P;
-  const bool in = tid < P && r0 + tid < (long)Lq * G;
+  const bool in = r0 + tid < (long)Lq * G;
   const unsigned r = (unsigned)(r0 + tid), i = G == 1 ? r : r / (unsigned)G;
   const int* const named = blocks + (((long)b * Hq + hk * G + (int)(r - i * (unsigned)G)) * Lq + i) * top;
   int* const of = offs + ((long)bh * pools + pool) * (nblk + 1);
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(P < 256 ? 256 : P) void block_plan_kernel(const int
   int base = 0;
   for (int j0 = 0; j0 < nblk; j0 += PLAN_CHUNK) {
     const int n = min(PLAN_CHUNK, nblk - j0);
-    for (int e = tid; e < PLAN_CHUNK * NG; e += NT) (&word[0][0])[e] = 0;
+    for (int e = tid; e < PLAN_CHUNK * NG; e += P) (&word[0][0])[e] = 0;
     __syncthreads();
     if (in) {
 #pragma unroll 8
@@ -288,9 +289,9 @@ struct Visits {
 };
 
 // One pool's place, its waves' tiles and the staging of the operand that is read transposed.
-template <int D, int P>
+template <int D>
 struct Pool {
-  static constexpr int NW = P / 64;
+  static constexpr int P = POOL, NW = P / 64;
   static constexpr int PIECES = 2 * BLK * D / 8, PER = (PIECES + P - 1) / P;   // 16-byte pieces of a block's keys and values
   // two buffers where they fit beside what the rows accumulate (all but 512 rows of 64 features)
   static constexpr int KV = 2 * Geo<D>::KV_BYTES, BUFS = P * (Geo<D>::DV * 4 + 24) + 2 * KV <= 160 * 1024 ? 2 : 1;
@@ -366,7 +367,7 @@ struct Pool {
     long i;
     int h;
     place(row, i, h);
-    return (unsigned)((i * sl + h * sh) >> 3);
+    return (unsigned)i * (unsigned)(sl >> 3) + (unsigned)h * (unsigned)(sh >> 3);
   }
 };
 
@@ -376,10 +377,11 @@ __device__ __forceinline__ bool pool_of_block(int nbh, int pools, int& bh, int& 
   return bh < nbh;
 }
 
-template <int D, int P>
-__global__ __launch_bounds__(P) void attend_pool_kernel(Args a) {
+template <int D>
+__global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
   using GE = Geo<D>;
-  using PL = Pool<D, P>;
+  using PL = Pool<D>;
+  constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
   __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
   __shared__ __attribute__((aligned(16))) f32x4_t stat[P];   // maximum, sum of the weights, sum of the weights as rounded
@@ -520,10 +522,11 @@ __global__ __launch_bounds__(P) void attend_pool_kernel(Args a) {
 }
 
 // dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end.
-template <int D, int P>
-__global__ __launch_bounds__(P) void dq_pool_kernel(Args a) {
+template <int D>
+__global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   using GE = Geo<D>;
-  using PL = Pool<D, P>;
+  using PL = Pool<D>;
+  constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
   __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
   __shared__ f32x2_t stat[P];   // lse, delta
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(P) void dq_pool_kernel(Args a) {
 // P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
 constexpr int LIST = 4096;
 template <int D>
-__global__ __launch_bounds__(256, 2) void dkv_kernel(Args a, int pool_rows) {
+__global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel(Args a) {
   using GE = Geo<D>;
   constexpr int TILE_BYTES = 32 * GE::ROWB;
   __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
@@ -684,14 +687,35 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a, int pool_rows) {
   const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int n0 = valid_keys(a.k_len, b, a.Lk) - j * BLK;
   const float sc = a.scale * LOG2E;
-  const bf16x8_t none = {};
+  // The chain of loads at the start (where the block's rows lie in the lists, the rows, their q and do) and the keys and values
+  // beside it decide the time of a short list: the first one goes out first.
+  constexpr int per = LIST / POOL;    // pools whose rows fit the list
+  int start = 0, own = 0;
+  auto find = [&](int p0) {           // lane x: the rows of pool p0 + x
+    const bool has = lane < per && p0 + lane < a.pools;
+    const int* at = a.offs + ((long)bh * a.pools + p0 + lane) * (a.nblk + 1) + j;
+    start = has ? at[0] : 0;
+    own = has ? at[1] - start : 0;
+  };
   if (n0 > 0) {
-    for (int e = tid; e < 2 * BLK * D / 8; e += 256) {
-      const int half = e >= BLK * D / 8 ? 1 : 0, p = e - half * (BLK * D / 8), t = p / (D / 8), c = p % (D / 8);
+    find(0);
+    constexpr int PER = (2 * BLK * D / 8 + 255) / 256;
+    const bf16x8_t none = {};
+    bf16x8_t x[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * 256 + tid, half = e >= BLK * D / 8 ? 1 : 0, p = e - half * (BLK * D / 8), t = p / (D / 8), c = p % (D / 8);
       const Rows& s = half ? a.v : a.k;
+      x[u] = e < 2 * BLK * D / 8 && t < n0 ? *(const bf16x8_t*)(s.p + b * s.sb + ((long)j * BLK + t) * s.sl + hk * s.sh + c * 8) : none;
+    }
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * 256 + tid, half = e >= BLK * D / 8 ? 1 : 0, p = e - half * (BLK * D / 8), t = p / (D / 8), c = p % (D / 8);
       char* to = half ? vbuf : kbuf;
-      *(bf16x8_t*)(to + lds_at<D>(t, c)) = t < n0 ? *(const bf16x8_t*)(s.p + b * s.sb + ((long)j * BLK + t) * s.sl + hk * s.sh + c * 8) : none;
-      if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+      if (e < 2 * BLK * D / 8) {
+        *(bf16x8_t*)(to + lds_at<D>(t, c)) = x[u];
+        if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+      }
     }
   }
   f32x4_t dk[4][GE::DT], dv[4][GE::DT];
@@ -699,115 +723,121 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a, int pool_rows) {
   for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
     for (int dt = 0; dt < GE::DT; ++dt) dk[kt][dt] = dv[kt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const unsigned q8l = (unsigned)(a.q.sl >> 3), q8h = (unsigned)(a.q.sh >> 3);
+  const bf16_t *const qbase = a.q.p + b * a.q.sb, *const obase = a.go + (long)b * a.Lq * a.Hq * D;
+  const float *const lbase = a.lse + (long)b * a.Hq * a.Lq, *const dbase = a.delta + (long)b * a.Hq * a.Lq;
   char *qb = rows[wave][0], *ob = rows[wave][1];
   float *st_lse = stat[wave][0], *st_delta = stat[wave][1];
-  const int per = LIST / pool_rows;   // pools whose rows fit the list
   for (int p0 = 0; p0 < a.pools && n0 > 0; p0 += per) {
-    const bool has = lane < per && p0 + lane < a.pools;
-    const int* of = a.offs + ((long)bh * a.pools + p0 + lane) * (a.nblk + 1) + j;
-    const int start = has ? of[0] : 0, own = has ? of[1] - start : 0;
+    if (p0) find(p0);
     int inc = own;
 #pragma unroll
-    for (int o = 1; o < LIST / 128; o <<= 1) {
+    for (int o = 1; o < per; o <<= 1) {
       const int up = __shfl_up(inc, o, 64);
       if (lane >= o) inc += up;
     }
-    const int count = __builtin_amdgcn_readlane(inc, LIST / 128 - 1), before = inc - own;
+    const int count = __builtin_amdgcn_readlane(inc, per - 1), before = inc - own;
     __syncthreads();   // the list's last use is over
     for (int x = wave; x < per && p0 + x < a.pools; x += 4) {
       const int s = __builtin_amdgcn_readlane(start, x), m = __builtin_amdgcn_readlane(own, x), to = __builtin_amdgcn_readlane(before, x);
-      const unsigned short* from = a.rows + ((long)bh * a.pools + p0 + x) * ((long)pool_rows * a.top) + s;
-      for (int e = lane; e < m; e += 64) list[to + e] = (unsigned short)(x * pool_rows + from[e]);
+      const unsigned short* from = a.rows + ((long)bh * a.pools + p0 + x) * ((long)POOL * a.top) + s;
+      for (int e = lane; e < m; e += 64) list[to + e] = (unsigned short)(x * POOL + from[e]);
     }
     __syncthreads();
-    for (int t = wave; t * 32 < count; t += 4) {
-      // a lane's two rows: 16 mt + (lane & 15)
-      Frag<D> qf[2], of[2];
+    // a lane's two rows of a tile, 16 mt + (lane & 15), as operands; behind the last row zeros, with a weight of zero
+    Frag<D> qf[2], of[2];
+    float lse[2], delta[2];
+    auto load = [&](int t) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         const int li = t * 32 + mt * 16 + (lane & 15);
         qf[mt].zero();
         of[mt].zero();
-        float lse = INFINITY, delta = 0.f;
+        lse[mt] = -INFINITY;
+        delta[mt] = 0.f;
         if (li < count) {
-          const unsigned r = (unsigned)(p0 * pool_rows + list[li]);
+          const unsigned r = (unsigned)(p0 * POOL + list[li]);
           const unsigned i = a.G == 1 ? r : r / (unsigned)a.G;
           const int h = hk * a.G + (int)(r - i * a.G);
-          const long lrow = ((long)b * a.Hq + h) * a.Lq + i;
-          qf[mt].load(a.q.p + b * a.q.sb + (long)i * a.q.sl + h * a.q.sh, g);
-          of[mt].load(a.go + (((long)b * a.Lq + i) * a.Hq + h) * D, g);
-          lse = a.lse[lrow];
-          lse = lse == -INFINITY ? INFINITY : lse * LOG2E;
-          delta = a.delta[lrow];
-        }
-        const int row = mt * 16 + (lane & 15);
-        if (g == 0) { st_lse[row] = lse; st_delta[row] = delta; }
-        if constexpr (D <= 16) {
-          *(bf16x4_t*)(qb + lds_at<D>(row, g >> 1) + (g & 1) * 8) = __builtin_shufflevector(qf[mt].x[0], qf[mt].x[0], 0, 1, 2, 3);
-          *(bf16x4_t*)(ob + lds_at<D>(row, g >> 1) + (g & 1) * 8) = __builtin_shufflevector(of[mt].x[0], of[mt].x[0], 0, 1, 2, 3);
-        } else {
-#pragma unroll
-          for (int s = 0; s < GE::KS; ++s) {
-            *(bf16x8_t*)(qb + lds_at<D>(row, s * 4 + g)) = qf[mt].x[s];
-            *(bf16x8_t*)(ob + lds_at<D>(row, s * 4 + g)) = of[mt].x[s];
-          }
+          // (32-bit places inside the sample, in units of 8 features: check_span)
+          qf[mt].load(qbase + (size_t)(i * q8l + (unsigned)h * q8h) * 8, g);
+          of[mt].load(obase + (size_t)((i * (unsigned)a.Hq + (unsigned)h) * (D / 8)) * 8, g);
+          const unsigned at = (unsigned)h * (unsigned)a.Lq + i;
+          lse[mt] = lbase[at];
+          delta[mt] = dbase[at];
         }
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes, read by its other lanes
-      bf16x8_t qt[GE::DT], ot[GE::DT];
-#pragma unroll
-      for (int dt = 0; dt < GE::DT; ++dt) {
-        qt[dt] = join4(read_tr<D>(qb, 0, dt, lane), read_tr<D>(qb, 16, dt, lane));
-        ot[dt] = join4(read_tr<D>(ob, 0, dt, lane), read_tr<D>(ob, 16, dt, lane));
-      }
-      f32x4_t lse4[2], delta4[2];
+    };
+    if (wave * 32 < count) load(wave);
+    for (int t = wave; t * 32 < count; t += 4) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        lse4[mt] = *(const f32x4_t*)(st_lse + mt * 16 + g * 4);
-        delta4[mt] = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
-      }
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        Frag<D> kf, vf;
-        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
-        vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
-        float p[8], ds[8];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - lse4[mt][e]);
-            ds[mt * 4 + e] = p[mt * 4 + e] * (dp[e] - delta4[mt][e]);
-          }
+        const int row = mt * 16 + (lane & 15);
+        if (g == 0) {
+          st_lse[row] = lse[mt] == -INFINITY ? INFINITY : lse[mt] * LOG2E;   // (also a row without a key: every weight is zero)
+          st_delta[row] = delta[mt];
         }
-        const bf16x8_t pt = dm_pack8(p), dst = dm_pack8(ds);
+        qf[mt].to_lds(qb, row, g);
+        of[mt].to_lds(ob, row, g);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes, read by its other lanes
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {   // 32 keys at a time (all 64 would not leave registers for the next rows)
+        bf16x8_t pt[2], dst[2];   // p and ds, rounded as the matrix instructions' operands
+#pragma unroll
+        for (int k2 = 0; k2 < 2; ++k2) {
+          const int kt = half * 2 + k2;
+          Frag<D> kf, vf;
+          kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
+          vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
+          float p[8], ds[8];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf);
+            const f32x4_t ls = *(const f32x4_t*)(st_lse + mt * 16 + g * 4), de = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - ls[e]);
+              ds[mt * 4 + e] = p[mt * 4 + e] * (dp[e] - de[e]);
+            }
+          }
+          pt[k2] = dm_pack8(p);
+          dst[k2] = dm_pack8(ds);
+        }
+        if (half == 1 && (t + 4) * 32 < count) load(t + 4);   // on its way during the last products
 #pragma unroll
         for (int dt = 0; dt < GE::DT; ++dt) {
-          dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pt, ot[dt], dv[kt][dt], 0, 0, 0);
-          dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dst, qt[dt], dk[kt][dt], 0, 0, 0);
+          const bf16x8_t qt = join4(read_tr<D>(qb, 0, dt, lane), read_tr<D>(qb, 16, dt, lane));
+          const bf16x8_t ot = join4(read_tr<D>(ob, 0, dt, lane), read_tr<D>(ob, 16, dt, lane));
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const int kt = half * 2 + k2;
+            dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pt[k2], ot, dv[kt][dt], 0, 0, 0);
+            dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dst[k2], qt, dk[kt][dt], 0, 0, 0);
+          }
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
-  // the four waves' sums, in wave order: [key][feature] fp32 in the tiles' memory (4 x 2 x 32 rows hold 64 rows twice)
-  float* sum = (float*)&rows[0][0][0];
+  // The four waves' sums in a fixed order, dk beginning with wave 0 and dv with wave 2 so that two waves work at a time, in the tiles'
+  // memory (4 x 2 x 32 rows hold the 64 keys twice in fp32) and in the order of the accumulator registers.
+  float* const sum = (float*)&rows[0][0][0];
   constexpr int HALF = BLK * GE::DV;
+  auto add = [&](float* to, const f32x4_t (&x)[4][GE::DT], bool first) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) {
+        f32x4_t* at = (f32x4_t*)(to + ((kt * GE::DT + dt) * 64 + lane) * 4);
+        *at = first ? x[kt][dt] : *at + x[kt][dt];
+      }
+  };
+#pragma unroll 1
   for (int x = 0; x < 4; ++x) {
     __syncthreads();
-    if (wave == x) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int dt = 0; dt < GE::DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int at = (kt * 16 + g * 4 + e) * GE::DV + dt * 16 + (lane & 15);
-            sum[at] = (x ? sum[at] : 0.f) + dk[kt][dt][e];
-            sum[HALF + at] = (x ? sum[HALF + at] : 0.f) + dv[kt][dt][e];
-          }
-    }
+    if (wave == x) add(sum, dk, x == 0);
+    if (wave == (x ^ 2)) add(sum + HALF, dv, x == 0);
   }
   __syncthreads();
   const int in = min(BLK, a.Lk - j * BLK);
@@ -816,12 +846,13 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a, int pool_rows) {
     if (t >= in) break;
     const long pos = (long)j * BLK + t;
     const bool live = t < n0;   // positions behind the last valid key: zero
+    const int place = (((t >> 4) * GE::DT + (d >> 4)) * 64 + ((t >> 2) & 3) * 16 + (d & 15)) * 4 + (t & 3);
     float f[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? sum[t * GE::DV + d + x] * a.scale : 0.f;
+    for (int x = 0; x < 8; ++x) f[x] = live ? sum[place + x * 4] * a.scale : 0.f;
     *(bf16x8_t*)(a.dk + b * a.dkb + pos * a.dkl + hk * a.dkh + d) = dm_pack8(f);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? sum[HALF + t * GE::DV + d + x] : 0.f;
+    for (int x = 0; x < 8; ++x) f[x] = live ? sum[HALF + place + x * 4] : 0.f;
     *(bf16x8_t*)(a.dv + b * a.dvb + pos * a.dvl + hk * a.dvh + d) = dm_pack8(f);
   }
 }
@@ -832,27 +863,35 @@ int check_span(const char* who, const dm_block_desc* d) {
   for (int i = 0; i < 3; ++i) DM_REQUIRE(s[i] >= 0, DM_ERR_ARG, "%s: negative stride of q", who);
   DM_REQUIRE((d->Lq - 1) * s[1] + (d->Hq - 1) * s[2] < (1L << 35) && (long)d->Lq * d->Hq * d->D < (1L << 35), DM_ERR_SHAPE,
              "%s: a sample of q spans more than 2^35 elements", who);
-  DM_REQUIRE(d->pool == 0 || d->pool == 1 || d->pool == 128 || d->pool == 256 || d->pool == 512, DM_ERR_ARG,
-             "%s: pool is 0, 1, 128, 256 or 512, not %d", who, d->pool);
+  DM_REQUIRE(d->pool == 0 || d->pool == 1 || d->pool == 512, DM_ERR_ARG, "%s: pool is 0, 1 or 512, not %d", who, d->pool);
   return DM_OK;
 }
-// Rows of a pool (0: one query a workgroup). Large pools fill tiles better and read keys and values less often; small ones
-// give more workgroups where there are few rows.
-int pool_rows(const dm_block_desc* d) {
-  if (d->pool) return d->pool == 1 ? 0 : d->pool;
-  const long rows = (long)d->Lq * (d->Hq / d->Hkv), heads = (long)d->B * d->Hkv;
-  if (rows < 16) return 0;
-  return heads * dm_cdiv(rows, 512) >= 256 ? 512 : 128;
+// Whether the rows are taken in pools on the matrix cores or one query a workgroup. A pool's time is the number of its visits (its
+// blocks) times what a visit takes from barrier to barrier, however few rows want the block: 1.1 us up to 32 features, 1.6 us with 64
+// (256 pools run at a time, twice as many up to 32 features); a query's is 2 ns + 0.2 .. 0.85 ns a block over the whole chip. Both sides
+// measured, forward (us), one query a workgroup against pools:
+//   8 heads x 256 queries, 8 of 64 blocks       D 8  19 / 76       D 64  26 / 92
+//   4 x 8 heads x 256 queries, 8 of 64          D 8  42 / 78       D 64  81 / 92
+//   4 x 8 heads x 1024 queries, 4 of 16         D 8  103 / 37      D 64  174 / 46
+//   2 x 8 heads x 2048 queries, 8 of 128        D 8  146 / 144     D 64  297 / 177
+//   4 x 8 heads x 4096 queries, 8 of 64         D 8  568 / 96      D 64  1141 / 115
+// (Pools of 128 and 256 rows, which occupy more CUs where there are few rows, were never faster by more than 5 %.)
+bool pooled(const dm_block_desc* d) {
+  if (d->pool) return d->pool == POOL;
+  // The two round differently, and a sample's result must not depend on the batch it is in: the choice is priced for 4 samples.
+  const double rows = (double)d->Lq * (d->Hq / d->Hkv), heads = 4.0 * d->Hkv;
+  const double pools = heads * ((long)(rows + POOL - 1) / POOL), rounds = (long)((pools + (d->D == 64 ? 255 : 511)) / (d->D == 64 ? 256 : 512));
+  const double most = (rows < POOL ? rows : POOL) * d->top, visits = most < blocks_of(d) ? most : blocks_of(d);
+  return heads * rows * (2.0 + d->top * (0.2 + 0.01 * d->D)) > 6000.0 + rounds * visits * (d->D == 64 ? 1600.0 : 1100.0);
 }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
-struct PlanLayout { int pool, pools; size_t offs, bytes; };
+struct PlanLayout { int pools; size_t offs, bytes; };
 PlanLayout plan_of(const dm_block_desc* d) {
   PlanLayout p;
-  p.pool = pool_rows(d) ? pool_rows(d) : 128;
-  p.pools = dm_cdiv((long)d->Lq * (d->Hq / d->Hkv), p.pool);
+  p.pools = dm_cdiv((long)d->Lq * (d->Hq / d->Hkv), POOL);
   const size_t all = (size_t)d->B * d->Hkv * p.pools;
   p.offs = (all * (blocks_of(d) + 1) * 4 + 15) / 16 * 16;
-  p.bytes = p.offs + all * p.pool * d->top * 2;
+  p.bytes = p.offs + all * POOL * d->top * 2;
   return p;
 }
 
@@ -869,7 +908,7 @@ Args args_of(const dm_block_desc* d) {
 
 extern "C" size_t dm_block_attention_plan_bytes(const dm_block_desc* d, int for_backward) {
   const char* who = "dm_block_attention_plan_bytes";
-  if (check_desc(who, d) || check_span(who, d) || (!for_backward && !pool_rows(d))) return 0;
+  if (check_desc(who, d) || check_span(who, d) || (!for_backward && !pooled(d))) return 0;
   return plan_of(d).bytes;
 }
 
@@ -886,27 +925,19 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   a.q = rows_of(q, d->q_stride); a.k = rows_of(k, d->k_stride); a.v = rows_of(v, d->v_stride);
   a.blocks = blocks; a.k_len = k_len; a.out = (bf16_t*)out; a.out_lo = (bf16_t*)out_lo; a.lse = lse;
   hipStream_t st = (hipStream_t)stream;
-  const int pool = pool_rows(d);
+  const bool pool = pooled(d);
   DM_REQUIRE(aligned(plan) || (!plan && !pool), DM_ERR_ARG, "%s: this shape needs a plan (dm_block_attention_plan_bytes), 16-byte aligned", who);
   if (plan) {
     const PlanLayout p = plan_of(d);
     int* offs = (int*)plan;
     unsigned short* rows = (unsigned short*)((char*)plan + p.offs);
     a.offs = offs; a.rows = rows;
-    const dim3 grid(p.pools, d->B * d->Hkv);
-#define GO(P) hipLaunchKernelGGL((block_plan_kernel<P>), grid, dim3(P < 256 ? 256 : P), 0, st, blocks, offs, rows, d->Lq, d->Hq, a.G, d->top, a.nblk, p.pools)
-    if (p.pool == 128) GO(128); else if (p.pool == 256) GO(256); else GO(512);
-#undef GO
+    hipLaunchKernelGGL(block_plan_kernel, dim3(p.pools, d->B * d->Hkv), dim3(POOL), 0, st, blocks, offs, rows, d->Lq, d->Hq, a.G, d->top, a.nblk, p.pools);
     DM_CHECK_LAUNCH();
   }
   const long rows = (long)d->B * d->Hq * d->Lq;
-  const dim3 grid(d->B * d->Hkv * a.pools);
-  switch (pool) {
-    case 0: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a)); break;
-    case 128: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 128>), grid, dim3(128), 0, st, a)); break;
-    case 256: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 256>), grid, dim3(256), 0, st, a)); break;
-    default: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, 512>), grid, dim3(512), 0, st, a)); break;
-  }
+  if (pool) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
+  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a))
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -942,15 +973,10 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   a.dvb = d->dv_stride[0]; a.dvl = d->dv_stride[1]; a.dvh = d->dv_stride[2];
   hipStream_t st = (hipStream_t)stream;
   const long rows = (long)d->B * d->Hq * d->Lq;
-  const dim3 grid(d->B * d->Hkv * a.pools);
-  switch (pool_rows(d)) {
-    case 0: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows)); break;
-    case 128: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 128>), grid, dim3(128), 0, st, a)); break;
-    case 256: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 256>), grid, dim3(256), 0, st, a)); break;
-    default: BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD, 512>), grid, dim3(512), 0, st, a)); break;
-  }
+  if (pooled(d)) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
+  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a, p.pool));
+  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a));
   DM_CHECK_LAUNCH();
   return DM_OK;
 }

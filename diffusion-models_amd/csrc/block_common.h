@@ -69,7 +69,7 @@ template <int D>
 __device__ __forceinline__ int acc_at(int r, int c) {
   if constexpr (D == 64) return r * 64 + ((c ^ (r & 15)) << 2);
   else if constexpr (D == 32) return r * 32 + ((c ^ (r & 7)) << 2);
-  else return r * 16 + (c << 2);
+  else return r * 16 + ((c ^ ((r >> 2) & 3)) << 2);
 }
 
 // 4 consecutive rows (row0 + 4 (lane >> 4) ...) of one feature (16 dt + (lane & 15)) for every lane
@@ -82,18 +82,32 @@ __device__ __forceinline__ bf16x4_t read_tr(const char* base, int row0, int dt, 
 __device__ __forceinline__ bf16x8_t join4(bf16x4_t a, bf16x4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // operand of a product over features: the row's KS pieces of 8 (or, up to 16 features, its piece of 4)
+template <int D> struct Piece { typedef bf16x8_t type; typedef __attribute__((ext_vector_type(4))) unsigned bits; };
+template <> struct Piece<8> { typedef bf16x4_t type; typedef __attribute__((ext_vector_type(2))) unsigned bits; };
+template <> struct Piece<16> : Piece<8> {};
 template <int D>
 struct Frag {
-  bf16x8_t x[Geo<D>::KS];
+  static constexpr int W = D <= 16 ? 4 : 8;
+  typedef typename Piece<D>::type piece_t;
+  piece_t x[Geo<D>::KS];
   // p: the row, g = lane >> 4
   __device__ __forceinline__ void load(const bf16_t* p, int g) {
-    if constexpr (D <= 16) {
-      const bf16x4_t z = {}, v = D == 16 || g < 2 ? *(const bf16x4_t*)(p + g * 4) : z;
-      x[0] = join4(v, z);
-    } else {
 #pragma unroll
-      for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const bf16x8_t*)(p + s * 32 + g * 8);
+    for (int s = 0; s < Geo<D>::KS; ++s) {
+      const piece_t none = {};
+      x[s] = D >= 16 || g < 2 ? *(const piece_t*)(p + s * 32 + g * W) : none;
     }
+  }
+  static __device__ __forceinline__ int place(int row, int s, int g) {   // byte offset of a lane's piece in an LDS row
+    return D <= 16 ? lds_at<D>(row, g >> 1) + (g & 1) * 8 : lds_at<D>(row, s * 4 + g);
+  }
+  __device__ __forceinline__ void from_lds(const char* base, int row, int g) {
+#pragma unroll
+    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const piece_t*)(base + place(row, s, g));
+  }
+  __device__ __forceinline__ void to_lds(char* base, int row, int g) const {
+#pragma unroll
+    for (int s = 0; s < Geo<D>::KS; ++s) *(piece_t*)(base + place(row, s, g)) = x[s];
   }
   // waits for the operand here and not behind younger loads (the compiler counts loads in order, and across branches all of them)
   __device__ __forceinline__ void arrived() {
@@ -101,32 +115,20 @@ struct Frag {
     for (int s = 0; s < Geo<D>::KS; ++s) asm volatile("" : "+v"(x[s]));
   }
   __device__ __forceinline__ void negate() {
-    typedef __attribute__((ext_vector_type(4))) unsigned bits_t;
 #pragma unroll
-    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = __builtin_bit_cast(bf16x8_t, __builtin_bit_cast(bits_t, x[s]) ^ 0x80008000u);
+    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = __builtin_bit_cast(piece_t, __builtin_bit_cast(typename Piece<D>::bits, x[s]) ^ 0x80008000u);
   }
   __device__ __forceinline__ void zero() {
-    const bf16x8_t z = {};
+    const piece_t none = {};
 #pragma unroll
-    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = z;
-  }
-  __device__ __forceinline__ void from_lds(const char* base, int row, int g) {
-    if constexpr (D <= 16) {
-      const bf16x4_t z = {};
-      x[0] = join4(*(const bf16x4_t*)(base + lds_at<D>(row, g >> 1) + (g & 1) * 8), z);
-    } else {
-#pragma unroll
-      for (int s = 0; s < Geo<D>::KS; ++s) x[s] = *(const bf16x8_t*)(base + lds_at<D>(row, s * 4 + g));
-    }
+    for (int s = 0; s < Geo<D>::KS; ++s) x[s] = none;
   }
 };
 template <int D>
 __device__ __forceinline__ f32x4_t dot_frag(const Frag<D>& a, const Frag<D>& b) {
   f32x4_t c = {0.f, 0.f, 0.f, 0.f};
   if constexpr (D <= 16) {
-    typedef __attribute__((ext_vector_type(4))) short half_t;
-    const bf16x4_t a4 = __builtin_shufflevector(a.x[0], a.x[0], 0, 1, 2, 3), b4 = __builtin_shufflevector(b.x[0], b.x[0], 0, 1, 2, 3);
-    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(half_t, a4), __builtin_bit_cast(half_t, b4), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a.x[0]), __builtin_bit_cast(s16x4_t, b.x[0]), c, 0, 0, 0);
   } else {
 #pragma unroll
     for (int s = 0; s < Geo<D>::KS; ++s) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.x[s], b.x[s], c, 0, 0, 0);

@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
 #pragma unroll
   for (int s = 0; s < Geo<D>::KS; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) qq += (float)qf.x[s][e] * (float)qf.x[s][e];
+    for (int e = 0; e < Frag<D>::W; ++e) qq += (float)qf.x[s][e] * (float)qf.x[s][e];
   qq = row_sum(qq);
   const int mine = 4 * (lane & 3) + ((lane & 15) >> 2);   // the block of a chunk of 16 that this lane fetches; it gets the scores of 4 e + g
   float best[K];

@@ -223,7 +223,7 @@ def rows_together(n):
 
 
 @gpu
-@pytest.mark.parametrize("pool", [0, 1, 128, 256, 512])
+@pytest.mark.parametrize("pool", [0, 1, 512])
 @pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", CASES)
 def test_block_attention(B, Lq, Lk, Hq, Hkv, D, top, ragged, pool):
     rows_together(pool)
@@ -245,7 +245,7 @@ def test_block_attention(B, Lq, Lk, Hq, Hkv, D, top, ragged, pool):
 
 
 @gpu
-@pytest.mark.parametrize("pool", [1, 128])
+@pytest.mark.parametrize("pool", [1, 512])
 def test_block_attention_of_one_sharp_weight(pool):
     """One key takes (almost) all the weight: ds is a small difference of large numbers."""
     rows_together(pool)
@@ -261,7 +261,7 @@ def test_block_attention_of_one_sharp_weight(pool):
 
 
 @gpu
-@pytest.mark.parametrize("pool", [1, 128])
+@pytest.mark.parametrize("pool", [1, 512])
 @pytest.mark.parametrize("scale", [-0.4, 0.0])
 def test_block_attention_of_a_scale_that_is_not_positive(scale, pool):
     rows_together(pool)
@@ -490,7 +490,7 @@ def test_refusals_of_the_c_abi():
     assert lib.dm_block_select(desc(q_stride=[2048, 33, 16]), p, p, None, p, None) == 1
     assert lib.dm_block_select(desc(), p, p, None, None, None) == 1
     assert lib.dm_block_attention_fwd(desc(), p, p, p, None, None, p, None, None, None, None) == 1
-    assert lib.dm_block_attention_fwd(desc(), p, p, p, p, None, p, None, None, None, None) == 1
+    assert lib.dm_block_attention_fwd(desc(pool=512), p, p, p, p, None, p, None, None, None, None) == 1
     assert "plan" in lib.dm_last_error().decode()
     assert lib.dm_block_attention_bwd(desc(), p, p, p, p, None, p, p, p, p, p, p, p, p, p, 8, None) == 1
     assert "workspace" in lib.dm_last_error().decode()
