@@ -29,51 +29,72 @@ struct Args {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// One query a workgroup: its blocks are dealt to the waves, whose partial results are joined through LDS. A block's keys
-// and values are read as whole rows, D/8 lanes a row with 16 bytes each; the lanes that hold a key's features also hold
-// the same features of its value, so a weight never moves between lanes. (The form for few queries.)
+// NW waves a query: its blocks are dealt to them and their partial results joined through LDS (NW = 4 where a sample has few
+// queries, else 1). A block's keys and values are read as whole rows, D/8 lanes a row with 16 bytes each, the next block's
+// while this one is computed; the lanes that hold a key's features also hold the same features of its value, so a
+// weight never moves between lanes.
 template <int D, int NW>
-__global__ __launch_bounds__(NW * 64) void attend_row_kernel(Args a) {
+__global__ __launch_bounds__(256) void attend_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
-  __shared__ float so[NW][D];
-  __shared__ float sm[NW], sl[NW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = blockIdx.x;
+  __shared__ float so[4][D], sm[4], sl[4];
+  const int lane = threadIdx.x & 63, w4 = threadIdx.x >> 6, wave = w4 % NW;
+  const long row = (long)blockIdx.x * (4 / NW) + w4 / NW;
+  if (row >= rows) return;   // (only without a join: 4 waves a query leave no remainder)
   const int i = row % a.Lq, h = (row / a.Lq) % a.Hq, b = row / ((long)a.Lq * a.Hq), hk = h / a.G;
   const int n = valid_keys(a.k_len, b, a.Lk);
   const int c = (lane % LPR) * 8, key = lane / LPR;
-  float q[8];
-  dm_unpack8(*(const bf16x8_t*)(a.q.p + b * a.q.sb + i * a.q.sl + h * a.q.sh + c), q);
+  const bf16x8_t q = *(const bf16x8_t*)(a.q.p + b * a.q.sb + i * a.q.sl + h * a.q.sh + c);
   const bf16_t* kp = a.k.p + b * a.k.sb + hk * a.k.sh + c;
   const bf16_t* vp = a.v.p + b * a.v.sb + hk * a.v.sh + c;
   const int listed = lane < a.top ? a.blocks[row * a.top + lane] : -1;
+  // which of the listed blocks count: in range, with a valid key, and not named before
+  bool first = listed >= 0 && listed < a.nblk && listed * BLK < n;
+  for (int t = 0; t < a.top - 1; ++t) first = first && !(t < lane && __builtin_amdgcn_readlane(listed, t) == listed);
+  unsigned long long todo = __ballot(first);
+  if (NW > 1) {   // every NW-th of them
+    unsigned long long left = todo, own = 0;
+    for (int x = 0; left; ++x) {
+      const unsigned long long bit = left & -left;
+      if (x % NW == wave) own |= bit;
+      left ^= bit;
+    }
+    todo = own;
+  }
   const float sc = a.scale * LOG2E;
-  float m = -INFINITY, l = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int t = wave; t < a.top; t += NW) {
-    const int j = __builtin_amdgcn_readlane(listed, t);
-    if (j < 0 || j >= a.nblk) continue;
-    if (__ballot(listed == j) & ((1ull << t) - 1)) continue;   // named before
-    const int n0 = n - j * BLK;
-    if (n0 <= 0) continue;
-    const bf16x8_t none = {};
-    bf16x8_t kk[NI], vv[NI];
+  const bf16x8_t none = {};
+  bf16x8_t kk[NI], vv[NI];
+  auto load = [&](int j) {
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      const long pos = (long)j * BLK + u * KPI + key;
-      kk[u] = u * KPI + key < n0 ? *(const bf16x8_t*)(kp + pos * a.k.sl) : none;
-      vv[u] = u * KPI + key < n0 ? *(const bf16x8_t*)(vp + pos * a.v.sl) : none;
+      const int t = u * KPI + key;
+      const long pos = (long)j * BLK + t;
+      const bool in = j * BLK + t < n;
+      kk[u] = in ? *(const bf16x8_t*)(kp + pos * a.k.sl) : none;
+      vv[u] = in ? *(const bf16x8_t*)(vp + pos * a.v.sl) : none;
     }
+  };
+  auto take = [&]() {
+    const int t = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    return __builtin_amdgcn_readlane(listed, t);
+  };
+  float m = -INFINITY, l = 0.f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  int j = -1;
+  if (todo) load(j = take());
+  while (j >= 0) {
+    const int n0 = n - j * BLK;
     float s[NI], mx = m;
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
-      float x[8], d = 0.f;
-      dm_unpack8(kk[u], x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d += q[e] * x[e];
-      d = group_sum<LPR>(d) * sc;
+      const float d = group_sum<LPR>(dot8(q, kk[u], 0.f)) * sc;
       s[u] = u * KPI + key < n0 ? d : -INFINITY;
       mx = fmaxf(mx, s[u]);
     }
+    bf16x8_t v[NI];
+#pragma unroll
+    for (int u = 0; u < NI; ++u) v[u] = vv[u];
+    j = -1;
+    if (todo) load(j = take());
     mx = across_max<LPR>(mx);
     const float base = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - base);
     m = mx;
@@ -84,7 +105,7 @@ __global__ __launch_bounds__(NW * 64) void attend_row_kernel(Args a) {
     for (int u = 0; u < NI; ++u) {
       const float p = __builtin_amdgcn_exp2f(s[u] - base);
       float x[8];
-      dm_unpack8(vv[u], x);
+      dm_unpack8(v[u], x);
       l += p;
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] += p * x[e];
@@ -93,29 +114,45 @@ __global__ __launch_bounds__(NW * 64) void attend_row_kernel(Args a) {
   l = across_sum<LPR>(l);
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = across_sum<LPR>(o[e]);
-  if (lane < LPR) {
+  if (NW > 1) {
+    if (lane < LPR) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) so[wave][c + e] = o[e];
-  }
-  if (lane == 0) { sm[wave] = m; sl[wave] = l; }
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float mx = -INFINITY, lt = 0.f, x = 0.f;
+      for (int e = 0; e < 8; ++e) so[wave][c + e] = o[e];
+    }
+    if (lane == 0) { sm[wave] = m; sl[wave] = l; }
+    __syncthreads();
+    if (wave) return;
+    float mt = -INFINITY, f[NW];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sm[w]);
-    const float base = mx == -INFINITY ? 0.f : mx;
+    for (int w = 0; w < NW; ++w) mt = fmaxf(mt, sm[w]);
+    const float base = mt == -INFINITY ? 0.f : mt;
+    l = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sm[w] - base);
-      lt += sl[w] * f;
-      x += so[w][threadIdx.x] * f;
+      f[w] = __builtin_amdgcn_exp2f(sm[w] - base);
+      l += sl[w] * f[w];
     }
-    const long at = (((long)b * a.Lq + i) * a.Hq + h) * D + threadIdx.x;
-    const float y = lt == 0.f ? 0.f : x / lt;
-    const bf16_t hi = (bf16_t)y;
-    a.out[at] = hi;
-    if (a.out_lo) a.out_lo[at] = (bf16_t)(y - (float)hi);
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = lt == 0.f ? -INFINITY : mx * LN2 + logf(lt);
+    m = mt;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) o[e] += so[w][c + e] * f[w];
+    }
+  }
+  if (lane < LPR) {
+    float lo[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = l == 0.f ? 0.f : o[e] / l;
+    const bf16x8_t y = dm_pack8(o);
+    const long at = (((long)b * a.Lq + i) * a.Hq + h) * D + c;
+    *(bf16x8_t*)(a.out + at) = y;
+    if (a.out_lo) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = o[e] - (float)y[e];
+      *(bf16x8_t*)(a.out_lo + at) = dm_pack8(lo);
+    }
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
   }
 }
 
@@ -868,13 +905,13 @@ int check_span(const char* who, const dm_block_desc* d) {
 }
 // Whether the rows are taken in pools on the matrix cores or one query a workgroup. A pool's time is the number of its visits (its
 // blocks) times what a visit takes from barrier to barrier, however few rows want the block: 1.1 us up to 32 features, 1.6 us with 64
-// (256 pools run at a time, twice as many up to 32 features); a query's is 2 ns + 0.2 .. 0.85 ns a block over the whole chip. Both sides
+// (256 pools run at a time, twice as many up to 32 features); a query's is 0.3 ns + 0.5 .. 0.8 ns a block over the whole chip. Both sides
 // measured, forward (us), one query a workgroup against pools:
-//   8 heads x 256 queries, 8 of 64 blocks       D 8  19 / 76       D 64  26 / 92
-//   4 x 8 heads x 256 queries, 8 of 64          D 8  42 / 78       D 64  81 / 92
-//   4 x 8 heads x 1024 queries, 4 of 16         D 8  103 / 37      D 64  174 / 46
-//   2 x 8 heads x 2048 queries, 8 of 128        D 8  146 / 144     D 64  297 / 177
-//   4 x 8 heads x 4096 queries, 8 of 64         D 8  568 / 96      D 64  1141 / 115
+//   8 heads x 256 queries, 8 of 64 blocks       D 8  20 / 69       D 64  26 / 90
+//   4 x 8 heads x 256 queries, 8 of 64          D 8  39 / 70       D 64  74 / 91
+//   4 x 8 heads x 1024 queries, 4 of 16         D 8  69 / 34       D 64  134 / 46
+//   2 x 8 heads x 2048 queries, 8 of 128        D 8  139 / 129     D 64  243 / 173
+//   4 x 8 heads x 4096 queries, 8 of 64         D 8  521 / 81      D 64  896 / 111
 // (Pools of 128 and 256 rows, which occupy more CUs where there are few rows, were never faster by more than 5 %.)
 bool pooled(const dm_block_desc* d) {
   if (d->pool) return d->pool == POOL;
@@ -882,7 +919,7 @@ bool pooled(const dm_block_desc* d) {
   const double rows = (double)d->Lq * (d->Hq / d->Hkv), heads = 4.0 * d->Hkv;
   const double pools = heads * ((long)(rows + POOL - 1) / POOL), rounds = (long)((pools + (d->D == 64 ? 255 : 511)) / (d->D == 64 ? 256 : 512));
   const double most = (rows < POOL ? rows : POOL) * d->top, visits = most < blocks_of(d) ? most : blocks_of(d);
-  return heads * rows * (2.0 + d->top * (0.2 + 0.01 * d->D)) > 6000.0 + rounds * visits * (d->D == 64 ? 1600.0 : 1100.0);
+  return heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 6000.0 + rounds * visits * (d->D == 64 ? 1600.0 : 1100.0);
 }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
 struct PlanLayout { int pools; size_t offs, bytes; };
@@ -937,7 +974,8 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   }
   const long rows = (long)d->B * d->Hq * d->Lq;
   if (pool) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
-  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a))
+  else if ((long)d->Hq * d->Lq < 512) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, rows))
+  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 1>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
   return DM_OK;
 }

@@ -35,11 +35,30 @@ __device__ __forceinline__ float group_sum(float x) {
   if constexpr (LPR > 4) x += lane_xor<4>(x);
   return x;
 }
-template <int LPR>   // over the lanes l, l + LPR, l + 2 LPR ...
+template <int O>   // lane distance 16 or 32: the other half's value
+__device__ __forceinline__ float half_xor(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  if constexpr (O == 16) { auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false); return __builtin_bit_cast(float, (unsigned)((threadIdx.x & 16) ? r[0] : r[1])); }
+  else { auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false); return __builtin_bit_cast(float, (unsigned)((threadIdx.x & 32) ? r[0] : r[1])); }
+}
+template <int LPR>   // over groups of LPR <= 8 lanes, each of which holds one value in all its lanes
 __device__ __forceinline__ float across_max(float x) {
+  if constexpr (LPR < 2) x = fmaxf(x, lane_xor<1>(x));
+  if constexpr (LPR < 4) x = fmaxf(x, lane_xor<2>(x));
+  if constexpr (LPR < 8) x = fmaxf(x, lane_xor<4>(x));
+  x = fmaxf(x, lane_xor<8>(x));
+  x = fmaxf(x, half_xor<16>(x));
+  return fmaxf(x, half_xor<32>(x));
+}
+// c + the products of 8 features, exact in fp32 but for the sum's roundings
+__device__ __forceinline__ float dot8(const bf16x8_t& a, const bf16x8_t& b, float c) {
 #pragma unroll
-  for (int o = LPR; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
+  for (int e = 0; e < 8; e += 2) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 pair_t;
+    const pair_t x = {a[e], a[e + 1]}, y = {b[e], b[e + 1]};
+    c = __builtin_amdgcn_fdot2_f32_bf16(x, y, c, false);
+  }
+  return c;
 }
 template <int LPR>
 __device__ __forceinline__ float across_sum(float x) {

@@ -23,9 +23,18 @@ int threads_per_row(int vecs) {
 }
 
 template <typename T, int V> struct Vec;
+template <typename T, int V> using Raw = T __attribute__((ext_vector_type(V)));   // as it lies in memory
 template <> struct Vec<float, 4> {
   static __device__ __forceinline__ void load(const float* p, float* f) { *(f32x4_t*)f = *(const f32x4_t*)p; }
   static __device__ __forceinline__ void store(float* p, const float* f) { *(f32x4_t*)p = *(const f32x4_t*)f; }
+};
+template <> struct Vec<float, 8> {
+  static __device__ __forceinline__ void load(const float* p, float* f) { *(f32x4_t*)f = *(const f32x4_t*)p; *(f32x4_t*)(f + 4) = *(const f32x4_t*)(p + 4); }
+  static __device__ __forceinline__ void store(float* p, const float* f) { *(f32x4_t*)p = *(const f32x4_t*)f; *(f32x4_t*)(p + 4) = *(const f32x4_t*)(f + 4); }
+};
+template <> struct Vec<bf16_t, 8> {
+  static __device__ __forceinline__ void load(const bf16_t* p, float* f) { dm_unpack8(*(const bf16x8_t*)p, f); }
+  static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *(bf16x8_t*)p = dm_pack8(f); }
 };
 template <> struct Vec<float, 1> {
   static __device__ __forceinline__ void load(const float* p, float* f) { *f = *p; }
@@ -49,20 +58,32 @@ template <> struct Vec<bf16_t, 1> {
   static __device__ __forceinline__ void store(bf16_t* p, const float* f) { *p = (bf16_t)*f; }
 };
 
-template <typename T, int V>
+// A thread copies V features of U rows: the U rows' loads are in flight together.
+template <typename T, int V, int U>
 __global__ __launch_bounds__(256) void token_embed_kernel(const float* __restrict__ table, const int64_t* __restrict__ tokens,
                                                           T* __restrict__ out, long n, long rows, int width, float scale, int tpr) {
-  const long i = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
-  if (i >= n) return;
-  const int64_t t = tokens[i];
-  const bool live = t >= 0 && t < rows;
-  const float* src = table + (live ? t : 0) * (long)width;
-  for (int e = (threadIdx.x & (tpr - 1)) * V; e < width; e += tpr * V) {
-    float f[V];
-    Vec<float, V>::load(src + e, f);
+  const int per = 256 / tpr;
+  const long i0 = (long)blockIdx.x * (per * U) + threadIdx.x / tpr;
+  const float* src[U];
+  bool live[U];
 #pragma unroll
-    for (int x = 0; x < V; ++x) f[x] = live ? f[x] * scale : 0.f;
-    Vec<T, V>::store(out + i * (long)width + e, f);
+  for (int u = 0; u < U; ++u) {
+    const long i = i0 + (long)u * per;
+    const int64_t t = i < n ? tokens[i] : -1;
+    live[u] = t >= 0 && t < rows;
+    src[u] = table + (live[u] ? t : 0) * (long)width;
+  }
+  for (int e = (threadIdx.x & (tpr - 1)) * V; e < width; e += tpr * V) {
+    float f[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<float, V>::load(src[u] + e, f[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long i = i0 + (long)u * per;
+#pragma unroll
+      for (int x = 0; x < V; ++x) f[u][x] = live[u] ? f[u][x] * scale : 0.f;
+      if (i < n) Vec<T, V>::store(out + i * (long)width + e, f[u]);
+    }
   }
 }
 
@@ -72,20 +93,21 @@ __device__ __forceinline__ unsigned key_of(const int64_t* tokens, long i, long r
   return t < 0 || t >= rows || t == padding ? (unsigned)rows : (unsigned)t;
 }
 
-// counts of the first digit in every tile; the later passes' counts are cleared (the pass before fills them)
-__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ tokens, unsigned* __restrict__ counts, long n,
-                                                         long rows, long padding, int tiles, int passes) {
+// counts of a pass's digit in every tile
+template <bool FIRST>
+__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ tokens, const unsigned* __restrict__ key_in,
+                                                         unsigned* __restrict__ counts, long n, long rows, long padding, int shift) {
   __shared__ unsigned c[RADIX];
   const int t = blockIdx.x, tid = threadIdx.x;
   c[tid] = 0;
   __syncthreads();
+#pragma unroll
   for (int u = 0; u < TILE / 256; ++u) {
     const long i = (long)t * TILE + u * 256 + tid;
-    if (i < n) atomicAdd(&c[key_of(tokens, i, rows, padding) & (RADIX - 1)], 1u);
+    if (i < n) atomicAdd(&c[((FIRST ? key_of(tokens, i, rows, padding) : key_in[i]) >> shift) & (RADIX - 1)], 1u);
   }
   __syncthreads();
   counts[(long)t * RADIX + tid] = c[tid];
-  for (int p = 1; p < passes; ++p) counts[((long)p * tiles + t) * RADIX + tid] = 0;
 }
 
 // One stable pass: a key's place is (keys of smaller digits) + (keys of its digit in earlier tiles, waves and lanes).
@@ -93,8 +115,8 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restri
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restrict__ tokens, const unsigned* __restrict__ key_in,
                                                         const unsigned* __restrict__ idx_in, unsigned* __restrict__ key_out,
-                                                        unsigned* __restrict__ idx_out, const unsigned* __restrict__ counts,
-                                                        unsigned* __restrict__ next, long n, long rows, long padding, int tiles, int shift) {
+                                                        unsigned* __restrict__ idx_out, const unsigned* __restrict__ counts, long n,
+                                                        long rows, long padding, int tiles, int shift) {
   __shared__ unsigned base[RADIX], wcount[4][RADIX];
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
@@ -161,55 +183,60 @@ __global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restric
     const unsigned to = wcount[wave][(key[u] >> shift) & (RADIX - 1)] + rank[u];
     key_out[to] = key[u];
     idx_out[to] = idx[u];
-    if (next) atomicAdd(&next[(long)(to / TILE) * RADIX + ((key[u] >> (shift + 8)) & (RADIX - 1))], 1u);
   }
 }
 
 // Sums of runs of equal keys inside one chunk of the sorted order. A run that lies inside the chunk goes to its row; the
 // part of a run that began before the chunk, and the part of one that goes on behind it, are left in part[chunk][0 / 1].
+// `chunk` <= MAX_CHUNK neighbouring positions a group of tpr threads, U rows' loads in flight at a time.
+constexpr int MAX_CHUNK = 64;
+template <int V>
+__device__ __forceinline__ void finish_row(float* to, const float* s, float scale, int accumulate) {
+  float g[V];
+  if (accumulate) Vec<float, V>::load(to, g);
+#pragma unroll
+  for (int x = 0; x < V; ++x) g[x] = accumulate ? g[x] + s[x] * scale : s[x] * scale;
+  Vec<float, V>::store(to, g);
+}
 template <typename T, int V>
 __global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout, const unsigned* __restrict__ key,
                                                       const unsigned* __restrict__ idx, float* __restrict__ dtable, float* __restrict__ part,
-                                                      long n, unsigned rows, int width, float scale, int tpr, int chunk) {
-  const long c = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
+                                                      long n, unsigned rows, int width, float scale, int tpr, int chunk, int accumulate) {
+  // the keys of the workgroup's chunks and of one position on either side; 256 / tpr chunks of at most 64, or of 16 (small calls)
+  __shared__ unsigned skey[4096 + 2], sidx[4096];
+  const int per = 256 / tpr, all = per * chunk;
+  const long first = (long)blockIdx.x * all;
+  for (int x = threadIdx.x; x < all + 2; x += 256) {
+    const long p = first + x - 1;
+    skey[x] = p >= 0 && p < n ? key[p] : 0xffffffffu;   // (no key: keys are at most `rows` < 2^31)
+    if (x >= 1 && x <= all) sidx[x - 1] = p < n ? idx[p] : 0;
+  }
+  __syncthreads();
+  const int c = threadIdx.x / tpr, p0 = c * chunk, p1 = (int)min((long)(p0 + chunk), n - first);
   const int e = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * V;
-  const long p0 = c * chunk, p1 = min(p0 + chunk, n);
-  if (p0 >= n || e >= width) return;
+  if (p0 >= p1 || e >= width) return;
   constexpr int U = 8;
   float s[V];
 #pragma unroll
   for (int x = 0; x < V; ++x) s[x] = 0.f;
-  bool began = p0 == 0 || key[p0 - 1] != key[p0];   // the current run began in this chunk
-  for (long p = p0; p < p1; p += U) {
-    float f[U][V];
-    unsigned k[U + 1];
+  bool began = skey[p0] != skey[p0 + 1];   // the current run began in this chunk
+  for (int p = p0; p < p1; p += U) {
+    if (skey[p + 1] >= rows) break;        // only positions without a gradient follow
+    T raw[U][V];
 #pragma unroll
-    for (int u = 0; u <= U; ++u) k[u] = p + u < n ? key[p + u] : 0xffffffffu;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool on = p + u < p1 && k[u] < rows;
-      if (on) Vec<T, V>::load(dout + (long)idx[p + u] * width + e, f[u]);
-      else
-#pragma unroll
-        for (int x = 0; x < V; ++x) f[u][x] = 0.f;
-    }
+    for (int u = 0; u < U; ++u)
+      if (p + u < p1) *(Raw<T, V>*)raw[u] = *(const Raw<T, V>*)(dout + (long)sidx[p + u] * width + e);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (p + u >= p1 || k[u] >= rows) break;
+      if (p + u >= p1) break;
+      const unsigned k = skey[p + u + 1];
+      if (k >= rows) break;
 #pragma unroll
-      for (int x = 0; x < V; ++x) s[x] += f[u][x];
-      const bool last = p + u + 1 >= p1, ends = k[u + 1] != k[u];
-      if (ends || last) {
-        if (began && ends) {
-          float* to = dtable + (long)k[u] * width + e;
-          float g[V];
-          Vec<float, V>::load(to, g);
-#pragma unroll
-          for (int x = 0; x < V; ++x) g[x] += s[x] * scale;
-          Vec<float, V>::store(to, g);
-        } else {
-          Vec<float, V>::store(part + (c * 2 + (began ? 1 : 0)) * (long)width + e, s);
-        }
+      for (int x = 0; x < V; ++x) s[x] += (float)raw[u][x];
+      const bool ends = skey[p + u + 2] != k;
+      if (ends || p + u + 1 >= p1) {
+        if (began && ends) finish_row<V>(dtable + (long)k * width + e, s, scale, accumulate);
+        else Vec<float, V>::store(part + (((long)blockIdx.x * per + c) * 2 + (began ? 1 : 0)) * (long)width + e, s);
 #pragma unroll
         for (int x = 0; x < V; ++x) s[x] = 0.f;
         began = true;
@@ -222,7 +249,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout
 template <int V>
 __global__ __launch_bounds__(256) void run_join_kernel(const unsigned* __restrict__ key, const float* __restrict__ part,
                                                        float* __restrict__ dtable, long n, unsigned rows, int width, float scale, int tpr,
-                                                       int chunk) {
+                                                       int chunk, int accumulate) {
   const long c = (long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   const int e = (blockIdx.y * tpr + (threadIdx.x & (tpr - 1))) * V;
   const long p0 = c * chunk, p1 = p0 + chunk;
@@ -230,23 +257,34 @@ __global__ __launch_bounds__(256) void run_join_kernel(const unsigned* __restric
   const unsigned k = key[p1 - 1];
   if (k >= rows || key[p1] != k) return;
   if (key[p0] == k && p0 > 0 && key[p0 - 1] == k) return;   // began before this chunk
+  long lo = c + 1, hi = (n + chunk - 1) / chunk;            // the first chunk behind that does not begin with the run
+  while (lo < hi) {
+    const long mid = (lo + hi) / 2;
+    if (key[mid * chunk] == k) lo = mid + 1;
+    else hi = mid;
+  }
   float s[V];
   Vec<float, V>::load(part + (c * 2 + 1) * (long)width + e, s);
-  for (long x = c + 1; x * chunk < n && key[x * chunk] == k; ++x) {
-    float f[V];
-    Vec<float, V>::load(part + x * 2 * (long)width + e, f);
+  constexpr int U = 16;
+  for (long x = c + 1; x < lo; x += U) {
+    float f[U][V];
 #pragma unroll
-    for (int y = 0; y < V; ++y) s[y] += f[y];
+    for (int u = 0; u < U; ++u)
+      if (x + u < lo) Vec<float, V>::load(part + (x + u) * 2 * (long)width + e, f[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (x + u < lo) {
+#pragma unroll
+        for (int y = 0; y < V; ++y) s[y] += f[u][y];
+      }
   }
-  float* to = dtable + (long)k * width + e;
-  float g[V];
-  Vec<float, V>::load(to, g);
-#pragma unroll
-  for (int x = 0; x < V; ++x) g[x] += s[x] * scale;
-  Vec<float, V>::store(to, g);
+  finish_row<V>(dtable + (long)k * width + e, s, scale, accumulate);
 }
 
-int chunk_of(long n) { return n >= 65536 ? 64 : 16; }
+int chunk_of(long n) { return n >= 65536 ? MAX_CHUNK : 16; }
+
+// (at least 4 threads a row: a workgroup's chunks, 256 / threads of them, fit its LDS)
+int sum_threads(int vecs) { return threads_per_row(vecs) < 4 ? 4 : threads_per_row(vecs); }
 
 struct Plan {   // parts of the workspace, in bytes
   long tiles, chunks;
@@ -263,7 +301,7 @@ Plan plan_of(long n, long rows, int width) {
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   for (int i = 0; i < 2; ++i) { p.key[i] = take(n * 4); p.idx[i] = take(n * 4); }
-  p.counts = take((size_t)p.passes * p.tiles * RADIX * 4);
+  p.counts = take((size_t)p.tiles * RADIX * 4);
   p.part = take((size_t)p.chunks * 2 * width * 4);
   p.total = at;
   return p;
@@ -275,8 +313,10 @@ int check_embed(const char* who, long n, long rows, int width) {
   DM_REQUIRE(width > 0 && width <= 65536, DM_ERR_SHAPE, "%s: width %d (1 to 65536)", who, width);
   return DM_OK;
 }
-bool vectors(int width, const void* a, const void* b) {
-  return width % 4 == 0 && (((uintptr_t)a | (uintptr_t)b) & 15) == 0;
+// features a thread handles at a time: 16 bytes of the bf16 side, or of fp32; 1 where rows or bases are not aligned
+int vectors(int width, const void* a, const void* b, int bf16) {
+  if (width % 4 || (((uintptr_t)a | (uintptr_t)b) & 15)) return 1;
+  return bf16 && width % 8 == 0 ? 8 : 4;
 }
 
 }  // namespace
@@ -288,13 +328,16 @@ extern "C" int dm_token_embed(const float* table, const int64_t* tokens, void* o
   if (rc) return rc;
   if (n == 0) return DM_OK;
   DM_REQUIRE(table && tokens && out, DM_ERR_ARG, "%s: null pointer", who);
-  const bool vec = vectors(width, table, out);
-  const int tpr = threads_per_row(vec ? width / 4 : width);
-  const dim3 grid(dm_cdiv(n, 256 / tpr)), block(256);
+  const int V = vectors(width, table, out, out_bf16);
+  const int tpr = threads_per_row(width / V);
+  const int U = n / (256 / tpr) >= 8192 ? 4 : 1;   // 4 rows a thread once that leaves 8 workgroups a CU (131072 rows of 1024: 129 -> 105 us)
+  const dim3 grid(dm_cdiv(n, 256 / tpr * U)), block(256);
   hipStream_t st = (hipStream_t)stream;
-#define GO(T, V) hipLaunchKernelGGL((token_embed_kernel<T, V>), grid, block, 0, st, table, tokens, (T*)out, n, rows, width, scale, tpr)
-  if (out_bf16) { if (vec) GO(bf16_t, 4); else GO(bf16_t, 1); }
-  else { if (vec) GO(float, 4); else GO(float, 1); }
+#define GO(T, V, U) hipLaunchKernelGGL((token_embed_kernel<T, V, U>), grid, block, 0, st, table, tokens, (T*)out, n, rows, width, scale, tpr)
+#define GO_U(T, V) do { if (U == 4) GO(T, V, 4); else GO(T, V, 1); } while (0)
+  if (out_bf16) { if (V == 8) GO_U(bf16_t, 8); else if (V == 4) GO_U(bf16_t, 4); else GO_U(bf16_t, 1); }
+  else { if (V == 4) GO_U(float, 4); else GO_U(float, 1); }
+#undef GO_U
 #undef GO
   DM_CHECK_LAUNCH();
   return DM_OK;
@@ -306,7 +349,7 @@ extern "C" size_t dm_token_embed_bwd_ws_bytes(long n, long rows, int width) {
 }
 
 extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t* tokens, float* dtable, long n, long rows, int width,
-                                  float scale, long padding, void* ws, size_t ws_bytes, void* stream) {
+                                  float scale, long padding, int accumulate, void* ws, size_t ws_bytes, void* stream) {
   const char* who = "dm_token_embed_bwd";
   int rc = check_embed(who, n, rows, width);
   if (rc) return rc;
@@ -320,29 +363,29 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   float* part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
-  hipLaunchKernelGGL(sort_count_kernel, tiles, block, 0, st, tokens, counts, n, rows, padding, (int)p.tiles, p.passes);
-  DM_CHECK_LAUNCH();
   for (int i = 0; i < p.passes; ++i) {
-    unsigned* now = counts + (long)i * p.tiles * RADIX;
-    unsigned* next = i + 1 < p.passes ? now + p.tiles * RADIX : nullptr;
-    if (i == 0)
-      hipLaunchKernelGGL((sort_pass_kernel<true>), tiles, block, 0, st, tokens, nullptr, nullptr, key[0], idx[0], now, next, n, rows, padding, (int)p.tiles, 0);
-    else
-      hipLaunchKernelGGL((sort_pass_kernel<false>), tiles, block, 0, st, tokens, key[(i - 1) & 1], idx[(i - 1) & 1], key[i & 1], idx[i & 1], now, next, n, rows, padding, (int)p.tiles, 8 * i);
+    const unsigned *ki = key[(i + 1) & 1], *ii = idx[(i + 1) & 1];
+    unsigned *ko = key[i & 1], *io = idx[i & 1];
+    if (i == 0) hipLaunchKernelGGL((sort_count_kernel<true>), tiles, block, 0, st, tokens, nullptr, counts, n, rows, padding, 0);
+    else hipLaunchKernelGGL((sort_count_kernel<false>), tiles, block, 0, st, nullptr, ki, counts, n, rows, padding, 8 * i);
+    DM_CHECK_LAUNCH();
+    if (i == 0) hipLaunchKernelGGL((sort_pass_kernel<true>), tiles, block, 0, st, tokens, nullptr, nullptr, ko, io, counts, n, rows, padding, (int)p.tiles, 0);
+    else hipLaunchKernelGGL((sort_pass_kernel<false>), tiles, block, 0, st, nullptr, ki, ii, ko, io, counts, n, rows, padding, (int)p.tiles, 8 * i);
     DM_CHECK_LAUNCH();
   }
   const unsigned *sk = key[(p.passes - 1) & 1], *si = idx[(p.passes - 1) & 1];
-  const bool vec = vectors(width, dout, dtable);
-  const int vecs = vec ? width / 4 : width, tpr = threads_per_row(vecs), chunk = chunk_of(n);
-  const dim3 grid(dm_cdiv(p.chunks, 256 / tpr), dm_cdiv(vecs, tpr));
-#define GO(T, V) hipLaunchKernelGGL((run_sum_kernel<T, V>), grid, block, 0, st, (const T*)dout, sk, si, dtable, part, n, (unsigned)rows, width, scale, tpr, chunk)
-  if (dout_bf16) { if (vec) GO(bf16_t, 4); else GO(bf16_t, 1); }
-  else { if (vec) GO(float, 4); else GO(float, 1); }
+  const int V = vectors(width, dout, dtable, dout_bf16), tpr = sum_threads(width / V), chunk = chunk_of(n);
+  const dim3 grid(dm_cdiv(p.chunks, 256 / tpr), dm_cdiv(width / V, tpr));
+#define GO(T, V) hipLaunchKernelGGL((run_sum_kernel<T, V>), grid, block, 0, st, (const T*)dout, sk, si, dtable, part, n, (unsigned)rows, width, scale, tpr, chunk, accumulate)
+  if (dout_bf16) { if (V == 8) GO(bf16_t, 8); else if (V == 4) GO(bf16_t, 4); else GO(bf16_t, 1); }
+  else { if (V == 4) GO(float, 4); else GO(float, 1); }
 #undef GO
   DM_CHECK_LAUNCH();
   if (p.chunks > 1) {
-    if (vec) hipLaunchKernelGGL((run_join_kernel<4>), grid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, tpr, chunk);
-    else hipLaunchKernelGGL((run_join_kernel<1>), grid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, tpr, chunk);
+    const int W = V == 1 ? 1 : 4, t = sum_threads(width / W);   // (the parts are fp32 whatever dout is)
+    const dim3 jgrid(dm_cdiv(p.chunks, 256 / t), dm_cdiv(width / W, t));
+    if (W == 4) hipLaunchKernelGGL((run_join_kernel<4>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate);
+    else hipLaunchKernelGGL((run_join_kernel<1>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate);
     DM_CHECK_LAUNCH();
   }
   return DM_OK;

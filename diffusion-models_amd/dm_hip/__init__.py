@@ -107,7 +107,7 @@ _SIGNATURES = {
     "dm_block_attention_bwd": (c_int, [P] * 15 + [ctypes.c_size_t, P]),
     "dm_token_embed": (c_int, [P, P, P, c_int, c_long, c_long, c_int, c_float, P]),
     "dm_token_embed_bwd_ws_bytes": (ctypes.c_size_t, [c_long, c_long, c_int]),
-    "dm_token_embed_bwd": (c_int, [P, c_int, P, P, c_long, c_long, c_int, c_float, c_long, P, ctypes.c_size_t, P]),
+    "dm_token_embed_bwd": (c_int, [P, c_int, P, P, c_long, c_long, c_int, c_float, c_long, c_int, P, ctypes.c_size_t, P]),
     "dm_timestep_embed": (c_int, [P, P, P, c_int, c_int, P]),
     "dm_linear_fwd": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, P]),
     "dm_linear_bwd": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, P]),

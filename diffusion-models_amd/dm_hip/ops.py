@@ -218,7 +218,7 @@ def _stream():
     that the consumer of the gradients has to wait for."""
     global LAUNCHES
     LAUNCHES += 1
-    raw = torch.cuda.current_stream().cuda_stream
+    raw = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())   # (current_stream().cuda_stream without the object)
     if _AUX:
         s = _AUX.get(raw)
         if s is not None:
@@ -1104,7 +1104,7 @@ class _TokenEmbedFn(Function):
                 need = lib.dm_token_embed_bwd_ws_bytes(n, rows, width)
                 ws = _scratch(dout.device, (need + 3) // 4)
                 check(lib.dm_token_embed_bwd(dout.data_ptr(), int(dout.dtype == BF16), tokens.data_ptr(), dtable.data_ptr(), n, rows,
-                                             width, scale, padding, ws.data_ptr(), need, _stream()))
+                                             width, scale, padding, int(sink is not None), ws.data_ptr(), need, _stream()))
         if sink is not None:
             _grad_done(ctx.param)
             return None, None, None, None, None

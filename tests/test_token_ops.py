@@ -384,6 +384,9 @@ def test_block_attention_same_bits_whatever_the_batch():
     (2049, 257, 64, 0, "float32", -2.0),
     (5000, 70000, 12, 3, "bfloat16", 1.0),      # three sort passes
     (30000, 2, 8, None, "float32", 1.0),        # two runs over nearly every chunk
+    (66000, 3, 1, None, "bfloat16", 1.0),       # one feature; long chunks and joins of many parts
+    (3000, 5000, 2, 7, "float32", 1.0),
+    (40000, 33, 1024, 5, "float32", 1.0),       # four rows a thread
     (70000, 900, 260, 1, "bfloat16", 22.0),     # the longer chunks of large calls
     (400, 50, 1500, None, "float32", 1.0),      # more features than one workgroup takes
 ])
@@ -502,7 +505,7 @@ def test_refusals_of_the_c_abi():
     assert lib.dm_token_embed(p, p, p, 0, 5, 9, 0, 1.0, None) == 2
     assert lib.dm_token_embed(p, None, p, 0, 5, 9, 4, 1.0, None) == 1
     assert lib.dm_token_embed(None, None, None, 0, 0, 9, 4, 1.0, None) == 0
-    assert lib.dm_token_embed_bwd(p, 0, p, p, 5, 9, 4, 1.0, -1, p, 16, None) == 1
+    assert lib.dm_token_embed_bwd(p, 0, p, p, 5, 9, 4, 1.0, -1, 1, p, 16, None) == 1
     assert lib.dm_token_embed_bwd_ws_bytes(5, 9, -1) == 0
 
 
