@@ -186,6 +186,99 @@ __global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restric
   }
 }
 
+// The whole sort of a small call in one launch: the same passes, by one workgroup in LDS
+constexpr int SMALL = 8192;
+__global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ tokens, unsigned* __restrict__ key_out,
+                                                          unsigned* __restrict__ idx_out, int n, long rows, long padding, int passes) {
+  __shared__ unsigned skey[SMALL];
+  __shared__ unsigned short sidx[SMALL], wcount[16][RADIX];
+  __shared__ unsigned wsum[4];
+  constexpr int ROUNDS = SMALL / 1024;
+  const int span = (n + 1023) / 1024 * 64;   // a wave's neighbouring keys
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = wave * span + lane, rounds = span / 64;
+  unsigned key[ROUNDS], idx[ROUNDS], rank[ROUNDS];
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const int i = first + u * 64;
+    if (u >= rounds) break;
+    key[u] = i < n ? key_of(tokens, i, rows, padding) : 0;
+    idx[u] = i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = 8 * pass;
+    for (int x = tid; x < 16 * RADIX / 2; x += 1024) ((unsigned*)&wcount[0][0])[x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+      if (u >= rounds) break;
+      const bool in = first + u * 64 < n;
+      const unsigned d = (key[u] >> shift) & (RADIX - 1);
+      unsigned long long same = __ballot(in);
+#pragma unroll
+      for (int bit = 0; bit < 8; ++bit) {
+        const bool one = (d >> bit) & 1;
+        const unsigned long long m = __ballot(one);
+        same &= one ? m : ~m;
+      }
+      const int lower = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+      const unsigned have = wcount[wave][d];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // as in the pass above
+      rank[u] = have + lower;
+      if (in && lower == 0) wcount[wave][d] = (unsigned short)(have + __builtin_popcountll(same));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    unsigned total = 0, inc = 0;
+    if (tid < RADIX) {
+#pragma unroll
+      for (int w = 0; w < 16; ++w) total += wcount[w][tid];
+      inc = total;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const unsigned up = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 63) wsum[wave] = inc;
+    }
+    __syncthreads();
+    if (tid < RADIX) {
+      unsigned at = inc - total;
+#pragma unroll
+      for (int w = 0; w < 3; ++w) at += w < wave ? wsum[w] : 0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const unsigned c = wcount[w][tid];
+        wcount[w][tid] = (unsigned short)at;   // (places are below 8192)
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+      if (u >= rounds || first + u * 64 >= n) break;
+      const unsigned to = wcount[wave][(key[u] >> shift) & (RADIX - 1)] + rank[u];
+      skey[to] = key[u];
+      sidx[to] = (unsigned short)idx[u];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+      const int i = first + u * 64;
+      if (u >= rounds) break;
+      key[u] = i < n ? skey[i] : 0;
+      idx[u] = i < n ? sidx[i] : 0;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const int i = first + u * 64;
+    if (u < rounds && i < n) {
+      key_out[i] = key[u];
+      idx_out[i] = idx[u];
+    }
+  }
+}
+
 // Sums of runs of equal keys inside one chunk of the sorted order. A run that lies inside the chunk goes to its row; the
 // part of a run that began before the chunk, and the part of one that goes on behind it, are left in part[chunk][0 / 1].
 // `chunk` <= MAX_CHUNK neighbouring positions a group of tpr threads, U rows' loads in flight at a time.
@@ -363,7 +456,12 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   float* part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
-  for (int i = 0; i < p.passes; ++i) {
+  // one workgroup up to 8192 tokens (4999 tokens, two passes: 20 us in 4 launches)
+  if (n <= SMALL) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, st, tokens, key[(p.passes - 1) & 1], idx[(p.passes - 1) & 1], (int)n, rows, padding, p.passes);
+    DM_CHECK_LAUNCH();
+  }
+  for (int i = 0; i < p.passes && n > SMALL; ++i) {
     const unsigned *ki = key[(i + 1) & 1], *ii = idx[(i + 1) & 1];
     unsigned *ko = key[i & 1], *io = idx[i & 1];
     if (i == 0) hipLaunchKernelGGL((sort_count_kernel<true>), tiles, block, 0, st, tokens, nullptr, counts, n, rows, padding, 0);

@@ -383,6 +383,9 @@ def test_block_attention_same_bits_whatever_the_batch():
     (2048, 256, 20, None, "bfloat16", 1.0),
     (2049, 257, 64, 0, "float32", -2.0),
     (5000, 70000, 12, 3, "bfloat16", 1.0),      # three sort passes
+    (8192, 3000, 8, None, "float32", 1.0),      # the largest call that one workgroup sorts
+    (8193, 70000, 8, 2, "float32", 1.0),        # ... and the smallest that it does not
+    (9000, 2 ** 24 + 5, 4, 2, "float32", 1.0),  # four passes
     (30000, 2, 8, None, "float32", 1.0),        # two runs over nearly every chunk
     (66000, 3, 1, None, "bfloat16", 1.0),       # one feature; long chunks and joins of many parts
     (3000, 5000, 2, 7, "float32", 1.0),
