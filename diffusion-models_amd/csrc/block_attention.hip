@@ -669,15 +669,26 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
         for (int e = 0; e < 16; ++e)
           if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) ds[e] = 0.f;
       }
-      bf16x8_t p[2];
+      // ds sums to zero over a row's keys, so what its keys have in common cancels in dq: rounded to bf16 it would not, by 2^-9 of
+      // the common part. Two bf16 operands, the rounded ds and what the rounding lost, keep 2^-17.
+      bf16x8_t p[2], lost[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) p[u] = dm_pack8(ds + u * 8);   // rounded as the matrix instruction's operand
+      for (int u = 0; u < 2; ++u) {
+        p[u] = dm_pack8(ds + u * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ds[u * 8 + e] -= (float)p[u][e];
+        lost[u] = dm_pack8(ds + u * 8);
+      }
       const bool live = w.live(it);
 #pragma unroll
       for (int dt = 0; dt < GE::DT; ++dt) {
         f32x4_t c = o[dt];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(tr[dt][2 * u], tr[dt][2 * u + 1]), p[u], c, 0, 0, 0);
+        for (int u = 0; u < 2; ++u) {
+          const bf16x8_t keys = join4(tr[dt][2 * u], tr[dt][2 * u + 1]);
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, p[u], c, 0, 0, 0);
+          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, lost[u], c, 0, 0, 0);
+        }
         if (live) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = c;
       }
       it = it1;
