@@ -50,9 +50,9 @@ __global__ __launch_bounds__(256) void block_keys_kernel(Rows k, const int* __re
 // ---------------------------------------------------------------------------------------------------------------
 // The choice of blocks. Scores are compared as 64-bit sums; two ways to get there:
 //
-// exact_top: one query a wave, all scores in 64 bits, EXACT_CHUNK blocks at a time beside the best of the earlier ones. A
+// exact_top: a query at a time, all scores in 64 bits, EXACT_CHUNK blocks at a time beside the best of the earlier ones. A
 // score becomes an unsigned number of the same order (NaN: that of -infinity), 0 stands for a block already taken.
-constexpr int EXACT_CHUNK = 512;
+constexpr int EXACT_CHUNK = 256;
 template <int O>
 __device__ __forceinline__ unsigned lane_xor_u(unsigned x) {   // as lane_xor, and O = 16, 32 (whole-wave reductions)
   if constexpr (O == 16) { auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); return (threadIdx.x & 16) ? r[0] : r[1]; }
@@ -67,47 +67,72 @@ __device__ __forceinline__ void take_best(unsigned long long& key, int& j) {
 }
 constexpr int NO_BLOCK = 0x7fffffff;
 
-// lane t's return value: the t-th block taken, or NO_BLOCK
-template <int D>
-__device__ int exact_top(const bf16_t* qp, const bf16_t* kp, int have, int top, unsigned long long* buf, int lane) {
-  unsigned long long won = 0;    // lane t: the t-th best of the chunks so far
-  int won_j = NO_BLOCK;
-  for (int c0 = 0; c0 < have; c0 += EXACT_CHUNK) {
-    const int n = min(EXACT_CHUNK, have - c0);
-    for (int x = lane; x < n; x += 64) {
-      double s = 0;
-#pragma unroll 2
-      for (int d = 0; d < D; d += 8) {
-        const bf16x8_t a = *(const bf16x8_t*)(qp + d), b = *(const bf16x8_t*)(kp + (long)(c0 + x) * D + d);
+// The `top` best of what the wave's lanes hold (PER candidates a lane, and one more, won / won_j), best first: the t-th goes to
+// lane t's won / won_j.
+template <int PER>
+__device__ __forceinline__ void keep_best(unsigned long long (&score)[PER], const int (&place)[PER], int top, int lane,
+                                          unsigned long long& won, int& won_j) {
+  unsigned long long next = 0;
+  int next_j = NO_BLOCK;
+  for (int t = 0; t < top; ++t) {
+    unsigned long long key = won;
+    int j = won_j;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += (double)(float)a[e] * (double)(float)b[e];
-      }
-      s = s == s ? s + 0.0 : -INFINITY;   // (-0 and 0 are equal)
-      const unsigned long long u = __builtin_bit_cast(unsigned long long, s);
-      buf[x] = (u >> 63) ? ~u : u | 0x8000000000000000ull;
-    }
-    unsigned long long next = 0;
-    int next_j = NO_BLOCK;
-    for (int t = 0; t < top; ++t) {
-      unsigned long long key = won;
-      int j = won_j;
-      for (int x = lane; x < n; x += 64)
-        if (buf[x] > key) { key = buf[x]; j = c0 + x; }   // (earlier chunks have the lower numbers: ties stay with them)
-      take_best<1>(key, j);
-      take_best<2>(key, j);
-      take_best<4>(key, j);
-      take_best<8>(key, j);
-      take_best<16>(key, j);
-      take_best<32>(key, j);
-      if (!key) break;
-      if (lane == t) { next = key; next_j = j; }
-      if (won_j == j) won = 0;
-      if (j >= c0 && ((j - c0) & 63) == lane) buf[j - c0] = 0;   // (a lane reads only what it wrote)
-    }
-    won = next;
-    won_j = next_j;
+    for (int u = 0; u < PER; ++u)
+      if (score[u] > key || (score[u] == key && place[u] < j)) { key = score[u]; j = place[u]; }
+    take_best<1>(key, j);
+    take_best<2>(key, j);
+    take_best<4>(key, j);
+    take_best<8>(key, j);
+    take_best<16>(key, j);
+    take_best<32>(key, j);
+    if (!key) break;
+    if (lane == t) { next = key; next_j = j; }
+    if (won_j == j) won = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+      if (place[u] == j) score[u] = 0;
   }
-  return won_j;
+  won = next;
+  won_j = next_j;
+}
+
+// The `top` best of the chunks first, first + step ... of a query's blocks; lane x scores blocks c0 + x, c0 + x + 64 ... of a chunk.
+template <int D>
+__device__ void exact_top(const bf16_t* qp, const bf16_t* kp, int have, int top, int lane, int first, int step, unsigned long long& won,
+                          int& won_j) {
+  constexpr int PER = EXACT_CHUNK / 64;
+  won = 0;
+  won_j = NO_BLOCK;
+  for (int c0 = first * EXACT_CHUNK; c0 < have; c0 += step * EXACT_CHUNK) {
+    double s[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) s[u] = 0;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 8) {
+      const bf16x8_t a = *(const bf16x8_t*)(qp + d);
+      double q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = (double)(float)a[e];
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        if (c0 + u * 64 >= have) break;
+        const bf16x8_t b = *(const bf16x8_t*)(kp + (long)min(c0 + u * 64 + lane, have - 1) * D + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[u] += q[e] * (double)(float)b[e];
+      }
+    }
+    unsigned long long score[PER];
+    int place[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const double x = s[u] == s[u] ? s[u] + 0.0 : -INFINITY;   // (-0 and 0 are equal)
+      const unsigned long long v = __builtin_bit_cast(unsigned long long, x);
+      place[u] = c0 + u * 64 + lane;
+      score[u] = place[u] >= have ? 0 : (v >> 63) ? ~v : v | 0x8000000000000000ull;
+    }
+    keep_best<PER>(score, place, top, lane, won, won_j);
+  }
 }
 // the blocks taken, in ascending order, -1 behind
 __device__ __forceinline__ void write_taken(int* to, int taken, int top, int lane) {
@@ -119,17 +144,35 @@ __device__ __forceinline__ void write_taken(int* to, int taken, int top, int lan
   if (lane < top) to[rank] = taken == NO_BLOCK ? -1 : taken;
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void block_select_row_kernel(Rows q, const bf16_t* __restrict__ keys, const int* __restrict__ k_len,
-                                                               int* __restrict__ blocks, int Lq, int Lk, int Hq, int G, int top,
-                                                               int nblk, long rows) {
-  __shared__ unsigned long long buf[4][EXACT_CHUNK];
+// NW waves a query: its chunks are dealt to them, and one wave takes the best of theirs
+template <int D, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_select_row_kernel(Rows q, const bf16_t* __restrict__ keys,
+                                                                                    const int* __restrict__ k_len, int* __restrict__ blocks,
+                                                                                    int Lq, int Lk, int Hq, int G, int top, int nblk, long rows) {
+  __shared__ unsigned long long score[NW][64];
+  __shared__ int place[NW][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = (long)blockIdx.x * 4 + wave;
+  const long row = NW == 1 ? (long)blockIdx.x * 4 + wave : blockIdx.x;
   if (row >= rows) return;
   const int i = row % Lq, h = (row / Lq) % Hq, b = row / ((long)Lq * Hq);
   const int have = (valid_keys(k_len, b, Lk) + BLK - 1) / BLK;
-  const int taken = exact_top<D>(q.p + b * q.sb + i * q.sl + h * q.sh, keys + ((long)b * (Hq / G) + h / G) * nblk * (long)D, have, top, buf[wave], lane);
+  unsigned long long won;
+  int taken;
+  exact_top<D>(q.p + b * q.sb + i * q.sl + h * q.sh, keys + ((long)b * (Hq / G) + h / G) * nblk * (long)D, have, top, lane, NW == 1 ? 0 : wave, NW,
+               won, taken);
+  if (NW > 1) {
+    score[wave][lane] = won;
+    place[wave][lane] = taken;
+    __syncthreads();
+    if (wave) return;
+    unsigned long long s[NW];
+    int p[NW];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { s[w] = score[w][lane]; p[w] = place[w][lane]; }
+    won = 0;
+    taken = NO_BLOCK;
+    keep_best<NW>(s, p, top, lane, won, taken);
+  }
   write_taken(blocks + row * top, taken, top, lane);
 }
 
@@ -145,24 +188,24 @@ __global__ __launch_bounds__(256) void block_select_row_kernel(Rows q, const bf1
 template <int D, int K>
 __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t* __restrict__ keys, const int* __restrict__ k_len,
                                                            int* __restrict__ blocks, int Lq, int Lk, int Hkv, int G, int top, int nblk) {
-  constexpr int EXACT_FLOATS = EXACT_CHUNK * 2, LIST_FLOATS = 2 * K * 64;
-  __shared__ __attribute__((aligned(16))) float scratch[4][EXACT_FLOATS > LIST_FLOATS ? EXACT_FLOATS : LIST_FLOATS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, bh = blockIdx.y, b = bh / Hkv, hk = bh - b * Hkv;
+  constexpr int LIST_FLOATS = 2 * K * 64, CHOICE_FLOATS = 16 * 64;
+  __shared__ __attribute__((aligned(16))) float scratch[4][CHOICE_FLOATS > LIST_FLOATS ? CHOICE_FLOATS : LIST_FLOATS];
+  __shared__ __attribute__((aligned(16))) char kbuf[2][Geo<D>::KV_BYTES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, bh = blockIdx.y, b_ = bh / Hkv, hk = bh - b_ * Hkv;
   const long rows = (long)Lq * G, r0 = ((long)blockIdx.x * 4 + wave) * 16;
-  if (r0 >= rows) return;   // (waves are independent: no barriers)
-  const long r = min(r0 + (lane & 15), rows - 1);
+  const long r = min(r0 + (lane & 15), rows - 1);   // (waves behind the last row work on it and write nothing)
   const bool in = r0 + (lane & 15) < rows;
   const unsigned i = G == 1 ? (unsigned)r : (unsigned)r / (unsigned)G;
   const int h = hk * G + (int)((unsigned)r - i * (unsigned)G), Hq = Hkv * G;
-  int* to = blocks + (((long)b * Hq + h) * Lq + i) * top;
-  const int have = (valid_keys(k_len, b, Lk) + BLK - 1) / BLK;
+  int* to = blocks + (((long)b_ * Hq + h) * Lq + i) * top;
+  const int have = (valid_keys(k_len, b_, Lk) + BLK - 1) / BLK;
   if (have <= top) {   // every block
     if (in)
       for (int t = g; t < top; t += 4) to[t] = t < have ? t : -1;
     return;
   }
   const bf16_t* kp = keys + (long)bh * nblk * D;
-  const bf16_t* qp = q.p + b * q.sb + (long)i * q.sl + h * q.sh;
+  const bf16_t* qp = q.p + b_ * q.sb + (long)i * q.sl + h * q.sh;
   Frag<D> qf;
   qf.load(qp, g);
   float qq = 0.f;
@@ -176,9 +219,38 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
 #pragma unroll
   for (int x = 0; x < K; ++x) best[x] = -INFINITY;
   unsigned kk = 0;   // the largest |key|^2, by its bits: a NaN is larger than any number
+  // The summaries pass through LDS, 64 at a time in two buffers, for the four waves (fetched by every wave for itself they were 1 GB
+  // of L2 traffic at 128x128 images: 180 us against XX).
+  constexpr int PER = (BLK * D / 8 + 255) / 256;
+  bf16x8_t piece[PER];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * 256 + threadIdx.x;
+      if (e < BLK * D / 8) piece[u] = *(const bf16x8_t*)(kp + (long)min(c0 + e / (D / 8), have - 1) * D + e % (D / 8) * 8);
+    }
+  };
+  auto stage = [&](char* to) {
+    const bf16x8_t none = {};
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int e = u * 256 + threadIdx.x, t = e / (D / 8), x = e % (D / 8);
+      if (e < BLK * D / 8) {
+        *(bf16x8_t*)(to + lds_at<D>(t, x)) = piece[u];
+        if constexpr (D == 8) *(bf16x8_t*)(to + lds_at<D>(t, 1)) = none;
+      }
+    }
+  };
+  Frag<D> kf;
+  fetch(0);
   for (int c = 0; c < have; c += 16) {
-    Frag<D> kf;
-    kf.load(kp + (long)min(c + mine, have - 1) * D, g);
+    const char* const kb = kbuf[(c >> 6) & 1];
+    if ((c & 63) == 0) {
+      stage(kbuf[(c >> 6) & 1]);
+      if (c + 64 < have) fetch(c + 64);
+      __syncthreads();
+    }
+    kf.from_lds(kb, (c & 63) + mine, g);
     const f32x4_t s = dot_frag<D>(kf, qf), n = dot_frag<D>(kf, kf);
     const float d01 = (lane & 1) ? n[1] : n[0], d23 = (lane & 1) ? n[3] : n[2], d = (lane & 2) ? d23 : d01;
     if (g == ((lane & 15) >> 2)) kk = max(kk, __builtin_bit_cast(unsigned, d) & 0x7fffffffu);
@@ -208,14 +280,16 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
 #pragma unroll
   for (int x = 0; x < 2 * K; ++x) lists[x * 64 + lane] = two[x];
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  float T = -INFINITY, U = -INFINITY;
+  float T = -INFINITY, U = -INFINITY, b[2 * K + 2];   // b[x]: the other list's (top + 1 - x)-th
+#pragma unroll
+  for (int x = 0; x < 2 * K + 2; ++x) b[x] = lists[min(max(top - x, 0), 2 * K - 1) * 64 + (lane ^ 32)];
+#pragma unroll
+  for (int x = 0; x < 2 * K + 2; ++x) b[x] = top + 1 - x == 0 ? INFINITY : top + 1 - x > 0 && top + 1 - x <= 2 * K ? b[x] : -INFINITY;
 #pragma unroll
   for (int x = 0; x <= 2 * K; ++x) {
     const float a = x == 0 ? INFINITY : two[x == 0 ? 0 : x - 1];
-    const int m = top - x;
-    auto other = [&](int y) { return y == 0 ? INFINITY : y > 0 && y <= 2 * K ? lists[(y - 1) * 64 + (lane ^ 32)] : -INFINITY; };
-    T = fmaxf(T, fminf(a, other(m)));
-    U = fmaxf(U, fminf(a, other(m + 1)));
+    T = fmaxf(T, fminf(a, b[x + 1]));
+    U = fmaxf(U, fminf(a, b[x]));
   }
   const float eps2 = 2.f * ((D < 16 ? 16 : D) * 0x1.04p-23f * __builtin_sqrtf(qq + 0x1p-118f) * __builtin_sqrtf(__builtin_bit_cast(float, kk) + 0x1p-118f) + 0x1p-118f);
   bool clear = T - U > eps2;                                            // (false if anything is NaN or infinite)
@@ -225,25 +299,40 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
     clear = clear && (l32 == -INFINITY || U > l32);                     // what a lane dropped is not above its last
   }
   clear = clear && kk < 0x7f800000u && qq < INFINITY;
+  // the choice in order into LDS (a row of `top` numbers a query), from there to memory by whole rows
+  int* const chosen = (int*)scratch[wave] + (lane & 15) * top;
+  fetch(0);
+  __syncthreads();   // (every wave is done with the buffers of the first pass, and this one with its lists)
   int count = 0;
   for (int c = 0; c < have; c += 16) {
-    Frag<D> kf;
-    kf.load(kp + (long)min(c + mine, have - 1) * D, g);
+    const char* const kb = kbuf[(c >> 6) & 1];
+    if ((c & 63) == 0) {
+      stage(kbuf[(c >> 6) & 1]);
+      if (c + 64 < have) fetch(c + 64);
+      __syncthreads();
+    }
+    kf.from_lds(kb, (c & 63) + mine, g);
     const f32x4_t s = dot_frag<D>(kf, qf);
     unsigned bits = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (c + 4 * e + g < have && s[e] > U) bits |= 1u << (4 * e + g);
+    if (!__ballot(bits != 0)) continue;
     unsigned all = bits | lane_xor_u<16>(bits);
     all |= lane_xor_u<32>(all);
-    if (clear && in) {
-      while (bits) {
-        const int x = __builtin_ctz(bits);
-        bits &= bits - 1;
-        to[count + __builtin_popcount(all & ((1u << x) - 1))] = c + x;
-      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned bit = 1u << (4 * e + g);
+      if (clear && (bits & bit)) chosen[count + __builtin_popcount(all & (bit - 1))] = c + 4 * e + g;
     }
     count += __builtin_popcount(all);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  {
+    const int x = lane >> 2;   // four lanes a query
+    int* const row = blocks + (((long)b_ * Hq + __shfl(h, x, 64)) * Lq + __shfl((int)i, x, 64)) * top;
+    const bool ok = (__ballot(clear && in) >> x) & 1;
+    for (int t = lane & 3; ok && t < top; t += 4) row[t] = ((int*)scratch[wave])[x * top + t];
   }
   unsigned long long open = __ballot(!clear && in && g == 0);
   while (open) {   // rows that 32 bits cannot decide
@@ -251,9 +340,10 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
     open &= open - 1;
     const unsigned ri = __builtin_amdgcn_readlane(i, x);
     const int rh = __builtin_amdgcn_readlane(h, x);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int taken = exact_top<D>(q.p + b * q.sb + (long)ri * q.sl + rh * q.sh, kp, have, top, (unsigned long long*)scratch[wave], lane);
-    write_taken(blocks + (((long)b * Hq + rh) * Lq + ri) * top, taken, top, lane);
+    unsigned long long won;
+    int taken;
+    exact_top<D>(q.p + b_ * q.sb + (long)ri * q.sl + rh * q.sh, kp, have, top, lane, 0, 1, won, taken);
+    write_taken(blocks + (((long)b_ * Hq + rh) * Lq + ri) * top, taken, top, lane);
   }
 }
 
@@ -285,8 +375,13 @@ extern "C" int dm_block_select(const dm_block_desc* d, const void* q, const void
   const long rows = (long)d->B * d->Hq * d->Lq, shared = (long)d->Lq * G;
   hipStream_t st = (hipStream_t)stream;
   if (shared < 16) {
-    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
-                                         (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows));
+    // one wave a query up to 256 blocks, 16 beyond (one query a head, 1025 blocks of 64 features: 69 us against XX)
+    if (n <= EXACT_CHUNK)
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 1>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
+                                           (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows))
+    else
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 16>), dim3((unsigned)rows), dim3(1024), 0, st, rows_of(q, d->q_stride),
+                                           (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows))
   } else {
     const dim3 grid(dm_cdiv(shared, 64), d->B * d->Hkv);
 #define GO(K) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_kernel<HD, K>), grid, dim3(256), 0, st, rows_of(q, d->q_stride), \
