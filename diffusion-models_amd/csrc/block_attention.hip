@@ -911,8 +911,7 @@ int check_span(const char* who, const dm_block_desc* d) {
   for (int i = 0; i < 3; ++i) DM_REQUIRE(s[i] >= 0, DM_ERR_ARG, "%s: negative stride of q", who);
   DM_REQUIRE((d->Lq - 1) * s[1] + (d->Hq - 1) * s[2] < (1L << 35) && (long)d->Lq * d->Hq * d->D < (1L << 35), DM_ERR_SHAPE,
              "%s: a sample of q spans more than 2^35 elements", who);
-  DM_REQUIRE(d->pool == 0 || d->pool == 1 || d->pool == 512, DM_ERR_ARG, "%s: pool is 0, 1 or 512, not %d", who, d->pool);
-  return DM_OK;
+  return check_pool(who, d);
 }
 // Whether the rows are taken in pools on the matrix cores or one query a workgroup. A pool's time is the number of its visits (its
 // blocks) times what a visit takes from barrier to barrier, however few rows want the block: 1.1 us up to 32 features, 1.6 us with 64

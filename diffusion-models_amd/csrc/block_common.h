@@ -190,6 +190,10 @@ bool aligned(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
     DM_REQUIRE(s[i] % 8 == 0, DM_ERR_ARG, "%s: strides of %s must be multiples of 8 elements (rows are read 16 bytes at a time)", who, name);
   return DM_OK;
 }
+[[maybe_unused]] int check_pool(const char* who, const dm_block_desc* d) {
+  DM_REQUIRE(d->pool == 0 || d->pool == 1 || d->pool == 512, DM_ERR_ARG, "%s: pool is 0, 1 or 512, not %d", who, d->pool);
+  return DM_OK;
+}
 int blocks_of(const dm_block_desc* d) { return (d->Lk + BLK - 1) / BLK; }
 
 Rows rows_of(const void* p, const long* s) { return Rows{(const bf16_t*)p, s[0], s[1], s[2]}; }

@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
   for (int x = 0; x < K; ++x) best[x] = -INFINITY;
   unsigned kk = 0;   // the largest |key|^2, by its bits: a NaN is larger than any number
   // The summaries pass through LDS, 64 at a time in two buffers, for the four waves (fetched by every wave for itself they were 1 GB
-  // of L2 traffic at 128x128 images: 180 us against XX).
+  // of L2 traffic at 128x128 images: 180 us against 170).
   constexpr int PER = (BLK * D / 8 + 255) / 256;
   bf16x8_t piece[PER];
   auto fetch = [&](int c0) {
@@ -370,12 +370,17 @@ extern "C" int dm_block_select(const dm_block_desc* d, const void* q, const void
   int rc = check_desc(who, d);
   if (rc) return rc;
   DM_REQUIRE(aligned(q) && aligned(keys) && blocks, DM_ERR_ARG, "%s: null or misaligned pointer", who);
-  if ((rc = check_strides(who, "q", d->q_stride))) return rc;
+  if ((rc = check_strides(who, "q", d->q_stride)) || (rc = check_pool(who, d))) return rc;
   const int G = d->Hq / d->Hkv, n = blocks_of(d), top = d->top;
   const long rows = (long)d->B * d->Hq * d->Lq, shared = (long)d->Lq * G;
   hipStream_t st = (hipStream_t)stream;
-  if (shared < 16) {
-    // one wave a query up to 256 blocks, 16 beyond (one query a head, 1025 blocks of 64 features: 69 us against XX)
+  // Every query by itself, or 16 a wave behind the screen (the results are the same). Measured (us, by itself / 16 a wave), 64 features:
+  //   2048 queries  top 8 of 64 blocks 12 / 14   top 16 of 256 26 / 43    top 8 of 512 96 / 44   top 16 of 1025 172 / 118
+  //    512 queries  top 8 of 64 blocks 12 / 14   top 16 of 256 18 / 43    top 8 of 512 32 / 44   top 16 of 1025 56 / 111
+  //   8192 queries  top 8 of 64 blocks 28 / 20   top 16 of 256 74 / 45    top 8 of 512 343 / 62  top 16 of 1025 637 / 173
+  // and by itself one wave a query up to 256 blocks, 16 beyond (one query a head, 1025 blocks: 69 us with one, 31 with 16).
+  const bool alone = d->pool ? d->pool == 1 : rows <= (n <= EXACT_CHUNK ? 2048 : 1024);
+  if (alone) {
     if (n <= EXACT_CHUNK)
       BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 1>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
                                            (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows))

@@ -844,7 +844,7 @@ def attention(qkv, n_heads, head_dim, scale=None):
 # Attention of each query over key blocks chosen for it, for sequences too long for `attention` above. Tensors are
 # [B, positions, heads, head_dim] (the parts of a packed qkv are read in place); BLOCK keys make a block.
 BLOCK = 64
-BLOCK_POOL = 0   # 512: rows in pools on the matrix cores, 1: one query a workgroup, 0: by the shape (dm_block_desc.pool)
+BLOCK_POOL = 0   # 512: queries together on the matrix cores, 1: every query by itself, 0: by the shape (dm_block_desc.pool)
 _HERE = contextlib.nullcontext()
 
 

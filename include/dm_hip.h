@@ -301,8 +301,8 @@ int dm_attention_bwd(const void* qkv, const void* out, const void* dout, const f
 typedef struct dm_block_desc {
   int B, Lq, Lk, Hq, Hkv, D;
   int top;      /* blocks a query names, 1 .. 64 */
-  int pool;     /* attention: 512: rows in pools of 512 on the matrix cores; 1: one query a workgroup; 0: by the shape.
-                   The same in the backward call as in its forward call */
+  int pool;     /* 512: many queries together on the matrix cores (attention: in pools of 512); 1: every query by itself;
+                   0: by the shape. The same in an attention's backward call as in its forward call */
   float scale;  /* of q . k */
   long q_stride[3], k_stride[3], v_stride[3];
   long dq_stride[3], dk_stride[3], dv_stride[3];   /* backward only */

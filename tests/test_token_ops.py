@@ -36,6 +36,18 @@ def randn(g, *shape, scale=1.0):
     return (torch.randn(*shape, generator=g, device="cuda") * scale).to(torch.bfloat16)
 
 
+@pytest.fixture(autouse=True)
+def _pool_by_shape():
+    yield
+    from dm_hip import ops as o
+    o.BLOCK_POOL = 0
+
+
+def rows_together(n):
+    """how many rows a workgroup takes: by the shape (0), one query (1), or a pool on the matrix cores"""
+    ops().BLOCK_POOL = n
+
+
 # -------------------------------------------------------------------------------------------------- references
 def lengths(k_len, B, L):
     return torch.full((B,), L, device="cuda") if k_len is None else k_len.clamp(0, L)
@@ -118,6 +130,7 @@ def some_blocks(g, B, Hq, Lq, n, top):
 
 # -------------------------------------------------------------------------------------------------- choice of blocks
 @gpu
+@pytest.mark.parametrize("pool", [0, 1, 512])
 @pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", [
     (1, 1, 1, 1, 1, 8, 1, False),
     (2, 5, 63, 2, 1, 16, 3, False),
@@ -132,7 +145,8 @@ def some_blocks(g, B, Hq, Lq, n, top):
     (2, 9, 5000, 4, 2, 32, 30, True),
     (1, 17, 5000, 2, 2, 16, 60, False),
 ])
-def test_block_choice(B, Lq, Lk, Hq, Hkv, D, top, ragged):
+def test_block_choice(B, Lq, Lk, Hq, Hkv, D, top, ragged, pool):
+    rows_together(pool)
     g = gen(1)
     q, k = randn(g, B, Lq, Hq, D), randn(g, B, Lk, Hkv, D)
     k_len = torch.tensor([Lk // 2, 0, Lk + 5], dtype=torch.int32, device="cuda")[:B] if ragged else None
@@ -146,7 +160,9 @@ def test_block_choice(B, Lq, Lk, Hq, Hkv, D, top, ragged):
 
 
 @gpu
-def test_block_choice_ties_and_values_that_are_no_numbers():
+@pytest.mark.parametrize("pool", [1, 512])
+def test_block_choice_ties_and_values_that_are_no_numbers(pool):
+    rows_together(pool)
     g = gen(2)
     q, k = randn(g, 1, 40, 1, 16), randn(g, 1, 640, 1, 16)
     k[:, 128:192] = k[:, 448:512]            # two equal blocks
@@ -167,8 +183,10 @@ def test_block_choice_ties_and_values_that_are_no_numbers():
 @gpu
 @pytest.mark.parametrize("scale_q,scale_k", [(1.0, 1.0), (2.0 ** 40, 2.0 ** -70), (2.0 ** -80, 2.0 ** -80), (2.0 ** 60, 2.0 ** 60)])
 @pytest.mark.parametrize("top", [1, 3, 8, 15, 25])
-def test_block_choice_among_near_ties(top, scale_q, scale_k):
+@pytest.mark.parametrize("pool", [1, 512])
+def test_block_choice_among_near_ties(top, scale_q, scale_k, pool):
     """Summaries of few distinct values: many scores are equal, or differ by the last bits of a 32-bit sum."""
+    rows_together(pool)
     g = gen(12)
     q = torch.randint(-3, 4, (1, 300, 2, 64), generator=g, device="cuda").to(torch.bfloat16) * scale_q
     keys = torch.randint(-2, 3, (1, 2, 130, 64), generator=g, device="cuda").to(torch.bfloat16)
@@ -181,8 +199,9 @@ def test_block_choice_among_near_ties(top, scale_q, scale_k):
 
 
 @gpu
-@pytest.mark.parametrize("n", [3, 40])   # fewer queries than a tile of 16 rows, and more
-def test_block_choice_decides_differences_that_32_bits_cannot_hold(n):
+@pytest.mark.parametrize("n,pool", [(3, 1), (40, 512)])
+def test_block_choice_decides_differences_that_32_bits_cannot_hold(n, pool):
+    rows_together(pool)
     # scores that differ by one part in 2^30: a large common product and a small one that differs
     q = torch.zeros(1, n, 1, 8, device="cuda", dtype=torch.bfloat16)
     q[..., 0], q[..., 1] = 1024.0, 1.0
@@ -208,18 +227,6 @@ CASES = [
     (1, 140, 5000, 2, 1, 64, 20, False),
     (4, 16, 320, 16, 16, 8, 3, False),
 ]
-
-
-@pytest.fixture(autouse=True)
-def _pool_by_shape():
-    yield
-    from dm_hip import ops as o
-    o.BLOCK_POOL = 0
-
-
-def rows_together(n):
-    """how many rows a workgroup takes: by the shape (0), one query (1), or a pool on the matrix cores"""
-    ops().BLOCK_POOL = n
 
 
 @gpu
