@@ -62,3 +62,15 @@ class GroupNorm(nn.GroupNorm):
         """This layer as the epilogue of the convolution that produces its input (Conv2d's `norm`)."""
         return ops.FusedNorm(self.weight, self.bias, self.num_groups, self.eps, act, scale_shift=scale_shift,
                              pre_add=pre_add)
+
+
+class TokenEmbedding(nn.Embedding):
+    """Rows by token of any shape, times `scale`, as bf16 tokens [..., embedding_dim] (or fp32 with dtype=torch.float32); the
+    padding row is zero and receives no gradient."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx: Optional[int] = None, scale: float = 1.0):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx)
+        self.scale = float(scale)
+
+    def forward(self, tokens, dtype=torch.bfloat16):
+        return ops.token_embed(tokens, self.weight, scale=self.scale, padding_idx=self.padding_idx, dtype=dtype)

@@ -10,6 +10,7 @@ from torch import nn
 
 from dm_hip import ops
 from modeling.activation import get_activation, is_silu
+from modeling.attention import Attention2D
 from modeling.blocks import ConvBlock, MidBlock, ProjectedEmbeddings, get_down_block, get_up_block
 from modeling.embeddings import MLPEmbedding, PeriodicEncoding
 from modeling.layers import GroupNorm
@@ -50,7 +51,10 @@ class UNet(nn.Module, GuidedPredictor):
             dropout: float = 0.0,
             downsample_use_conv: bool = True,
             upsample_use_conv: bool = True,
+            attention_top_blocks: Optional[int] = None,
     ):
+        """attention_top_blocks (not in the reference): every attention layer's pixels attend to this many blocks of 64
+        positions where the layer's map has more (Attention2D.attend_to); None: to all."""
         super().__init__()
         assert len(down_block_types) == len(up_block_types) == len(block_out_channels)
         n_levels = len(block_out_channels)
@@ -93,6 +97,10 @@ class UNet(nn.Module, GuidedPredictor):
         self.out_norm = GroupNorm(norm_groups, widths[0])
         self.out_act = get_activation(activation)
         self.out_conv = _EdgeConv(widths[0], out_channels, image_side="out")
+        if attention_top_blocks is not None:
+            for m in self.modules():
+                if isinstance(m, Attention2D):
+                    m.attend_to(attention_top_blocks)
         self._conv_blocks = [m for m in self.modules() if isinstance(m, ConvBlock)]  # plain list: not registered
 
     def forward(self, x: torch.Tensor, t: torch.Tensor, cls: Optional[torch.Tensor] = None,

@@ -542,3 +542,261 @@ def test_refusals():
                 lambda: o.token_embed(i(3), torch.zeros(3, 4, device="cuda"), padding_idx=3), lambda: o.token_embed(i(3).cpu(), torch.zeros(3, 4, device="cuda"))]:
         with pytest.raises(RuntimeError):
             bad()
+
+
+# -------------------------------------------------------------------------------------------------- streams, graphs, long offsets
+def _everything(x):
+    """one pass through every operator; x: the inputs, returned: every result"""
+    o = ops()
+    emb = o.token_embed(x["tokens"], x["table"], 1.5, 0, torch.float32)
+    grads = list(torch.autograd.grad(emb, x["table"], x["demb"]))
+    keys = o.block_keys(x["k"].detach(), x["k_len"])
+    blocks = o.block_select(x["q"].detach(), keys, 3, x["k_len"])
+    att = o.block_attention(x["q"], x["k"], x["v"], blocks, k_len=x["k_len"])
+    grads += torch.autograd.grad(att, (x["q"], x["k"], x["v"]), x["datt"])
+    packed = o.sparse_attention(x["qkv"], 4, 16, 2)
+    grads += torch.autograd.grad(packed, x["qkv"], x["dpacked"])
+    return [emb.detach(), keys, blocks, att.detach(), packed.detach()] + grads
+
+
+def _inputs(seed):
+    g = gen(seed)
+    x = {"table": torch.randn(50, 24, generator=g, device="cuda"), "q": randn(g, 2, 600, 4, 16), "k": randn(g, 2, 700, 2, 16),
+         "v": randn(g, 2, 700, 2, 16), "qkv": randn(g, 2, 520, 3 * 64)}
+    x = {n: t.requires_grad_(True) for n, t in x.items()}
+    x["k_len"] = torch.tensor([seed * 37 % 701, 700], dtype=torch.int32, device="cuda")
+    x["tokens"] = torch.randint(0, 50, (9000,), generator=g, device="cuda")
+    x["demb"], x["datt"], x["dpacked"] = torch.randn(9000, 24, generator=g, device="cuda"), randn(g, 2, 600, 4, 16), randn(g, 2, 520, 64)
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("pool", [0, 1, 512])
+def test_graph_replays_equal_eager(pool):
+    rows_together(pool)
+    want = [[t.clone() for t in _everything(_inputs(s))] for s in (1, 2, 3)]   # (the eager graphs are gone before the capture)
+    static = _inputs(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _everything(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = ops().new_graph()
+    with torch.cuda.graph(graph):
+        got = _everything(static)
+    for s in (1, 2, 3, 2, 1):
+        fresh = _inputs(s)
+        with torch.no_grad():
+            for n in static:
+                static[n].copy_(fresh[n])
+        graph.replay()
+        for a, b in zip(got, want[s - 1]):
+            assert torch.equal(a, b)
+        torch.randn(1 << 20, device="cuda").sum().item()      # eager work between the replays
+
+
+@gpu
+def test_two_captured_graphs_do_not_share_scratch():
+    a, b = _inputs(4), _inputs(5)
+    want = [[t.clone() for t in _everything(x)] for x in (_inputs(4), _inputs(5))]
+    graphs, got = [], []
+    for x in (a, b):
+        g = ops().new_graph()
+        with torch.cuda.graph(g):
+            got.append(_everything(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for res, ref in zip(got, want):
+            for u, v in zip(res, ref):
+                assert torch.equal(u, v)
+
+
+@gpu
+def test_on_a_stream_of_the_callers():
+    want = _everything(_inputs(6))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        x = _inputs(6)
+        got = _everything(x)
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("pool", [1, 512])
+def test_offsets_beyond_32_bits(pool):
+    """A sequence whose keys are 2^31 elements and more (4.4 GB), attended to at its end, equals the end by itself."""
+    rows_together(pool)
+    g = gen(14)
+    L, tail = 4_300_000 // 64 * 64, 64 * 40
+    k = torch.zeros(1, L + 17, 8, 64, device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    assert k.numel() > 2 ** 31
+    k[:, L - tail:], v[:, L - tail:] = randn(g, 1, tail + 17, 8, 64), randn(g, 1, tail + 17, 8, 64)
+    ke, ve = k[:, L - tail:].clone(), v[:, L - tail:].clone()
+    first = (L - tail) // 64
+    for Lq in (2, 600):
+        q = randn(g, 1, Lq, 8, 64, scale=2.0)
+        keys = ops().block_keys(k)
+        assert torch.equal(keys[:, :, first:], ops().block_keys(ke)) and not bool(keys[:, :, :first].any())
+        blocks = ops().block_select(q, keys, 4)
+        near = ops().block_select(q, keys[:, :, first:], 4)
+        assert torch.equal(blocks, near + first)   # a summary of zero never beats the best of 40 random ones here
+        assert torch.equal(ops().block_attention(q, k, v, blocks), ops().block_attention(q, ke, ve, near))
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    small = [x.detach().clone().requires_grad_(True) for x in (q, ke, ve)]
+    do = randn(g, 1, 600, 8, 64)
+    dq, dk, dv = torch.autograd.grad(ops().block_attention(*leaves, blocks), leaves, do)
+    sq, sk, sv = torch.autograd.grad(ops().block_attention(*small, near), small, do)
+    assert torch.equal(dq, sq) and torch.equal(dk[:, L - tail:], sk) and torch.equal(dv[:, L - tail:], sv)
+    assert not bool(dk[:, :L - tail].any())
+
+
+@gpu
+def test_token_embed_offsets_beyond_32_bits():
+    rows, width = 70000, 32768
+    table = torch.zeros(rows, width, device="cuda")
+    assert table.numel() > 2 ** 31
+    table[rows - 3:] = torch.randn(3, width, generator=gen(15), device="cuda")
+    tokens = torch.tensor([rows - 1, 0, rows - 3, rows - 1], device="cuda")
+    leaf = table.requires_grad_(True)
+    out = ops().token_embed(tokens, leaf, dtype=torch.float32)
+    assert torch.equal(out, table.detach()[tokens])
+    (grad,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert grad[rows - 1].eq(2).all() and grad[rows - 3].eq(1).all() and grad[0].eq(1).all() and float(grad.sum()) == 4.0 * width
+
+
+# -------------------------------------------------------------------------------------------------- in the model
+def test_attention_layer_keeps_its_parameters_and_refuses():
+    from modeling.attention import Attention2D
+    from modeling.unet import UNet
+    assert list(Attention2D(64, n_dim_head=8).state_dict()) == list(Attention2D(64, n_dim_head=8, top_blocks=3).state_dict())
+    assert Attention2D(64, n_dim_head=8, n_context=128).context_proj.weight.shape == (128, 128)
+    for bad in (lambda: Attention2D(64, n_dim_head=8, top_blocks=0), lambda: Attention2D(64, n_dim_head=8, top_blocks=65),
+                lambda: Attention2D(64, n_dim_head=8, top_blocks=2, dropout=0.1), lambda: Attention2D(64, n_dim_head=8, n_context=63),
+                lambda: Attention2D(64, n_dim_head=8, n_context=64, dropout=0.1)):
+        with pytest.raises(ValueError):
+            bad()
+    net = UNet(block_out_channels=(64, 64), down_block_types=("UNetDownBlock", "UNetAttnDownBlock"),
+               up_block_types=("UNetAttnUpBlock", "UNetUpBlock"), n_dim_attention_head=8, attention_top_blocks=2)
+    layers = [m for m in net.modules() if isinstance(m, Attention2D)]
+    assert layers and all(m.top_blocks == 2 for m in layers)
+
+
+def _layer(seed, **kw):
+    from modeling.attention import Attention2D
+    torch.manual_seed(seed)
+    return Attention2D(64, n_dim_head=8, norm_groups=8, **kw).cuda()
+
+
+def _plain_layer(m, x, blocks_of, context=None, context_len=None):
+    """the layer in fp32 from its parameters, attending where `blocks_of(q, k)` says"""
+    B, C, Hh, W = x.shape
+    L = Hh * W
+    h = torch.nn.functional.group_norm(x, m.norm.num_groups, m.norm.weight, m.norm.bias, m.norm.eps)
+    qkv = torch.nn.functional.linear(h.flatten(2).transpose(1, 2), m.qkv_proj.weight, m.qkv_proj.bias)
+    q, k, v = qkv.view(B, L, 3, m.n_heads, m.n_dim_head).unbind(2)
+    live = torch.ones(B, L, dtype=torch.bool, device="cuda")
+    if context is not None:
+        kv = torch.nn.functional.linear(context, m.context_proj.weight, m.context_proj.bias)
+        T = context.shape[1]
+        ck, cv = kv.view(B, T, 2, m.n_heads, m.n_dim_head).unbind(2)
+        k, v = torch.cat([k, ck], 1), torch.cat([v, cv], 1)
+        live = torch.cat([live, torch.arange(T, device="cuda") < context_len[:, None]], 1)
+    Lk = k.shape[1]
+    picked = blocks_of(q, k, live)
+    s = torch.matmul(q.transpose(1, 2), k.transpose(1, 2).transpose(2, 3)) * m.n_dim_head ** -0.5
+    s = s.masked_fill(~(picked.repeat_interleave(64, 3)[..., :Lk] & live[:, None, None]), -float("inf"))
+    att = torch.matmul(torch.softmax(s, -1), v.transpose(1, 2)).transpose(1, 2).reshape(B, L, -1)
+    out = torch.nn.functional.linear(att, m.out_proj.weight, m.out_proj.bias)
+    return x + out.transpose(1, 2).view(B, C, Hh, W)
+
+
+@gpu
+def test_attention_layer_on_chosen_blocks(monkeypatch):
+    o = ops()
+    m = _layer(1, top_blocks=2)
+    g = gen(16)
+    x = torch.randn(2, 64, 20, 18, generator=g, device="cuda").to(torch.bfloat16).float()     # 360 pixels: 6 blocks
+    do = torch.randn(2, 64, 20, 18, generator=g, device="cuda").to(torch.bfloat16)
+    made, select = [], o.block_select
+    monkeypatch.setattr(o, "block_select", lambda *a, **k: made.append(select(*a, **k)) or made[-1])
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    out = m(b)
+    got = torch.autograd.grad(out, [b, *m.parameters()], do)
+    assert len(made) == 1
+    picked = torch.zeros(2, m.n_heads, 360, 6, dtype=torch.bool, device="cuda").scatter_(3, made[0].long(), True)
+    ref = _plain_layer(m, a, lambda q, k, live: picked)     # (the choice itself is tested by itself: it has no gradient)
+    want = torch.autograd.grad(ref, [a, *m.parameters()], do.float())
+    # a handful of bf16 roundings (2^-8 each) one behind the other, as for the dense layer
+    assert rel_err(out.detach().float().cpu(), ref.detach().cpu()) < 1e-2
+    for u, v in zip(got, want):
+        assert rel_err(u.float().cpu(), v.cpu()) < 3e-2
+    m.attend_to(6)             # as many blocks as there are: the dense operator
+    assert torch.equal(m(b), _layer(1)(b)) and len(made) == 1
+
+
+@gpu
+def test_text_conditioned_attention_from_tokens_to_their_table():
+    """Token rows -> keys and values beside the pixels' -> attention of pixels over both -> gradients back into the rows."""
+    from modeling.layers import TokenEmbedding
+    torch.manual_seed(3)
+    emb = TokenEmbedding(40, 128, padding_idx=0, scale=128 ** 0.5 / 8).cuda()
+    m = _layer(2, n_context=128)
+    g = gen(19)
+    tokens = torch.randint(1, 40, (3, 20), generator=g, device="cuda")
+    length = torch.tensor([20, 0, 7], device="cuda")
+    tokens[torch.arange(20, device="cuda") >= length[:, None]] = 0
+    x = torch.randn(3, 64, 9, 9, generator=g, device="cuda").to(torch.bfloat16).float()
+    do = torch.randn(3, 64, 9, 9, generator=g, device="cuda").to(torch.bfloat16)
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    params = [emb.weight, *m.parameters()]
+    every = lambda q, k, live: torch.ones(3, m.n_heads, q.shape[1], -(-k.shape[1] // 64), dtype=torch.bool, device="cuda")  # noqa: E731
+    ref = _plain_layer(m, a, every, emb.weight[tokens] * emb.scale, length)
+    want = torch.autograd.grad(ref, [a, *params], do.float())
+    out = m(b, context=emb(tokens), context_len=length)
+    got = torch.autograd.grad(out, [b, *params], do)
+    assert rel_err(out.detach().float().cpu(), ref.detach().cpu()) < 1e-2
+    for u, v in zip(got, want):
+        assert rel_err(u.float().cpu(), v.float().cpu()) < 3e-2
+    assert not bool(got[1][0].any())                   # the padding row
+    # the padded text changes nothing, the valid one does
+    other = tokens.clone()
+    other[2, 7:] = 5
+    assert torch.equal(m(b, context=emb(other), context_len=length), out)
+    m.attend_to(1)
+    assert m(b, context=emb(tokens), context_len=length).shape == out.shape
+    with pytest.raises(RuntimeError):
+        m(b, context=emb(tokens)[:2])
+    with pytest.raises(RuntimeError):
+        _layer(2)(b, context=emb(tokens))
+
+
+@gpu
+def test_unet_attending_to_chosen_blocks():
+    from modeling.unet import UNet
+    kw = dict(block_out_channels=(64, 64), down_block_types=("UNetAttnDownBlock", "UNetDownBlock"),
+              up_block_types=("UNetUpBlock", "UNetAttnUpBlock"), n_blocks_per_layer=1, n_dim_attention_head=8, norm_groups=8,
+              time_encoding_dim=64, embedding_dim=64)
+    nets = []
+    for top in (None, 16, 3):
+        torch.manual_seed(4)
+        nets.append(UNet(attention_top_blocks=top, **kw).cuda())
+    g = gen(20)
+    x, t = torch.randn(4, 3, 32, 32, generator=g, device="cuda"), torch.randint(0, 1000, (4,), generator=g, device="cuda")
+    with torch.no_grad():
+        dense, full, sparse = (n(x, t) for n in nets)
+        assert torch.equal(dense, full)                # 32x32 pixels are 16 blocks
+        assert not torch.equal(dense, sparse)
+        assert torch.equal(nets[2](x[1:3], t[1:3]), sparse[1:3])   # whatever the batch
+    nets[2](x, t).square().mean().backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in nets[2].parameters())
