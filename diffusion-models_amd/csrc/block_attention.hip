@@ -456,6 +456,7 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
     const char *const kb = kv[buf], *const vb = kb + GE::KV_BYTES;
     while (it.j == cur.j) {
       if (sc < 0.f) qf.negate();
+      const unsigned off1 = rowoff[row1];   // (LDS answers in order: asked for behind the reads below, the next rows would go out late)
       float s[16];
       {
         Frag<D> kf[4];
@@ -464,7 +465,10 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) *(f32x4_t*)(s + kt * 4) = dot_frag<D>(kf[kt], qf);
       }
-      // what the tile reads from LDS and the next tile's operands are under way before the softmax
+      // the next tile's rows and what this one reads from LDS are under way before the softmax
+      if (it1.j >= 0) qf.load(qbase + (size_t)off1 * 8, g);
+      const typename PL::Tile it2 = w.next(it1);
+      const int row2 = w.row_of(it2);
       f32x4_t st = stat[row], o[GE::DT];
       bf16x4_t vt[GE::DT][4];
 #pragma unroll
@@ -473,9 +477,6 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) vt[dt][u] = read_tr<D>(vb, u * 16, dt, lane);
       }
-      if (it1.j >= 0) qf.load(qbase + (size_t)rowoff[row1] * 8, g);
-      const typename PL::Tile it2 = w.next(it1);
-      const int row2 = w.row_of(it2);
       __builtin_amdgcn_sched_barrier(0);
       const int n0 = w.n - cur.j * BLK;   // valid keys from this block on
       if (n0 < BLK) {
@@ -496,9 +497,11 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
           if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) s[e] = 0.f;   // (a scale of zero times -infinity is no zero)
       }
       float sum = 0.f;
+      if (a.lse) {   // (only the saved statistic needs it)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += s[e];
-      sum = row_sum(sum);
+        for (int e = 0; e < 16; ++e) sum += s[e];
+        sum = row_sum(sum);
+      }
       // The weights are rounded to bf16 as the matrix instruction's operand. The output is divided by the sum of the
       // ROUNDED weights (one more product, with ones), so that it stays an average of values: a rounding then counts only
       // with the value's distance from the output. The saved statistic is of the unrounded ones.
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
     *(f32x4_t*)f = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2));
     *(f32x4_t*)(f + 4) = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2 + 1));
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = st[1] == 0.f ? 0.f : f[x] * inv;
+    for (int x = 0; x < 8; ++x) f[x] = st[2] == 0.f ? 0.f : f[x] * inv;
     const bf16x8_t y = dm_pack8(f);
     const long at = (((long)w.b * a.Lq + i) * a.Hq + h) * D + c * 8;
     *(bf16x8_t*)(a.out + at) = y;
@@ -554,7 +557,7 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
       for (int x = 0; x < 8; ++x) lo[x] = f[x] - (float)y[x];
       *(bf16x8_t*)(a.out_lo + at) = dm_pack8(lo);
     }
-    if (a.lse && c == 0) a.lse[((long)w.b * a.Hq + h) * a.Lq + i] = st[1] == 0.f ? -INFINITY : st[0] * LN2 + logf(st[1]);
+    if (a.lse && c == 0) a.lse[((long)w.b * a.Hq + h) * a.Lq + i] = st[2] == 0.f ? -INFINITY : st[0] * LN2 + logf(st[1]);
   }
 }
 
@@ -611,9 +614,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   const bf16_t* const qbase = a.q.p + w.b * a.q.sb;
   const bf16_t* const obase = a.go + (long)w.b * a.Lq * a.Hq * D;
   Frag<D> qf, of;
-  auto load = [&](int row) {
-    qf.load(qbase + (size_t)rowoff[row] * 8, g);
-    of.load(obase + (size_t)gooff[row] * 8, g);
+  auto load = [&](unsigned at_q, unsigned at_o) {
+    qf.load(qbase + (size_t)at_q * 8, g);
+    of.load(obase + (size_t)at_o * 8, g);
   };
   auto arrived = [&]() {
     qf.arrived();
@@ -623,7 +626,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   of.zero();
   typename PL::Tile it = w.next(typename PL::Tile{-2, 0, 0, 0}), it1 = w.next(it);
   int row = w.row_of(it), row1 = w.row_of(it1);
-  if (it.j >= 0) load(row);
+  if (it.j >= 0) load(rowoff[row], gooff[row]);
   arrived();
   int buf = 0;
   while (cur.j >= 0) {
@@ -631,6 +634,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     if (nxt.j >= 0) w.fetch(nxt.j);
     const char *const kb = kv[buf], *const vb = kb + GE::KV_BYTES;
     while (it.j == cur.j) {
+      const unsigned off1 = rowoff[row1], off2 = gooff[row1];   // (first, as in the forward kernel)
       f32x4_t s[4], dp[4];
       {
         Frag<D> kf[4], vf[4];
@@ -645,6 +649,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
           dp[kt] = dot_frag<D>(vf[kt], of);
         }
       }
+      if (it1.j >= 0) load(off1, off2);
+      const typename PL::Tile it2 = w.next(it1);
+      const int row2 = w.row_of(it2);
       const f32x2_t st = stat[row];
       f32x4_t o[GE::DT];
       bf16x4_t tr[GE::DT][4];
@@ -654,9 +661,6 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) tr[dt][u] = read_tr<D>(kb, u * 16, dt, lane);
       }
-      if (it1.j >= 0) load(row1);
-      const typename PL::Tile it2 = w.next(it1);
-      const int row2 = w.row_of(it2);
       __builtin_amdgcn_sched_barrier(0);
       float ds[16];
 #pragma unroll
