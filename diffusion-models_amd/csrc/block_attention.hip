@@ -310,7 +310,7 @@ struct Visits {
   unsigned long long bits = 0;
   __device__ __forceinline__ Visits(const int* o, int nb_, int lane_) : offs(o), nb(nb_), lane(lane_) {}
   __device__ __forceinline__ Hit next(int least) {
-    while (!bits) {
+    while (__builtin_expect(!bits, 0)) {
       if (next0 >= nb) return Hit{-1, 0, 0};
       base = next0;
       next0 += 64;
@@ -341,6 +341,9 @@ struct Pool {
   const bf16_t* src[PER];   // this thread's pieces of block 0, the distance of a block, the key they belong to
   long step[PER];
   int key[PER];
+  // which of keys and values a wave's piece u is of, and whether it has one (the same for all lanes: no branch by lane)
+  __device__ __forceinline__ int half(int u) const { return u * P + wave * 64 >= PIECES / 2 ? 1 : 0; }
+  __device__ __forceinline__ bool has(int u) const { return PIECES % P == 0 || u * P + wave * 64 < PIECES; }
 
   __device__ __forceinline__ Pool(const Args& a_, int bh_, int pool_)
       : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), pool(pool_), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
@@ -349,11 +352,11 @@ struct Pool {
         mine(offsets(a_, bh_, pool_), nb, threadIdx.x & 63) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int e = u * P + threadIdx.x, half = e >= PIECES / 2 ? 1 : 0, x = e - half * (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
-      const Rows& r = half ? a.v : a.k;
+      const int x = (u * P + threadIdx.x) % (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
+      const Rows& r = half(u) ? a.v : a.k;
       src[u] = r.p + b * r.sb + t * r.sl + hk * r.sh + c * 8;
       step[u] = BLK * r.sl;
-      key[u] = e < PIECES ? t : 0x40000000;   // (no piece: behind every valid key)
+      key[u] = t;
     }
   }
   static __device__ __forceinline__ const int* offsets(const Args& a, int bh, int pool) {
@@ -362,34 +365,39 @@ struct Pool {
   __device__ __forceinline__ void fetch(int j) {   // block j's keys and values into registers; zeros behind the valid keys
     const bf16x8_t none = {};
     const int left = n - j * BLK;
+    if (__builtin_expect(left >= BLK, 1)) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) piece[u] = key[u] < left ? *(const bf16x8_t*)(src[u] + j * step[u]) : none;
+      for (int u = 0; u < PER; ++u)
+        if (has(u)) piece[u] = *(const bf16x8_t*)(src[u] + j * step[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) piece[u] = has(u) && key[u] < left ? *(const bf16x8_t*)(src[u] + j * step[u]) : none;
+    }
   }
   __device__ __forceinline__ void stage(char* buf) const {   // keys, then values
     const bf16x8_t none = {};
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int e = u * P + threadIdx.x, half = e >= PIECES / 2 ? 1 : 0, x = e - half * (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
-      if (PIECES % P == 0 || e < PIECES) {
-        *(bf16x8_t*)(buf + half * Geo<D>::KV_BYTES + lds_at<D>(t, c)) = piece[u];
-        if constexpr (D == 8) *(bf16x8_t*)(buf + half * Geo<D>::KV_BYTES + lds_at<D>(t, 1)) = none;
+      const int x = (u * P + threadIdx.x) % (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
+      if (has(u)) {
+        *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, c)) = piece[u];
+        if constexpr (D == 8) *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, 1)) = none;
       }
     }
   }
 
-  // the tile that this wave computes behind `it` (start with Tile{-2, ...}); j = -1: none
+  // the tile that this wave computes behind `it` (start with Tile{}); j = -1: none
   __device__ __forceinline__ Tile next(const Tile& it) {
-    if (it.j == -1) return it;
-    if (it.j >= 0 && (it.t + NW) * 16 < it.n) return Tile{it.j, it.start, it.n, it.t + NW};
+    if (__builtin_expect((it.t + NW) * 16 < it.n, 0)) return Tile{it.j, it.start, it.n, it.t + NW};
     const Hit h = mine.next(wave * 16);
     return Tile{h.j, h.start, h.n, wave};
   }
-  // a lane's row of a tile (behind the last: the tile's first)
+  // A lane's row of a tile. Behind the last one row P, which belongs to nobody: a tile's sums are written back without a
+  // branch by lane, so that the compiler may interleave the products of its features.
   __device__ __forceinline__ int row_of(const Tile& it) const {
     const int li = it.t * 16 + l15;
-    return it.j < 0 ? 0 : rows[it.start + (li < it.n ? li : it.t * 16)];
+    return li < it.n ? rows[it.start + li] : P;
   }
-  __device__ __forceinline__ bool live(const Tile& it) const { return it.t * 16 + l15 < it.n; }
 
   __device__ __forceinline__ long row_index(int row) const { return (long)pool * P + row; }
   __device__ __forceinline__ bool inside(int row) const { return row_index(row) < (long)a.Lq * a.G; }
@@ -397,6 +405,17 @@ struct Pool {
     const unsigned r = (unsigned)row_index(row), q = a.G == 1 ? r : r / (unsigned)a.G;
     i = q;
     h = hk * a.G + (int)(r - q * a.G);
+  }
+  // each(e) for the scores of keys n0 and behind. (n0 is hidden from the compiler, which would
+  // otherwise compare every lane's keys with it at every visit, also of whole blocks.)
+  template <typename F>
+  __device__ __forceinline__ void behind(int n0, F&& each) const {
+    if (__builtin_expect(n0 < BLK, 0)) {
+      asm volatile("" : "+s"(n0));
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) each(e);
+    }
   }
   // a row's place in a [..][positions][heads][D] tensor, in units of 8 features from the sample's first (0 behind the last row)
   __device__ __forceinline__ unsigned offset(int row, long sl, long sh) const {
@@ -420,9 +439,9 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
   using PL = Pool<D>;
   constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
-  __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
-  __shared__ __attribute__((aligned(16))) f32x4_t stat[P];   // maximum, sum of the weights, sum of the weights as rounded
-  __shared__ unsigned rowoff[P];
+  __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
+  __shared__ __attribute__((aligned(16))) f32x4_t stat[P + 1];   // maximum, sum of the weights, sum of the weights as rounded
+  __shared__ unsigned rowoff[P + 1];
   int bh, pool;
   if (!pool_of_block(a.B * a.Hkv, a.pools, bh, pool)) return;
   PL w(a, bh, pool);
@@ -440,14 +459,18 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
   for (int e = tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
   rowoff[tid] = w.offset(tid, a.q.sl, a.q.sh);
   stat[tid] = f32x4_t{-INFINITY, 0.f, 0.f, 0.f};
+  if (tid < GE::OC) *(f32x4_t*)(acc + (P * GE::OC + tid) * 4) = zero4;
+  if (tid == 0) {
+    rowoff[P] = 0;
+    stat[P] = zero4;
+  }
   __syncthreads();
 
   const bf16_t* const qbase = a.q.p + w.b * a.q.sb;
   Frag<D> qf;
-  qf.zero();
-  typename PL::Tile it = w.next(typename PL::Tile{-2, 0, 0, 0}), it1 = w.next(it);
+  typename PL::Tile it = w.next(typename PL::Tile{}), it1 = w.next(it);
   int row = w.row_of(it), row1 = w.row_of(it1);
-  if (it.j >= 0) qf.load(qbase + (size_t)rowoff[row] * 8, g);
+  qf.load(qbase + (size_t)rowoff[row] * 8, g);
   qf.arrived();
   int buf = 0;
   while (cur.j >= 0) {
@@ -455,20 +478,19 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
     if (nxt.j >= 0) w.fetch(nxt.j);
     const char *const kb = kv[buf], *const vb = kb + GE::KV_BYTES;
     while (it.j == cur.j) {
-      if (sc < 0.f) qf.negate();
       const unsigned off1 = rowoff[row1];   // (LDS answers in order: asked for behind the reads below, the next rows would go out late)
-      float s[16];
-      {
-        Frag<D> kf[4];
+      Frag<D> kf[4];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) kf[kt].from_lds(kb, kt * 16 + w.l15, g);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) *(f32x4_t*)(s + kt * 4) = dot_frag<D>(kf[kt], qf);
-      }
-      // the next tile's rows and what this one reads from LDS are under way before the softmax
-      if (it1.j >= 0) qf.load(qbase + (size_t)off1 * 8, g);
+      for (int kt = 0; kt < 4; ++kt) kf[kt].from_lds(kb, kt * 16 + w.l15, g);
       const typename PL::Tile it2 = w.next(it1);
       const int row2 = w.row_of(it2);
+      if (sc < 0.f) qf.negate();
+      __builtin_amdgcn_sched_barrier(0);
+      float s[16];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) *(f32x4_t*)(s + kt * 4) = dot_frag<D>(kf[kt], qf);
+      // the next tile's rows and what this one reads from LDS are under way before the softmax
+      qf.load(qbase + (size_t)off1 * 8, g);
       f32x4_t st = stat[row], o[GE::DT];
       bf16x4_t vt[GE::DT][4];
 #pragma unroll
@@ -479,28 +501,21 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
       }
       __builtin_amdgcn_sched_barrier(0);
       const int n0 = w.n - cur.j * BLK;   // valid keys from this block on
-      if (n0 < BLK) {
+      w.behind(n0, [&](int e) { s[e] = -INFINITY; });
+      float mx[4];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) s[e] = -INFINITY;
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-      const float m_new = fmaxf(st[0], row_max(mx) * asc), at = m_new == -INFINITY ? 0.f : m_new;
+      for (int kt = 0; kt < 4; ++kt) mx[kt] = fmaxf(fmaxf(s[kt * 4], s[kt * 4 + 1]), fmaxf(s[kt * 4 + 2], s[kt * 4 + 3]));
+      const float m_new = fmaxf(st[0], row_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * asc), at = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = __builtin_amdgcn_exp2f(st[0] - at);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * asc - at);
-      if (n0 < BLK) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) s[e] = 0.f;   // (a scale of zero times -infinity is no zero)
-      }
+      w.behind(n0, [&](int e) { s[e] = 0.f; });   // (a scale of zero times -infinity is no zero)
       float sum = 0.f;
       if (a.lse) {   // (only the saved statistic needs it)
+        float part[4];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += s[e];
-        sum = row_sum(sum);
+        for (int kt = 0; kt < 4; ++kt) part[kt] = (s[kt * 4] + s[kt * 4 + 1]) + (s[kt * 4 + 2] + s[kt * 4 + 3]);
+        sum = row_sum((part[0] + part[1]) + (part[2] + part[3]));
       }
       // The weights are rounded to bf16 as the matrix instruction's operand. The output is divided by the sum of the
       // ROUNDED weights (one more product, with ones), so that it stays an average of values: a rounding then counts only
@@ -511,18 +526,20 @@ __global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
       const float r_old = st[2] * alpha;
       f32x4_t rs = {r_old, r_old, r_old, r_old};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
-      const bool live = w.live(it);
-      if (live && g == 0) stat[row] = f32x4_t{m_new, st[1] * alpha + sum, rs[0], 0.f};
-#pragma unroll
       for (int dt = 0; dt < GE::DT; ++dt) {
-        f32x4_t c = o[dt];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] *= alpha;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(vt[dt][2 * u], vt[dt][2 * u + 1]), p[u], c, 0, 0, 0);
-        if (live) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = c;
+        for (int e = 0; e < 4; ++e) o[dt][e] *= alpha;
       }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int dt = 0; dt < GE::DT; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(vt[dt][2 * u], vt[dt][2 * u + 1]), p[u], o[dt], 0, 0, 0);
+        rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
+      }
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = o[dt];
+      stat[row] = f32x4_t{m_new, st[1] * alpha + sum, rs[0], 0.f};   // (four lanes, the same values)
       it = it1;
       row = row1;
       it1 = it2;
@@ -568,9 +585,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   using PL = Pool<D>;
   constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
-  __shared__ __attribute__((aligned(16))) float acc[P * GE::DV];
-  __shared__ f32x2_t stat[P];   // lse, delta
-  __shared__ unsigned rowoff[P], gooff[P];
+  __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
+  __shared__ f32x2_t stat[P + 1];   // lse, delta
+  __shared__ unsigned rowoff[P + 1], gooff[P + 1];
   int bh, pool;
   if (!pool_of_block(a.B * a.Hkv, a.pools, bh, pool)) return;
   PL w(a, bh, pool);
@@ -586,6 +603,11 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   for (int e = tid; e < P * GE::OC; e += P) *(f32x4_t*)(acc + e * 4) = zero4;
   rowoff[tid] = w.offset(tid, a.q.sl, a.q.sh);
   gooff[tid] = w.offset(tid, (long)a.Hq * D, D);
+  if (tid < GE::OC) *(f32x4_t*)(acc + (P * GE::OC + tid) * 4) = zero4;
+  if (tid == 0) {
+    rowoff[P] = gooff[P] = 0;
+    stat[P] = f32x2_t{INFINITY, 0.f};
+  }
   constexpr int PC = D / 8;
   for (int e = tid; e < P * PC; e += P) {   // (a row's PC lanes are neighbours: P is a multiple of PC)
     const int r = e / PC, c = e % PC;
@@ -622,11 +644,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     qf.arrived();
     of.arrived();
   };
-  qf.zero();
-  of.zero();
-  typename PL::Tile it = w.next(typename PL::Tile{-2, 0, 0, 0}), it1 = w.next(it);
+  typename PL::Tile it = w.next(typename PL::Tile{}), it1 = w.next(it);
   int row = w.row_of(it), row1 = w.row_of(it1);
-  if (it.j >= 0) load(rowoff[row], gooff[row]);
+  load(rowoff[row], gooff[row]);
   arrived();
   int buf = 0;
   while (cur.j >= 0) {
@@ -635,23 +655,22 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     const char *const kb = kv[buf], *const vb = kb + GE::KV_BYTES;
     while (it.j == cur.j) {
       const unsigned off1 = rowoff[row1], off2 = gooff[row1];   // (first, as in the forward kernel)
-      f32x4_t s[4], dp[4];
-      {
-        Frag<D> kf[4], vf[4];
+      Frag<D> kf[4], vf[4];
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          kf[kt].from_lds(kb, kt * 16 + w.l15, g);
-          vf[kt].from_lds(vb, kt * 16 + w.l15, g);
-        }
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          s[kt] = dot_frag<D>(kf[kt], qf);
-          dp[kt] = dot_frag<D>(vf[kt], of);
-        }
+      for (int kt = 0; kt < 4; ++kt) {
+        kf[kt].from_lds(kb, kt * 16 + w.l15, g);
+        vf[kt].from_lds(vb, kt * 16 + w.l15, g);
       }
-      if (it1.j >= 0) load(off1, off2);
       const typename PL::Tile it2 = w.next(it1);
       const int row2 = w.row_of(it2);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4_t s[4], dp[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        s[kt] = dot_frag<D>(kf[kt], qf);
+        dp[kt] = dot_frag<D>(vf[kt], of);
+      }
+      load(off1, off2);
       const f32x2_t st = stat[row];
       f32x4_t o[GE::DT];
       bf16x4_t tr[GE::DT][4];
@@ -667,12 +686,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[kt][e] * sc - st[0]) * (dp[kt][e] - st[1]);
-      const int n0 = w.n - cur.j * BLK;
-      if (n0 < BLK) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) ds[e] = 0.f;
-      }
+      w.behind(w.n - cur.j * BLK, [&](int e) { ds[e] = 0.f; });
       // ds sums to zero over a row's keys, so what its keys have in common cancels in dq: rounded to bf16 it would not, by 2^-9 of
       // the common part. Two bf16 operands, the rounded ds and what the rounding lost, keep 2^-17.
       bf16x8_t p[2], lost[2];
@@ -683,18 +697,16 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
         for (int e = 0; e < 8; ++e) ds[u * 8 + e] -= (float)p[u][e];
         lost[u] = dm_pack8(ds + u * 8);
       }
-      const bool live = w.live(it);
 #pragma unroll
-      for (int dt = 0; dt < GE::DT; ++dt) {
-        f32x4_t c = o[dt];
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int dt = 0; dt < GE::DT; ++dt) {
           const bf16x8_t keys = join4(tr[dt][2 * u], tr[dt][2 * u + 1]);
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, p[u], c, 0, 0, 0);
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, lost[u], c, 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, p[u], o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, lost[u], o[dt], 0, 0, 0);
         }
-        if (live) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = c;
-      }
+#pragma unroll
+      for (int dt = 0; dt < GE::DT; ++dt) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = o[dt];
       it = it1;
       row = row1;
       it1 = it2;
