@@ -340,7 +340,7 @@ struct Pool {
   bf16x8_t piece[PER];
   const bf16_t* src[PER];   // this thread's pieces of block 0, the distance of a block, the key they belong to
   long step[PER];
-  int key[PER];
+  int key[PER], left = 0;   // (left: valid keys from the fetched block on)
   // which of keys and values a wave's piece u is of, and whether it has one (the same for all lanes: no branch by lane)
   __device__ __forceinline__ int half(int u) const { return u * P + wave * 64 >= PIECES / 2 ? 1 : 0; }
   __device__ __forceinline__ bool has(int u) const { return PIECES % P == 0 || u * P + wave * 64 < PIECES; }
@@ -362,24 +362,24 @@ struct Pool {
   static __device__ __forceinline__ const int* offsets(const Args& a, int bh, int pool) {
     return a.offs + ((long)bh * a.pools + pool) * (a.nblk + 1);
   }
-  __device__ __forceinline__ void fetch(int j) {   // block j's keys and values into registers; zeros behind the valid keys
-    const bf16x8_t none = {};
-    const int left = n - j * BLK;
-    if (__builtin_expect(left >= BLK, 1)) {
+  // Block j's keys and values into registers. Behind the valid keys the last one is read, and becomes zeros on its way into LDS: a
+  // load that a branch may replace by zeros makes the compiler wait for the loads before it.
+  __device__ __forceinline__ void fetch(int j) {
+    left = n - j * BLK;
 #pragma unroll
-      for (int u = 0; u < PER; ++u)
-        if (has(u)) piece[u] = *(const bf16x8_t*)(src[u] + j * step[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < PER; ++u) piece[u] = has(u) && key[u] < left ? *(const bf16x8_t*)(src[u] + j * step[u]) : none;
+    for (int u = 0; u < PER; ++u) {
+      const bf16_t* at = src[u] + j * step[u];
+      if (__builtin_expect(left < BLK, 0)) at -= (long)max(key[u] - (left - 1), 0) * (step[u] / BLK);
+      if (has(u)) piece[u] = *(const bf16x8_t*)at;
     }
   }
-  __device__ __forceinline__ void stage(char* buf) const {   // keys, then values
+  __device__ __forceinline__ void stage(char* buf) {   // keys, then values
     const bf16x8_t none = {};
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int x = (u * P + threadIdx.x) % (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
       if (has(u)) {
+        if (__builtin_expect(left < BLK, 0)) piece[u] = t < left ? piece[u] : none;
         *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, c)) = piece[u];
         if constexpr (D == 8) *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, 1)) = none;
       }
