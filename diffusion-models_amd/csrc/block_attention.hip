@@ -406,15 +406,16 @@ struct Pool {
     i = q;
     h = hk * a.G + (int)(r - q * a.G);
   }
-  // each(e) for the scores of keys n0 and behind. (n0 is hidden from the compiler, which would
-  // otherwise compare every lane's keys with it at every visit, also of whole blocks.)
+  // each(e) for the scores of keys n0 and behind. (The place is hidden from the compiler, which would
+  // otherwise keep every lane's keys in registers and compare them at every visit, also of whole blocks.)
   template <typename F>
   __device__ __forceinline__ void behind(int n0, F&& each) const {
     if (__builtin_expect(n0 < BLK, 0)) {
-      asm volatile("" : "+s"(n0));
+      int mine0 = n0 - g * 4;
+      asm volatile("" : "+v"(mine0));
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if ((e >> 2) * 16 + g * 4 + (e & 3) >= n0) each(e);
+        if ((e >> 2) * 16 + (e & 3) >= mine0) each(e);
     }
   }
   // a row's place in a [..][positions][heads][D] tensor, in units of 8 features from the sample's first (0 behind the last row)
@@ -434,7 +435,7 @@ __device__ __forceinline__ bool pool_of_block(int nbh, int pools, int& bh, int& 
 }
 
 template <int D>
-__global__ __launch_bounds__(POOL) void attend_pool_kernel(Args a) {
+__global__ __launch_bounds__(POOL, D <= 16 ? 6 : 2) void attend_pool_kernel(Args a) {
   using GE = Geo<D>;
   using PL = Pool<D>;
   constexpr int P = POOL;
@@ -930,22 +931,23 @@ int check_span(const char* who, const dm_block_desc* d) {
   return check_pool(who, d);
 }
 // Whether the rows are taken in pools on the matrix cores or one query a workgroup. A pool's time is the number of its visits (its
-// blocks) times what a visit takes from barrier to barrier, however few rows want the block: 1.1 us up to 32 features, 1.6 us with 64
-// (256 pools run at a time, twice as many up to 32 features); a query's is 0.3 ns + 0.5 .. 0.8 ns a block over the whole chip. Both sides
-// measured, forward (us), one query a workgroup against pools:
-//   8 heads x 256 queries, 8 of 64 blocks       D 8  20 / 69       D 64  26 / 90
-//   4 x 8 heads x 256 queries, 8 of 64          D 8  39 / 70       D 64  74 / 91
-//   4 x 8 heads x 1024 queries, 4 of 16         D 8  69 / 34       D 64  134 / 46
-//   2 x 8 heads x 2048 queries, 8 of 128        D 8  139 / 129     D 64  243 / 173
-//   4 x 8 heads x 4096 queries, 8 of 64         D 8  521 / 81      D 64  896 / 111
+// blocks) times what a visit takes from barrier to barrier, however few rows want the block: 0.9 us up to 16 features, 1.05 us with
+// 32, 1.5 us with 64 (256 pools run at a time, twice as many up to 16 features); a query's is 0.3 ns + 0.5 .. 0.8 ns a block over the
+// whole chip. Both sides measured, forward (us), one query a workgroup against pools:
+//   8 heads x 256 queries, 8 of 64 blocks       D 8  16 / 57       D 64  25 / 84
+//   4 x 8 heads x 256 queries, 8 of 64          D 8  40 / 57       D 64  74 / 85
+//   4 x 8 heads x 1024 queries, 4 of 16         D 8  70 / 28       D 64  137 / 41
+//   2 x 8 heads x 2048 queries, 8 of 128        D 8  139 / 103     D 64  243 / 160
+//   4 x 8 heads x 4096 queries, 8 of 64         D 8  514 / 66      D 64  893 / 103
 // (Pools of 128 and 256 rows, which occupy more CUs where there are few rows, were never faster by more than 5 %.)
 bool pooled(const dm_block_desc* d) {
   if (d->pool) return d->pool == POOL;
   // The two round differently, and a sample's result must not depend on the batch it is in: the choice is priced for 4 samples.
   const double rows = (double)d->Lq * (d->Hq / d->Hkv), heads = 4.0 * d->Hkv;
-  const double pools = heads * ((long)(rows + POOL - 1) / POOL), rounds = (long)((pools + (d->D == 64 ? 255 : 511)) / (d->D == 64 ? 256 : 512));
+  const double at_once = d->D <= 16 ? 512 : 256, visit = d->D <= 16 ? 900 : d->D == 32 ? 1050 : 1500;
+  const double pools = heads * dm_cdiv((long)rows, POOL), rounds = (double)(long)((pools + at_once - 1) / at_once);
   const double most = (rows < POOL ? rows : POOL) * d->top, visits = most < blocks_of(d) ? most : blocks_of(d);
-  return heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 6000.0 + rounds * visits * (d->D == 64 ? 1600.0 : 1100.0);
+  return heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 6000.0 + rounds * visits * visit;
 }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
 struct PlanLayout { int pools; size_t offs, bytes; };
