@@ -587,7 +587,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
   __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
-  __shared__ f32x2_t stat[P + 1];   // lse, delta
+  __shared__ f32x2_t stat[P + 1];   // lse, -delta (the products of do and v start from it)
   __shared__ unsigned rowoff[P + 1], gooff[P + 1];
   int bh, pool;
   if (!pool_of_block(a.B * a.Hkv, a.pools, bh, pool)) return;
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     delta = group_sum<PC>(delta);
     if (c == 0) {
       const float lse = in ? a.lse[lrow] : 0.f;
-      stat[r] = f32x2_t{lse == -INFINITY ? INFINITY : lse * LOG2E, delta};   // no key: every weight becomes zero
+      stat[r] = f32x2_t{lse == -INFINITY ? INFINITY : lse * LOG2E, -delta};   // no key: every weight becomes zero
       if (in) a.delta[lrow] = delta;
     }
   }
@@ -656,6 +656,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     const char *const kb = kv[buf], *const vb = kb + GE::KV_BYTES;
     while (it.j == cur.j) {
       const unsigned off1 = rowoff[row1], off2 = gooff[row1];   // (first, as in the forward kernel)
+      const f32x2_t st = stat[row];
       Frag<D> kf[4], vf[4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
@@ -669,10 +670,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
         s[kt] = dot_frag<D>(kf[kt], qf);
-        dp[kt] = dot_frag<D>(vf[kt], of);
+        dp[kt] = dot_frag<D>(vf[kt], of, f32x4_t{st[1], st[1], st[1], st[1]});
       }
       load(off1, off2);
-      const f32x2_t st = stat[row];
       f32x4_t o[GE::DT];
       bf16x4_t tr[GE::DT][4];
 #pragma unroll
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[kt][e] * sc - st[0]) * (dp[kt][e] - st[1]);
+        for (int e = 0; e < 4; ++e) ds[kt * 4 + e] = __builtin_amdgcn_exp2f(s[kt][e] * sc - st[0]) * dp[kt][e];
       w.behind(w.n - cur.j * BLK, [&](int e) { ds[e] = 0.f; });
       // ds sums to zero over a row's keys, so what its keys have in common cancels in dq: rounded to bf16 it would not, by 2^-9 of
       // the common part. Two bf16 operands, the rounded ds and what the rounding lost, keep 2^-17.
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
   constexpr int TILE_BYTES = 32 * GE::ROWB;
   __shared__ __attribute__((aligned(16))) char kbuf[GE::KV_BYTES], vbuf[GE::KV_BYTES];
   __shared__ __attribute__((aligned(16))) char rows[4][2][TILE_BYTES];    // q and do of a wave's tile; at the end the sums
-  __shared__ __attribute__((aligned(16))) float stat[4][2][32];           // lse, delta
+  __shared__ __attribute__((aligned(16))) float stat[4][2][32];           // lse, -delta
   __shared__ unsigned short list[LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.Hkv, hk = bh - b * a.Hkv;
@@ -840,7 +840,7 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
         const int row = mt * 16 + (lane & 15);
         if (g == 0) {
           st_lse[row] = lse[mt] == -INFINITY ? INFINITY : lse[mt] * LOG2E;   // (also a row without a key: every weight is zero)
-          st_delta[row] = delta[mt];
+          st_delta[row] = -delta[mt];
         }
         qf[mt].to_lds(qb, row, g);
         of[mt].to_lds(ob, row, g);
@@ -858,12 +858,12 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
           float p[8], ds[8];
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf);
             const f32x4_t ls = *(const f32x4_t*)(st_lse + mt * 16 + g * 4), de = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
+            const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf, de);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - ls[e]);
-              ds[mt * 4 + e] = p[mt * 4 + e] * (dp[e] - de[e]);
+              ds[mt * 4 + e] = p[mt * 4 + e] * dp[e];
             }
           }
           pt[k2] = dm_pack8(p);

@@ -144,8 +144,7 @@ struct Frag {
   }
 };
 template <int D>
-__device__ __forceinline__ f32x4_t dot_frag(const Frag<D>& a, const Frag<D>& b) {
-  f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ f32x4_t dot_frag(const Frag<D>& a, const Frag<D>& b, f32x4_t c = f32x4_t{0.f, 0.f, 0.f, 0.f}) {
   if constexpr (D <= 16) {
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4_t, a.x[0]), __builtin_bit_cast(s16x4_t, b.x[0]), c, 0, 0, 0);
   } else {
