@@ -251,15 +251,20 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
       __syncthreads();
     }
     kf.from_lds(kb, (c & 63) + mine, g);
-    const f32x4_t s = dot_frag<D>(kf, qf), n = dot_frag<D>(kf, kf);
+    f32x4_t s = dot_frag<D>(kf, qf);
+    const f32x4_t n = dot_frag<D>(kf, kf);
     const float d01 = (lane & 1) ? n[1] : n[0], d23 = (lane & 1) ? n[3] : n[2], d = (lane & 2) ? d23 : d01;
     if (g == ((lane & 15) >> 2)) kk = max(kk, __builtin_bit_cast(unsigned, d) & 0x7fffffffu);
+    if (c + 16 > have) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + 4 * e + g >= have) s[e] = -INFINITY;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = c + 4 * e + g < have ? s[e] : -INFINITY;
 #pragma unroll
-      for (int p = K - 1; p > 0; --p) best[p] = __builtin_amdgcn_fmed3f(best[p - 1], best[p], x);
-      best[0] = fmaxf(best[0], x);
+      for (int p = K - 1; p > 0; --p) best[p] = __builtin_amdgcn_fmed3f(best[p - 1], best[p], s[e]);
+      best[0] = __builtin_amdgcn_fmed3f(best[0], s[e], INFINITY);   // (the larger of two, in one instruction)
     }
   }
 #pragma unroll
@@ -304,26 +309,31 @@ __global__ __launch_bounds__(256) void block_select_kernel(Rows q, const bf16_t*
   fetch(0);
   __syncthreads();   // (every wave is done with the buffers of the first pass, and this one with its lists)
   int count = 0;
-  for (int c = 0; c < have; c += 16) {
+  for (int c = 0; c < have; c += 32) {   // a word of 32 blocks at a time
     const char* const kb = kbuf[(c >> 6) & 1];
     if ((c & 63) == 0) {
       stage(kbuf[(c >> 6) & 1]);
       if (c + 64 < have) fetch(c + 64);
       __syncthreads();
     }
-    kf.from_lds(kb, (c & 63) + mine, g);
-    const f32x4_t s = dot_frag<D>(kf, qf);
     unsigned bits = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + 4 * e + g < have && s[e] > U) bits |= 1u << (4 * e + g);
+    for (int half = 0; half < 2; ++half) {
+      kf.from_lds(kb, (c & 63) + half * 16 + mine, g);
+      const f32x4_t s = dot_frag<D>(kf, qf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits |= s[e] > U ? 1u << (half * 16 + 4 * e) : 0u;
+    }
+    bits <<= g;
+    if (c + 32 > have) bits &= (1u << (have - c)) - 1;
     if (!__ballot(bits != 0)) continue;
     unsigned all = bits | lane_xor_u<16>(bits);
     all |= lane_xor_u<32>(all);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned bit = 1u << (4 * e + g);
-      if (clear && (bits & bit)) chosen[count + __builtin_popcount(all & (bit - 1))] = c + 4 * e + g;
+    if (!clear) bits = 0;
+    while (bits) {
+      const unsigned bit = bits & -bits;
+      chosen[count + __builtin_popcount(all & (bit - 1))] = c + __builtin_ctz(bits);
+      bits ^= bit;
     }
     count += __builtin_popcount(all);
   }
