@@ -941,26 +941,39 @@ def block_select(q, keys, top, k_len=None):
 
 
 def _block_forward(d, q, k, v, blocks, k_len, training):
-    dev = q.device
-    out = torch.empty((d.B, d.Lq, d.Hq, d.D), dtype=BF16, device=dev)
-    out_lo = torch.empty_like(out) if training else None
-    lse = torch.empty((d.B, d.Hq, d.Lq), dtype=torch.float32, device=dev) if training else None
+    """The output and, for training, what the backward pass needs besides it in one tensor: the plan, what out's rounding lost
+    and the statistics (_block_kept)."""
+    out = torch.empty((d.B, d.Lq, d.Hq, d.D), dtype=BF16, device=q.device)
     n = lib.dm_block_attention_plan_bytes(ctypes.byref(d), int(training))
-    plan = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    out_lo, lse, size = _block_kept(d, n) if training else (0, 0, n)
+    kept = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    at = kept.data_ptr() if size else 0
     check(lib.dm_block_attention_fwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
-                                     out.data_ptr(), _p(out_lo), _p(lse), _p(plan), _stream()))
-    return out, (plan, out_lo, lse)
+                                     out.data_ptr(), at + out_lo if training else None, at + lse if training else None,
+                                     at or None, _stream()))
+    return out, kept
 
 
-def _block_backward(d, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
-    plan, out_lo, lse = kept
-    for t, to in ((dq, d.dq_stride), (dk, d.dk_stride), (dv, d.dv_stride)):
-        to[:] = t.stride()[:3]
-    n = lib.dm_block_attention_bwd_ws_bytes(ctypes.byref(d))
+def _block_kept(d, plan_bytes):
+    """Where what out's rounding lost and the statistics begin in the kept tensor, behind the plan, and its size"""
+    out_lo = (plan_bytes + 15) // 16 * 16
+    rows = d.B * d.Lq * d.Hq
+    lse = out_lo + rows * d.D * 2
+    return out_lo, lse, lse + rows * 4
+
+
+def _block_backward(desc, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
+    d = BlockDesc.from_buffer_copy(desc)
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+    ref = ctypes.byref(d)
+    n = lib.dm_block_attention_bwd_ws_bytes(ref)
     ws = _scratch(q.device, (n + 3) // 4)
-    check(lib.dm_block_attention_bwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
-                                     plan.data_ptr(), out.data_ptr(), out_lo.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n, _stream()))
+    out_lo, lse, _ = _block_kept(d, lib.dm_block_attention_plan_bytes(ref, 1))
+    at = kept.data_ptr()
+    check(lib.dm_block_attention_bwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len), at,
+                                     out.data_ptr(), at + out_lo, at + lse, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                     dv.data_ptr(), ws.data_ptr(), n, _stream()))
 
 
 class _BlockAttentionFn(Function):
@@ -968,18 +981,17 @@ class _BlockAttentionFn(Function):
     def forward(ctx, q, k, v, blocks, k_len, d):
         with _on(q.device):
             out, kept = _block_forward(d, q, k, v, blocks, k_len, True)
-        ctx.save_for_backward(q, k, v, blocks, k_len, out, *kept)
+        ctx.save_for_backward(q, k, v, blocks, k_len, out, kept)
         ctx.d = d
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, blocks, k_len, out, *kept = ctx.saved_tensors
+        q, k, v, blocks, k_len, out, kept = ctx.saved_tensors
         with _on(q.device):
-            dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=t.device) for t in (q, k, v))
-            d = _block_desc(*(getattr(ctx.d, n) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "top", "scale")), q, k, v, ctx.d.pool)
-            _block_backward(d, q, k, v, blocks, k_len, out, kept, _aligned(dout), dq, dk, dv)
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+            _block_backward(ctx.d, q, k, v, blocks, k_len, out, kept, _aligned(dout), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -1034,20 +1046,19 @@ class _SparseAttentionFn(Function):
             blocks = block_select(q, block_keys(k), top)
             out, kept = _block_forward(d, q, k, v, blocks, None, training)
         if training:
-            ctx.save_for_backward(qkv, blocks, out, *kept)
-            ctx.cfg = (B, L, H, D, top, scale, d.pool)
+            ctx.save_for_backward(qkv, blocks, out, kept)
+            ctx.d = d
         return out.view(B, L, H * D)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, blocks, out, *kept = ctx.saved_tensors
-        B, L, H, D, top, scale, pool = ctx.cfg
-        q, k, v = qkv.view(B, L, 3, H, D).unbind(2)
+        qkv, blocks, out, kept = ctx.saved_tensors
+        d = ctx.d
+        parts = (d.B, d.Lq, 3, d.Hq, d.D)
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            d = _block_desc(B, L, L, H, H, D, top, scale, q, k, v, pool)
-            _block_backward(d, q, k, v, blocks, None, out, kept, _aligned(dout), *dqkv.view(B, L, 3, H, D).unbind(2))
+            _block_backward(d, *qkv.view(parts).unbind(2), blocks, None, out, kept, _aligned(dout), *dqkv.view(parts).unbind(2))
         return dqkv, None, None, None, None, None
 
 
