@@ -38,8 +38,8 @@ __global__ __launch_bounds__(256) void attend_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
   __shared__ float so[4][D], sm[4], sl[4];
   const int lane = threadIdx.x & 63, w4 = threadIdx.x >> 6, wave = w4 % NW;
-  const long row = (long)blockIdx.x * (4 / NW) + w4 / NW;
-  if (row >= rows) return;   // (only without a join: 4 waves a query leave no remainder)
+  const long row = dm_block_index() * (4 / NW) + w4 / NW;
+  if (row >= rows) return;   // (all of a query's waves)
   const int i = row % a.Lq, h = (row / a.Lq) % a.Hq, b = row / ((long)a.Lq * a.Hq), hk = h / a.G;
   const int n = valid_keys(a.k_len, b, a.Lk);
   const int c = (lane % LPR) * 8, key = lane / LPR;
@@ -161,7 +161,7 @@ template <int D>
 __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
   const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long row = dm_block_index() * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int i = row % a.Lq, h = (row / a.Lq) % a.Hq, b = row / ((long)a.Lq * a.Hq), hk = h / a.G;
   const int n = valid_keys(a.k_len, b, a.Lk);
@@ -1002,8 +1002,8 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   }
   const long rows = (long)d->B * d->Hq * d->Lq;
   if (pool) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
-  else if ((long)d->Hq * d->Lq < 512) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, rows))
-  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 1>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
+  else if ((long)d->Hq * d->Lq < 512) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dm_grid(rows), dim3(256), 0, st, a, rows))
+  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 1>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -1040,7 +1040,7 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   hipStream_t st = (hipStream_t)stream;
   const long rows = (long)d->B * d->Hq * d->Lq;
   if (pooled(d)) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
-  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
+  else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
   BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a));
   DM_CHECK_LAUNCH();

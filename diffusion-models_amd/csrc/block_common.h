@@ -179,9 +179,9 @@ bool aligned(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
   DM_REQUIRE(d->Hq % d->Hkv == 0, DM_ERR_SHAPE, "%s: %d query heads do not share %d key heads evenly", who, d->Hq, d->Hkv);
   DM_REQUIRE(d->D == 8 || d->D == 16 || d->D == 32 || d->D == 64, DM_ERR_SHAPE, "%s: head dim %d (8, 16, 32 and 64 are covered)", who, d->D);
   DM_REQUIRE(d->top > 0 && d->top <= 64, DM_ERR_SHAPE, "%s: top %d (1 to 64 blocks a query)", who, d->top);
-  DM_REQUIRE(d->Lk <= 0x7fffff00, DM_ERR_SHAPE, "%s: more than 2^31-256 keys", who);
-  DM_REQUIRE((long)d->B * d->Hq * d->Lq <= 0x7fffffffL && (long)d->B * d->Hkv <= 65535 && (long)d->Lq * (d->Hq / d->Hkv) <= 0x7fffffffL,
-             DM_ERR_SHAPE, "%s: more than 2^31-1 queries or 65535 (sample, key head) pairs", who);
+  DM_REQUIRE(d->Lk < (1 << 30) - BLK, DM_ERR_SHAPE, "%s: 2^30 keys and more are not covered", who);
+  DM_REQUIRE((long)d->B * d->Hq * d->Lq <= 0x7fffffffL && (long)d->B * d->Hkv <= 65535 && (long)d->Lq * (d->Hq / d->Hkv) < (1L << 30),
+             DM_ERR_SHAPE, "%s: more than 2^31-1 queries, 2^30 of one key head or 65535 (sample, key head) pairs", who);
   return DM_OK;
 }
 [[maybe_unused]] int check_strides(const char* who, const char* name, const long* s) {

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void block_select_row_kern
   __shared__ unsigned long long score[NW][64];
   __shared__ int place[NW][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long row = NW == 1 ? (long)blockIdx.x * 4 + wave : blockIdx.x;
+  const long row = NW == 1 ? dm_block_index() * 4 + wave : dm_block_index();
   if (row >= rows) return;
   const int i = row % Lq, h = (row / Lq) % Hq, b = row / ((long)Lq * Hq);
   const int have = (valid_keys(k_len, b, Lk) + BLK - 1) / BLK;
@@ -392,10 +392,10 @@ extern "C" int dm_block_select(const dm_block_desc* d, const void* q, const void
   const bool alone = d->pool ? d->pool == 1 : rows <= (n <= EXACT_CHUNK ? 2048 : 1024);
   if (alone) {
     if (n <= EXACT_CHUNK)
-      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 1>), dim3(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 1>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, rows_of(q, d->q_stride),
                                            (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows))
     else
-      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 16>), dim3((unsigned)rows), dim3(1024), 0, st, rows_of(q, d->q_stride),
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((block_select_row_kernel<HD, 16>), dm_grid(rows), dim3(1024), 0, st, rows_of(q, d->q_stride),
                                            (const bf16_t*)keys, k_len, blocks, d->Lq, d->Lk, d->Hq, G, top, n, rows))
   } else {
     const dim3 grid(dm_cdiv(shared, 64), d->B * d->Hkv);

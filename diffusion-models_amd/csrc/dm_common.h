@@ -39,6 +39,10 @@ void dm_set_error(const char* fmt, ...);
   } while (0)
 
 static inline int dm_cdiv(long a, long b) { return (int)((a + b - 1) / b); }
+// n workgroups in two dimensions, numbered by dm_block_index() (numbers from n on do nothing): one dimension may hold fewer
+// than 2^32 threads
+static inline dim3 dm_grid(long n) { return n <= (1L << 20) ? dim3((unsigned)n) : dim3(1u << 20, (unsigned)((n + (1L << 20) - 1) >> 20)); }
+__device__ __forceinline__ long dm_block_index() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
 
 // Ordered sum of per-workgroup partial vectors into accumulating outputs (dm_sum_item, see the public header): the
 // library's replacement for float atomics on parameter gradients. With `deferred` the item is handed to the caller

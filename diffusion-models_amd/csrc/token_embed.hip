@@ -14,6 +14,7 @@ namespace {
 
 constexpr int TILE = 2048;      // keys a workgroup sorts at a time: 4 waves x 8 rounds x 64 lanes
 constexpr int RADIX = 256;
+constexpr int SCAN_TILES = 256;
 
 // number of threads that share a row of `vecs` vectors: a power of two, so that a workgroup holds whole rows
 int threads_per_row(int vecs) {
@@ -63,7 +64,7 @@ template <typename T, int V, int U>
 __global__ __launch_bounds__(256) void token_embed_kernel(const float* __restrict__ table, const int64_t* __restrict__ tokens,
                                                           T* __restrict__ out, long n, long rows, int width, float scale, int tpr) {
   const int per = 256 / tpr;
-  const long i0 = (long)blockIdx.x * (per * U) + threadIdx.x / tpr;
+  const long i0 = dm_block_index() * (per * U) + threadIdx.x / tpr;
   const float* src[U];
   bool live[U];
 #pragma unroll
@@ -110,23 +111,50 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restri
   counts[(long)t * RADIX + tid] = c[tid];
 }
 
+// The counts become the number of that digit's keys in earlier tiles, and their sums stand behind the last tile: a thread is a
+// digit of a quarter of the tiles. (Up to SCAN_TILES tiles every workgroup of the pass adds them up by itself.)
+__global__ __launch_bounds__(1024) void sort_scan_kernel(unsigned* __restrict__ counts, int tiles) {
+  __shared__ unsigned sum[4][RADIX];
+  const int digit = threadIdx.x & (RADIX - 1), part = threadIdx.x / RADIX, per = (tiles + 3) / 4;
+  const int first = part * per, end = min(first + per, tiles);
+  unsigned s = 0;
+#pragma unroll 16
+  for (int t = first; t < end; ++t) s += counts[(long)t * RADIX + digit];
+  sum[part][digit] = s;
+  __syncthreads();
+  s = 0;
+  for (int p = 0; p < part; ++p) s += sum[p][digit];
+#pragma unroll 16
+  for (int t = first; t < end; ++t) {
+    const unsigned c = counts[(long)t * RADIX + digit];
+    counts[(long)t * RADIX + digit] = s;
+    s += c;
+  }
+  if (part == 3) counts[(long)tiles * RADIX + digit] = s;
+}
+
 // One stable pass: a key's place is (keys of smaller digits) + (keys of its digit in earlier tiles, waves and lanes).
 // Inside a wave the lanes of one digit find each other with 8 ballots.
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restrict__ tokens, const unsigned* __restrict__ key_in,
                                                         const unsigned* __restrict__ idx_in, unsigned* __restrict__ key_out,
                                                         unsigned* __restrict__ idx_out, const unsigned* __restrict__ counts, long n,
-                                                        long rows, long padding, int tiles, int shift) {
+                                                        long rows, long padding, int tiles, int scanned, int shift) {
   __shared__ unsigned base[RADIX], wcount[4][RADIX];
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
   for (int w = 0; w < 4; ++w) wcount[w][tid] = 0;
   unsigned before = 0, total = 0;
+  if (scanned) {
+    before = counts[(long)t * RADIX + tid];
+    total = counts[(long)tiles * RADIX + tid];
+  } else {
 #pragma unroll 8
-  for (int x = 0; x < tiles; ++x) {
-    const unsigned c = counts[(long)x * RADIX + tid];
-    total += c;
-    before += x < t ? c : 0;
+    for (int x = 0; x < tiles; ++x) {
+      const unsigned c = counts[(long)x * RADIX + tid];
+      total += c;
+      before += x < t ? c : 0;
+    }
   }
   base[tid] = total;
   __syncthreads();
@@ -394,7 +422,7 @@ Plan plan_of(long n, long rows, int width) {
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   for (int i = 0; i < 2; ++i) { p.key[i] = take(n * 4); p.idx[i] = take(n * 4); }
-  p.counts = take((size_t)p.tiles * RADIX * 4);
+  p.counts = take((size_t)(p.tiles + 1) * RADIX * 4);
   p.part = take((size_t)p.chunks * 2 * width * 4);
   p.total = at;
   return p;
@@ -424,7 +452,7 @@ extern "C" int dm_token_embed(const float* table, const int64_t* tokens, void* o
   const int V = vectors(width, table, out, out_bf16);
   const int tpr = threads_per_row(width / V);
   const int U = n / (256 / tpr) >= 8192 ? 4 : 1;   // 4 rows a thread once that leaves 8 workgroups a CU (131072 rows of 1024: 129 -> 105 us)
-  const dim3 grid(dm_cdiv(n, 256 / tpr * U)), block(256);
+  const dim3 grid = dm_grid(dm_cdiv(n, 256 / tpr * U)), block(256);
   hipStream_t st = (hipStream_t)stream;
 #define GO(T, V, U) hipLaunchKernelGGL((token_embed_kernel<T, V, U>), grid, block, 0, st, table, tokens, (T*)out, n, rows, width, scale, tpr)
 #define GO_U(T, V) do { if (U == 4) GO(T, V, 4); else GO(T, V, 1); } while (0)
@@ -456,6 +484,7 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   float* part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
+  const int scan = p.tiles > SCAN_TILES;
   // one workgroup up to 8192 tokens (4999 tokens, two passes: 20 us in 4 launches)
   if (n <= SMALL) {
     hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, st, tokens, key[(p.passes - 1) & 1], idx[(p.passes - 1) & 1], (int)n, rows, padding, p.passes);
@@ -467,8 +496,12 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
     if (i == 0) hipLaunchKernelGGL((sort_count_kernel<true>), tiles, block, 0, st, tokens, nullptr, counts, n, rows, padding, 0);
     else hipLaunchKernelGGL((sort_count_kernel<false>), tiles, block, 0, st, nullptr, ki, counts, n, rows, padding, 8 * i);
     DM_CHECK_LAUNCH();
-    if (i == 0) hipLaunchKernelGGL((sort_pass_kernel<true>), tiles, block, 0, st, tokens, nullptr, nullptr, ko, io, counts, n, rows, padding, (int)p.tiles, 0);
-    else hipLaunchKernelGGL((sort_pass_kernel<false>), tiles, block, 0, st, nullptr, ki, ii, ko, io, counts, n, rows, padding, (int)p.tiles, 8 * i);
+    if (scan) {
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, st, counts, (int)p.tiles);
+      DM_CHECK_LAUNCH();
+    }
+    if (i == 0) hipLaunchKernelGGL((sort_pass_kernel<true>), tiles, block, 0, st, tokens, nullptr, nullptr, ko, io, counts, n, rows, padding, (int)p.tiles, scan, 0);
+    else hipLaunchKernelGGL((sort_pass_kernel<false>), tiles, block, 0, st, nullptr, ki, ii, ko, io, counts, n, rows, padding, (int)p.tiles, scan, 8 * i);
     DM_CHECK_LAUNCH();
   }
   const unsigned *sk = key[(p.passes - 1) & 1], *si = idx[(p.passes - 1) & 1];
