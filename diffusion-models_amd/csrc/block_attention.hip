@@ -24,7 +24,9 @@ struct Args {
   const int* k_len;
   const int* offs;             // the plan (block_plan_kernel)
   const unsigned short* rows;
-  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools;
+  float* part;                 // of a pool whose blocks are split: its slices' sums, [slice][row of the call][D], and statistics behind
+  f32x4_t* part_stat;
+  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools, slices;
   float scale;
 };
 
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 // maximum and sum are two lane swaps away, and exp(S^T) is in the register layout that the second product takes as its
 // right operand (its left operand, V^T or K^T, is read by transposing LDS reads in the same order of keys).
 
-constexpr int POOL = 512;
+constexpr int POOL = 512, MAX_SLICES = 8;
 
 // offs[b][hkv][pool][0 .. nblk]: where the rows of a block begin in rows[b][hkv][pool][512 top] (numbers inside the pool,
 // ascending). A set: a block that a query names twice counts once, numbers outside 0 .. nblk-1 name none.
@@ -306,9 +308,9 @@ __global__ __launch_bounds__(POOL) void block_plan_kernel(const int* __restrict_
 struct Hit { int j, start, n; };   // block (-1: no more), its rows' place in the list, their number
 struct Visits {
   const int* offs;
-  int nb, lane, base = 0, next0 = 0, start = 0, count = 0;
+  int nb, lane, base = 0, next0, start = 0, count = 0;
   unsigned long long bits = 0;
-  __device__ __forceinline__ Visits(const int* o, int nb_, int lane_) : offs(o), nb(nb_), lane(lane_) {}
+  __device__ __forceinline__ Visits(const int* o, int first, int nb_, int lane_) : offs(o), nb(nb_), lane(lane_), next0(first) {}
   __device__ __forceinline__ Hit next(int least) {
     while (__builtin_expect(!bits, 0)) {
       if (next0 >= nb) return Hit{-1, 0, 0};
@@ -334,29 +336,33 @@ struct Pool {
   static constexpr int KV = 2 * Geo<D>::KV_BYTES, BUFS = P * (Geo<D>::DV * 4 + 24) + 2 * KV <= 160 * 1024 ? 2 : 1;
   struct Tile { int j, start, n, t; };
   const Args& a;
-  int bh, b, hk, pool, n, nb, lane, wave, l15, g;
+  int bh, b, hk, pool, slice, n, lo, nb, lane, wave, l15, g;   // (blocks lo .. nb - 1 of the pool's are this workgroup's)
   const unsigned short* rows;
   Visits mine;
   bf16x8_t piece[PER];
-  const bf16_t* src[PER];   // this thread's pieces of block 0, the distance of a block, the key they belong to
+  const bf16_t* src[PER];   // this thread's pieces of block 0, the distance of a block
   long step[PER];
-  int key[PER], left = 0;   // (left: valid keys from the fetched block on)
+  int left = 0;             // valid keys from the fetched block on
   // which of keys and values a wave's piece u is of, and whether it has one (the same for all lanes: no branch by lane)
   __device__ __forceinline__ int half(int u) const { return u * P + wave * 64 >= PIECES / 2 ? 1 : 0; }
+  static __device__ __forceinline__ int key(int u) {   // the key of piece u (for a sample's last block alone: not kept in a register)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    return (u * P + tid) % (PIECES / 2) / (D / 8);
+  }
   __device__ __forceinline__ bool has(int u) const { return PIECES % P == 0 || u * P + wave * 64 < PIECES; }
 
-  __device__ __forceinline__ Pool(const Args& a_, int bh_, int pool_)
-      : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), pool(pool_), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
-        nb((n + BLK - 1) / BLK), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
+  __device__ __forceinline__ Pool(const Args& a_, int bh_, int pool_, int slice_)
+      : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), pool(pool_), slice(slice_), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
+        lo((int)((long)((n + BLK - 1) / BLK) * slice_ / a_.slices)), nb((int)((long)((n + BLK - 1) / BLK) * (slice_ + 1) / a_.slices)), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
         g((threadIdx.x & 63) >> 4), rows(a_.rows + ((long)bh_ * a_.pools + pool_) * ((long)P * a_.top)),
-        mine(offsets(a_, bh_, pool_), nb, threadIdx.x & 63) {
+        mine(offsets(a_, bh_, pool_), lo, nb, threadIdx.x & 63) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int x = (u * P + threadIdx.x) % (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
       const Rows& r = half(u) ? a.v : a.k;
       src[u] = r.p + b * r.sb + t * r.sl + hk * r.sh + c * 8;
       step[u] = BLK * r.sl;
-      key[u] = t;
     }
   }
   static __device__ __forceinline__ const int* offsets(const Args& a, int bh, int pool) {
@@ -369,7 +375,7 @@ struct Pool {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const bf16_t* at = src[u] + j * step[u];
-      if (__builtin_expect(left < BLK, 0)) at -= (long)max(key[u] - (left - 1), 0) * (step[u] / BLK);
+      if (__builtin_expect(left < BLK, 0)) at -= (long)max(key(u) - (left - 1), 0) * (step[u] / BLK);
       if (has(u)) piece[u] = *(const bf16x8_t*)at;
     }
   }
@@ -379,7 +385,7 @@ struct Pool {
     for (int u = 0; u < PER; ++u) {
       const int x = (u * P + threadIdx.x) % (PIECES / 2), t = x / (D / 8), c = x % (D / 8);
       if (has(u)) {
-        if (__builtin_expect(left < BLK, 0)) piece[u] = t < left ? piece[u] : none;
+        if (__builtin_expect(left < BLK, 0)) piece[u] = key(u) < left ? piece[u] : none;
         *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, c)) = piece[u];
         if constexpr (D == 8) *(bf16x8_t*)(buf + half(u) * Geo<D>::KV_BYTES + lds_at<D>(t, 1)) = none;
       }
@@ -428,14 +434,36 @@ struct Pool {
   }
 };
 
-__device__ __forceinline__ bool pool_of_block(int nbh, int pools, int& bh, int& pool) {
-  if ((nbh & 7) == 0) dm_xcd_tile(blockIdx.x, pools, bh, pool);   // one head's pools on one XCD: its keys and values stay in that L2
-  else { bh = blockIdx.x / pools; pool = blockIdx.x % pools; }
+__device__ __forceinline__ bool pool_of_block(const Args& a, int& bh, int& pool, int& slice) {
+  const int nbh = a.B * a.Hkv, each = a.pools * a.slices;
+  if ((nbh & 7) == 0) dm_xcd_tile(blockIdx.x, each, bh, pool);   // one head's pools on one XCD: its keys and values stay in that L2
+  else { bh = blockIdx.x / each; pool = blockIdx.x % each; }
+  slice = a.slices == 1 ? 0 : pool / a.pools;
+  pool -= slice * a.pools;
   return bh < nbh;
+}
+// where a slice's sums of a row begin (`row` counts the call's rows: (sample, position, head))
+__device__ __forceinline__ long part_row(const Args& a, int slice, long row) { return (long)slice * ((long)a.B * a.Lq * a.Hq) + row; }
+
+// 8 features of a row's output, what their rounding lost and the row's statistic, from its sums f and its maximum, sum of the
+// weights and sum of the weights as rounded
+template <int D>
+__device__ __forceinline__ void write_out(const Args& a, float (&f)[8], const f32x4_t& st, long row, int c, long lrow) {
+  const float inv = 1.0f / st[2];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) f[x] = st[2] == 0.f ? 0.f : f[x] * inv;
+  const bf16x8_t y = dm_pack8(f);
+  *(bf16x8_t*)(a.out + row * D + c * 8) = y;
+  if (a.out_lo) {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) f[x] -= (float)y[x];
+    *(bf16x8_t*)(a.out_lo + row * D + c * 8) = dm_pack8(f);
+  }
+  if (a.lse && c == 0) a.lse[lrow] = st[2] == 0.f ? -INFINITY : st[0] * LN2 + logf(st[1]);
 }
 
 template <int D>
-__global__ __launch_bounds__(POOL, D <= 16 ? 6 : 2) void attend_pool_kernel(Args a) {
+__global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_pool_kernel(Args a) {
   using GE = Geo<D>;
   using PL = Pool<D>;
   constexpr int P = POOL;
@@ -443,15 +471,15 @@ __global__ __launch_bounds__(POOL, D <= 16 ? 6 : 2) void attend_pool_kernel(Args
   __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
   __shared__ __attribute__((aligned(16))) f32x4_t stat[P + 1];   // maximum, sum of the weights, sum of the weights as rounded
   __shared__ unsigned rowoff[P + 1];
-  int bh, pool;
-  if (!pool_of_block(a.B * a.Hkv, a.pools, bh, pool)) return;
-  PL w(a, bh, pool);
+  int bh, pool, slice;
+  if (!pool_of_block(a, bh, pool, slice)) return;
+  PL w(a, bh, pool, slice);
   const int tid = threadIdx.x, lane = w.lane, g = w.g;
   const float sc = a.scale * LOG2E, asc = fabsf(sc);   // (the sign of the scale goes to q: a maximum is scaled by the amount)
   const bf16_t one = (bf16_t)1.f;
   const bf16x8_t ones = {one, one, one, one, one, one, one, one};
   const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
-  Visits visits(PL::offsets(a, bh, pool), w.nb, lane);
+  Visits visits(PL::offsets(a, bh, pool), w.lo, w.nb, lane);
   Hit cur = visits.next(0);
   if (cur.j >= 0) {
     w.fetch(cur.j);
@@ -561,22 +589,78 @@ __global__ __launch_bounds__(POOL, D <= 16 ? 6 : 2) void attend_pool_kernel(Args
     int h;
     w.place(r, i, h);
     const f32x4_t st = stat[r];
-    const float inv = 1.0f / st[2];
-    float f[8], lo[8];
+    float f[8];
     *(f32x4_t*)f = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2));
     *(f32x4_t*)(f + 4) = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2 + 1));
-#pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = st[2] == 0.f ? 0.f : f[x] * inv;
-    const bf16x8_t y = dm_pack8(f);
-    const long at = (((long)w.b * a.Lq + i) * a.Hq + h) * D + c * 8;
-    *(bf16x8_t*)(a.out + at) = y;
-    if (a.out_lo) {
-#pragma unroll
-      for (int x = 0; x < 8; ++x) lo[x] = f[x] - (float)y[x];
-      *(bf16x8_t*)(a.out_lo + at) = dm_pack8(lo);
+    const long at = ((long)w.b * a.Lq + i) * a.Hq + h;
+    if (a.slices == 1) {
+      write_out<D>(a, f, st, at, c, ((long)w.b * a.Hq + h) * a.Lq + i);
+    } else {
+      const long p = part_row(a, w.slice, at);
+      *(f32x4_t*)(a.part + p * D + c * 8) = *(const f32x4_t*)f;
+      *(f32x4_t*)(a.part + p * D + c * 8 + 4) = *(const f32x4_t*)(f + 4);
+      if (c == 0) a.part_stat[p] = st;
     }
-    if (a.lse && c == 0) a.lse[((long)w.b * a.Hq + h) * a.Lq + i] = st[2] == 0.f ? -INFINITY : st[0] * LN2 + logf(st[1]);
   }
+}
+
+// The slices of a split pool become one: their sums, brought to a common maximum, in the order of the slices
+template <int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(Args a) {
+  constexpr int PC = D / 8;
+  const long e = dm_block_index() * 256 + threadIdx.x, at = e / PC;
+  const int c = (int)(e % PC);
+  if (at >= (long)a.B * a.Lq * a.Hq) return;
+  f32x4_t st[MAX_SLICES];
+  float m = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < MAX_SLICES; ++s)
+    if (s < a.slices) st[s] = a.part_stat[part_row(a, s, at)];
+#pragma unroll
+  for (int s = 0; s < MAX_SLICES; ++s)
+    if (s < a.slices) m = fmaxf(m, st[s][0]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  f32x4_t all = {m, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < MAX_SLICES; ++s)
+    if (s < a.slices) {
+      const float* p = a.part + part_row(a, s, at) * D + c * 8;
+      const f32x4_t x = *(const f32x4_t*)p, y = *(const f32x4_t*)(p + 4);
+      const float by = __builtin_amdgcn_exp2f(st[s][0] - base);
+      all[1] += st[s][1] * by;
+      all[2] += st[s][2] * by;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f[k] += x[k] * by;
+        f[k + 4] += y[k] * by;
+      }
+    }
+  const long h = at % a.Hq, i = at / a.Hq % a.Lq, b = at / ((long)a.Hq * a.Lq);
+  write_out<D>(a, f, all, at, c, (b * a.Hq + h) * a.Lq + i);
+}
+template <int D>
+__global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
+  constexpr int PC = D / 8;
+  const long e = dm_block_index() * 256 + threadIdx.x, at = e / PC;
+  const int c = (int)(e % PC);
+  if (at >= (long)a.B * a.Lq * a.Hq) return;
+  float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < MAX_SLICES; ++s)
+    if (s < a.slices) {
+      const float* p = a.part + part_row(a, s, at) * D + c * 8;
+      const f32x4_t x = *(const f32x4_t*)p, y = *(const f32x4_t*)(p + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f[k] += x[k];
+        f[k + 4] += y[k];
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] *= a.scale;
+  const long h = at % a.Hq, i = at / a.Hq % a.Lq, b = at / ((long)a.Hq * a.Lq);
+  *(bf16x8_t*)(a.dq + b * a.dqb + i * a.dql + h * a.dqh + c * 8) = dm_pack8(f);
 }
 
 // dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end.
@@ -589,13 +673,13 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
   __shared__ f32x2_t stat[P + 1];   // lse, -delta (the products of do and v start from it)
   __shared__ unsigned rowoff[P + 1], gooff[P + 1];
-  int bh, pool;
-  if (!pool_of_block(a.B * a.Hkv, a.pools, bh, pool)) return;
-  PL w(a, bh, pool);
+  int bh, pool, slice;
+  if (!pool_of_block(a, bh, pool, slice)) return;
+  PL w(a, bh, pool, slice);
   const int tid = threadIdx.x, lane = w.lane, g = w.g;
   const float sc = a.scale * LOG2E;
   const f32x4_t zero4 = {0.f, 0.f, 0.f, 0.f};
-  Visits visits(PL::offsets(a, bh, pool), w.nb, lane);
+  Visits visits(PL::offsets(a, bh, pool), w.lo, w.nb, lane);
   Hit cur = visits.next(0);
   if (cur.j >= 0) {
     w.fetch(cur.j);
@@ -629,7 +713,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     if (c == 0) {
       const float lse = in ? a.lse[lrow] : 0.f;
       stat[r] = f32x2_t{lse == -INFINITY ? INFINITY : lse * LOG2E, -delta};   // no key: every weight becomes zero
-      if (in) a.delta[lrow] = delta;
+      if (in && w.slice == 0) a.delta[lrow] = delta;
     }
   }
   __syncthreads();
@@ -729,9 +813,15 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
     float f[8];
     *(f32x4_t*)f = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2));
     *(f32x4_t*)(f + 4) = *(const f32x4_t*)(acc + acc_at<D>(r, c * 2 + 1));
+    if (a.slices == 1) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] *= a.scale;
-    *(bf16x8_t*)(a.dq + w.b * a.dqb + i * a.dql + h * a.dqh + c * 8) = dm_pack8(f);
+      for (int x = 0; x < 8; ++x) f[x] *= a.scale;
+      *(bf16x8_t*)(a.dq + w.b * a.dqb + i * a.dql + h * a.dqh + c * 8) = dm_pack8(f);
+    } else {
+      float* p = a.part + part_row(a, w.slice, ((long)w.b * a.Lq + i) * a.Hq + h) * D + c * 8;
+      *(f32x4_t*)p = *(const f32x4_t*)f;
+      *(f32x4_t*)(p + 4) = *(const f32x4_t*)(f + 4);
+    }
   }
 }
 
@@ -930,24 +1020,36 @@ int check_span(const char* who, const dm_block_desc* d) {
              "%s: a sample of q spans more than 2^35 elements", who);
   return check_pool(who, d);
 }
-// Whether the rows are taken in pools on the matrix cores or one query a workgroup. A pool's time is the number of its visits (its
-// blocks) times what a visit takes from barrier to barrier, however few rows want the block: 0.9 us up to 16 features, 1.05 us with
-// 32, 1.5 us with 64 (256 pools run at a time, twice as many up to 16 features); a query's is 0.3 ns + 0.5 .. 0.8 ns a block over the
-// whole chip. Both sides measured, forward (us), one query a workgroup against pools:
-//   8 heads x 256 queries, 8 of 64 blocks       D 8  16 / 57       D 64  25 / 84
-//   4 x 8 heads x 256 queries, 8 of 64          D 8  40 / 57       D 64  74 / 85
-//   4 x 8 heads x 1024 queries, 4 of 16         D 8  70 / 28       D 64  137 / 41
-//   2 x 8 heads x 2048 queries, 8 of 128        D 8  139 / 103     D 64  243 / 160
-//   4 x 8 heads x 4096 queries, 8 of 64         D 8  514 / 66      D 64  893 / 103
+// Whether the rows are taken in pools on the matrix cores or one query a workgroup, and in how many slices a pool's blocks are dealt to
+// workgroups (joined by attend_join_kernel and dq_join_kernel) where pools alone would leave CUs idle. A pool's time is the
+// number of its visits (its blocks) times what a visit takes from barrier to barrier, however few rows want the block: 0.9 us up to
+// 16 features, 1.05 us with 32, 1.5 us with 64 (256 pools run at a time, twice as many up to 16 features); a slice's sums cross
+// memory twice (3 TB/s); a query's time is 0.3 ns + 0.5 .. 0.8 ns a block over the whole chip, a quarter less where little of it is
+// in use. Measured, a forward call on its own (us): one query a workgroup / pools unsplit / as the rule splits them
+//   8 heads x 256 queries, 8 of 64 blocks       D 8  16 / 57 / 25       D 64  25 / 84 / 28
+//   4 x 8 heads x 256 queries, 8 of 64          D 8  40 / 57 / 27       D 64  74 / 85 / 31
+//   4 x 8 heads x 1024 queries, 4 of 16         D 8  70 / 28 / 28       D 64  132 / 41 / 40
+//   2 x 8 heads x 2048 queries, 8 of 128        D 8  139 / 103 / 44     D 64  243 / 160 / 91
+//   4 x 8 heads x 4096 queries, 8 of 64         D 8  507 / 66 / 58      D 64  893 / 103 / 95
+//   2 heads of 4 x 200 queries, 16 of 256       D 8  15 / 191 / 45      D 64  41 / 309 / 57
 // (Pools of 128 and 256 rows, which occupy more CUs where there are few rows, were never faster by more than 5 %.)
-bool pooled(const dm_block_desc* d) {
-  if (d->pool) return d->pool == POOL;
+struct Form { bool pool; int slices; };
+Form form_of(const dm_block_desc* d) {
   // The two round differently, and a sample's result must not depend on the batch it is in: the choice is priced for 4 samples.
   const double rows = (double)d->Lq * (d->Hq / d->Hkv), heads = 4.0 * d->Hkv;
   const double at_once = d->D <= 16 ? 512 : 256, visit = d->D <= 16 ? 900 : d->D == 32 ? 1050 : 1500;
-  const double pools = heads * dm_cdiv((long)rows, POOL), rounds = (double)(long)((pools + at_once - 1) / at_once);
-  const double most = (rows < POOL ? rows : POOL) * d->top, visits = most < blocks_of(d) ? most : blocks_of(d);
-  return heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 6000.0 + rounds * visits * visit;
+  const double pools = heads * dm_cdiv((long)rows, POOL), most = (rows < POOL ? rows : POOL) * d->top;
+  const double visits = most < blocks_of(d) ? most : blocks_of(d);
+  Form f = {true, 1};
+  double best = 0;
+  for (int s = 1; s <= MAX_SLICES; s *= 2) {
+    const double rounds = (double)(long)((pools * s + at_once - 1) / at_once), moved = s > 1 ? heads * rows * s * (d->D * 4 + 16) * 2 : 0;
+    const double ns = (s > 1 ? 14000.0 : 8000.0) + rounds * visits / s * visit + moved / 3000;
+    if (s == 1 || ns < best) { best = ns; f.slices = s; }
+  }
+  if (d->pool) return Form{d->pool == POOL, 1};
+  f.pool = heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 1.25 * best;
+  return f;
 }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
 struct PlanLayout { int pools; size_t offs, bytes; };
@@ -966,6 +1068,7 @@ Args args_of(const dm_block_desc* d) {
   a.nblk = blocks_of(d);
   a.pools = plan_of(d).pools;
   a.scale = d->scale;
+  a.slices = 1;
   return a;
 }
 
@@ -973,12 +1076,19 @@ Args args_of(const dm_block_desc* d) {
 
 extern "C" size_t dm_block_attention_plan_bytes(const dm_block_desc* d, int for_backward) {
   const char* who = "dm_block_attention_plan_bytes";
-  if (check_desc(who, d) || check_span(who, d) || (!for_backward && !pooled(d))) return 0;
+  if (check_desc(who, d) || check_span(who, d) || (!for_backward && !form_of(d).pool)) return 0;
   return plan_of(d).bytes;
 }
 
+extern "C" size_t dm_block_attention_fwd_ws_bytes(const dm_block_desc* d) {
+  const char* who = "dm_block_attention_fwd_ws_bytes";
+  if (check_desc(who, d) || check_span(who, d)) return 0;
+  const Form f = form_of(d);
+  return f.pool && f.slices > 1 ? (size_t)f.slices * d->B * d->Hq * d->Lq * (d->D * 4 + 16) : 0;
+}
+
 extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
-                                      const int* k_len, void* out, void* out_lo, float* lse, void* plan, void* stream) {
+                                      const int* k_len, void* out, void* out_lo, float* lse, void* plan, void* ws, size_t ws_bytes, void* stream) {
   const char* who = "dm_block_attention_fwd";
   int rc = check_desc(who, d);
   if (rc) return rc;
@@ -990,8 +1100,11 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   a.q = rows_of(q, d->q_stride); a.k = rows_of(k, d->k_stride); a.v = rows_of(v, d->v_stride);
   a.blocks = blocks; a.k_len = k_len; a.out = (bf16_t*)out; a.out_lo = (bf16_t*)out_lo; a.lse = lse;
   hipStream_t st = (hipStream_t)stream;
-  const bool pool = pooled(d);
+  const Form form = form_of(d);
+  const bool pool = form.pool;
   DM_REQUIRE(aligned(plan) || (!plan && !pool), DM_ERR_ARG, "%s: this shape needs a plan (dm_block_attention_plan_bytes), 16-byte aligned", who);
+  const size_t need = dm_block_attention_fwd_ws_bytes(d);
+  DM_REQUIRE(!need || (aligned(ws) && ws_bytes >= need), DM_ERR_ARG, "%s: workspace of %zu bytes is too small or misaligned (%zu)", who, ws_bytes, need);
   if (plan) {
     const PlanLayout p = plan_of(d);
     int* offs = (int*)plan;
@@ -1001,16 +1114,33 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
     DM_CHECK_LAUNCH();
   }
   const long rows = (long)d->B * d->Hq * d->Lq;
-  if (pool) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
+  if (pool) {
+    a.slices = form.slices;
+    if (a.slices > 1) {
+      a.part = (float*)ws;
+      a.part_stat = (f32x4_t*)(a.part + a.slices * rows * d->D);
+    }
+    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools * a.slices), dim3(POOL), 0, st, a))
+    if (a.slices > 1) {
+      DM_CHECK_LAUNCH();
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_join_kernel<HD>), dm_grid((rows * (HD / 8) + 255) / 256), dim3(256), 0, st, a))
+    }
+  }
   else if ((long)d->Hq * d->Lq < 512) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 4>), dm_grid(rows), dim3(256), 0, st, a, rows))
   else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_row_kernel<HD, 1>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
 
+// (delta first in the workspace, the slices' sums behind it)
+static size_t delta_bytes(size_t rows) { return (rows * 4 + 15) / 16 * 16; }
+
 extern "C" size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d) {
-  if (check_desc("dm_block_attention_bwd_ws_bytes", d)) return 0;
-  return (size_t)d->B * d->Hq * d->Lq * 4;
+  const char* who = "dm_block_attention_bwd_ws_bytes";
+  if (check_desc(who, d) || check_pool(who, d)) return 0;
+  const Form f = form_of(d);
+  const size_t rows = (size_t)d->B * d->Hq * d->Lq;
+  return delta_bytes(rows) + (f.pool && f.slices > 1 ? f.slices * rows * d->D * 4 : 0);
 }
 
 extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
@@ -1039,7 +1169,16 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   a.dvb = d->dv_stride[0]; a.dvl = d->dv_stride[1]; a.dvh = d->dv_stride[2];
   hipStream_t st = (hipStream_t)stream;
   const long rows = (long)d->B * d->Hq * d->Lq;
-  if (pooled(d)) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools), dim3(POOL), 0, st, a))
+  const Form form = form_of(d);
+  if (form.pool) {
+    a.slices = form.slices;
+    a.part = (float*)((char*)ws + delta_bytes(rows));
+    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools * a.slices), dim3(POOL), 0, st, a))
+    if (a.slices > 1) {
+      DM_CHECK_LAUNCH();
+      BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_join_kernel<HD>), dm_grid((rows * (HD / 8) + 255) / 256), dim3(256), 0, st, a))
+    }
+  }
   else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
   BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a));

@@ -102,7 +102,8 @@ _SIGNATURES = {
     "dm_block_keys": (c_int, [P] * 5),
     "dm_block_select": (c_int, [P] * 6),
     "dm_block_attention_plan_bytes": (ctypes.c_size_t, [P, c_int]),
-    "dm_block_attention_fwd": (c_int, [P] * 11),
+    "dm_block_attention_fwd_ws_bytes": (ctypes.c_size_t, [P]),
+    "dm_block_attention_fwd": (c_int, [P] * 11 + [ctypes.c_size_t, P]),
     "dm_block_attention_bwd_ws_bytes": (ctypes.c_size_t, [P]),
     "dm_block_attention_bwd": (c_int, [P] * 15 + [ctypes.c_size_t, P]),
     "dm_token_embed": (c_int, [P, P, P, c_int, c_long, c_long, c_int, c_float, P]),

@@ -944,13 +944,15 @@ def _block_forward(d, q, k, v, blocks, k_len, training):
     """The output and, for training, what the backward pass needs besides it in one tensor: the plan, what out's rounding lost
     and the statistics (_block_kept)."""
     out = torch.empty((d.B, d.Lq, d.Hq, d.D), dtype=BF16, device=q.device)
-    n = lib.dm_block_attention_plan_bytes(ctypes.byref(d), int(training))
+    ref = ctypes.byref(d)
+    n, need = lib.dm_block_attention_plan_bytes(ref, int(training)), lib.dm_block_attention_fwd_ws_bytes(ref)
+    ws = _scratch(q.device, (need + 3) // 4) if need else None
     out_lo, lse, size = _block_kept(d, n) if training else (0, 0, n)
     kept = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     at = kept.data_ptr() if size else 0
-    check(lib.dm_block_attention_fwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
+    check(lib.dm_block_attention_fwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len),
                                      out.data_ptr(), at + out_lo if training else None, at + lse if training else None,
-                                     at or None, _stream()))
+                                     at or None, _p(ws), need, _stream()))
     return out, kept
 
 

@@ -301,8 +301,9 @@ int dm_attention_bwd(const void* qkv, const void* out, const void* dout, const f
 typedef struct dm_block_desc {
   int B, Lq, Lk, Hq, Hkv, D;
   int top;      /* blocks a query names, 1 .. 64 */
-  int pool;     /* 512: many queries together on the matrix cores (attention: in pools of 512); 1: every query by itself;
-                   0: by the shape. The same in an attention's backward call as in its forward call */
+  int pool;     /* 512: many queries together on the matrix cores (attention: in unsplit pools of 512); 1: every query by
+                   itself; 0: by the shape (and where pools are few their blocks are split). The same in an attention's
+                   backward call as in its forward call */
   float scale;  /* of q . k */
   long q_stride[3], k_stride[3], v_stride[3];
   long dq_stride[3], dk_stride[3], dv_stride[3];   /* backward only */
@@ -318,11 +319,14 @@ int dm_block_select(const dm_block_desc* d, const void* q, const void* keys, con
  * repeated block counts once, numbers outside 0 .. nblk-1 name none), times v. A query without a key gets zeros.
  * For the backward call: out_lo bf16, what the rounding of out lost; lse fp32 [B][Hq][Lq] (natural log; -infinity without
  * a key); both may be null. plan: the rows of every block, written here and read by the backward call;
- * dm_block_attention_plan_bytes(d, whether there will be one), 16-byte aligned, null where that is 0.
+ * dm_block_attention_plan_bytes(d, whether there will be one), 16-byte aligned, null where that is 0. ws:
+ * dm_block_attention_fwd_ws_bytes, 16-byte aligned, null where that is 0, contents irrelevant.
  * A sample of q spans less than 2^35 elements. */
 size_t dm_block_attention_plan_bytes(const dm_block_desc* d, int for_backward);
+size_t dm_block_attention_fwd_ws_bytes(const dm_block_desc* d);
 int dm_block_attention_fwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
-                           const int* k_len, void* out, void* out_lo, float* lse, void* plan, void* stream);
+                           const int* k_len, void* out, void* out_lo, float* lse, void* plan, void* ws, size_t ws_bytes,
+                           void* stream);
 /* dq, dk, dv bf16 by their strides, written (keys that no query attended get zeros), from what the forward call was
  * given and wrote. ws: dm_block_attention_bwd_ws_bytes, 16-byte aligned, contents irrelevant. */
 size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d);

@@ -252,6 +252,44 @@ def test_block_attention(B, Lq, Lk, Hq, Hkv, D, top, ragged, pool):
 
 
 @gpu
+@pytest.mark.parametrize("chosen", ["any", "one block"])
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", [
+    (2, 700, 5000, 4, 2, 8, 12, True),
+    (1, 900, 3000, 6, 3, 16, 9, False),
+    (3, 333, 4111, 8, 2, 32, 7, True),
+    (2, 520, 4111, 4, 1, 64, 10, True),
+])
+def test_block_attention_of_split_pools(B, Lq, Lk, Hq, Hkv, D, top, ragged, chosen):
+    """Few pools with many blocks: the blocks are dealt to several workgroups, whose sums are joined."""
+    import ctypes
+    from dm_hip import lib
+    g = gen(16)
+    q, k, v, do = randn(g, B, Lq, Hq, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lq, Hq, D)
+    k_len = torch.tensor([Lk - 1, 0, Lk // 3], dtype=torch.int32, device="cuda")[:B] if ragged else None
+    if ragged:
+        for b in range(B):
+            k[b, int(k_len[b]):], v[b, int(k_len[b]):] = float("nan"), float("inf")
+    blocks = some_blocks(g, B, Hq, Lq, -(-Lk // BLOCK), top)
+    if chosen == "one block":
+        blocks.fill_(2)
+    desc = ops()._block_desc(B, Lq, Lk, Hq, Hkv, D, top, 1.0, q, k, v)
+    assert lib.dm_block_attention_fwd_ws_bytes(ctypes.byref(desc)) > 0
+    scale = 1.3 * D ** -0.5
+    ref = ref_attention(q, k, v, blocks, scale, k_len, do)
+
+    def run(sl):
+        leaves = [x[sl].clone().requires_grad_(True) for x in (q, k, v)]
+        out = ops().block_attention(*leaves, blocks[sl], scale, None if k_len is None else k_len[sl])
+        return [out.detach(), *torch.autograd.grad(out, leaves, do[sl])]
+    got = run(slice(0, B))
+    for name, x, (want, bound) in zip(("out", "dq", "dk", "dv"), got, ref):
+        within(name, x, want, bound)
+    assert torch.equal(ops().block_attention(q, k, v, blocks, scale, k_len), got[0])
+    for x, y in zip(got, run(slice(B - 1, B))):   # the same bits alone
+        assert torch.equal(x[B - 1:], y)
+
+
+@gpu
 @pytest.mark.parametrize("pool", [1, 512])
 def test_block_attention_of_one_sharp_weight(pool):
     """One key takes (almost) all the weight: ds is a small difference of large numbers."""
@@ -392,6 +430,8 @@ def test_block_attention_same_bits_whatever_the_batch():
     (5000, 70000, 12, 3, "bfloat16", 1.0),      # three sort passes
     (8192, 3000, 8, None, "float32", 1.0),      # the largest call that one workgroup sorts
     (8193, 70000, 8, 2, "float32", 1.0),        # ... and the smallest that it does not
+    (526000, 700, 8, None, "float32", 1.0),     # so many tiles that their counts are summed by themselves
+    (1100000, 300000, 2, 3, "bfloat16", 1.0),   # ... in three passes
     (9000, 2 ** 24 + 5, 4, 2, "float32", 1.0),  # four passes
     (30000, 2, 8, None, "float32", 1.0),        # two runs over nearly every chunk
     (66000, 3, 1, None, "bfloat16", 1.0),       # one feature; long chunks and joins of many parts
@@ -502,14 +542,14 @@ def test_refusals_of_the_c_abi():
     assert lib.dm_block_keys(desc(), ctypes.c_void_p(4100), None, p, None) == 1
     assert lib.dm_block_select(desc(q_stride=[2048, 33, 16]), p, p, None, p, None) == 1
     assert lib.dm_block_select(desc(), p, p, None, None, None) == 1
-    assert lib.dm_block_attention_fwd(desc(), p, p, p, None, None, p, None, None, None, None) == 1
-    assert lib.dm_block_attention_fwd(desc(pool=512), p, p, p, p, None, p, None, None, None, None) == 1
+    assert lib.dm_block_attention_fwd(desc(), p, p, p, None, None, p, None, None, None, None, 0, None) == 1
+    assert lib.dm_block_attention_fwd(desc(pool=512), p, p, p, p, None, p, None, None, None, None, 0, None) == 1
     assert "plan" in lib.dm_last_error().decode()
     assert lib.dm_block_attention_bwd(desc(), p, p, p, p, None, p, p, p, p, p, p, p, p, p, 8, None) == 1
     assert "workspace" in lib.dm_last_error().decode()
     assert lib.dm_block_attention_plan_bytes(desc(D=3), 1) == 0
     assert lib.dm_block_attention_plan_bytes(desc(pool=64), 1) == 0
-    assert lib.dm_block_attention_fwd(desc(q_stride=[0, 2 ** 32, 16]), p, p, p, p, None, p, None, None, p, None) == 2
+    assert lib.dm_block_attention_fwd(desc(q_stride=[0, 2 ** 32, 16]), p, p, p, p, None, p, None, None, p, None, 0, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 5, 0, 4, 1.0, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 2 ** 31, 9, 4, 1.0, None) == 2
     assert lib.dm_token_embed(p, p, p, 0, 5, 9, 0, 1.0, None) == 2
