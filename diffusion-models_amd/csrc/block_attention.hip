@@ -35,6 +35,8 @@ struct Args {
 // queries, else 1). A block's keys and values are read as whole rows, D/8 lanes a row with 16 bytes each, the next block's
 // while this one is computed; the lanes that hold a key's features also hold the same features of its value, so a
 // weight never moves between lanes.
+// Bound by the latency of a query's chain of blocks where the queries are few (2 x 32 heads with one query, 16 of 1025 blocks of 64
+// features: 13 us for 16.8 MB, 1.3 TB/s), by the caches' traffic where they are many, which is where the pools take over.
 template <int D, int NW>
 __global__ __launch_bounds__(256) void attend_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
@@ -158,7 +160,8 @@ __global__ __launch_bounds__(256) void attend_row_kernel(Args a, long rows) {
   }
 }
 
-// dq of one query a wave, and delta for the kernel behind
+// dq of one query a wave, and delta for the kernel behind: blocks are read once more from the caches (2 x 4 heads x 200 queries, 16 of
+// 256 blocks of 64 features: the whole backward pass takes what its host calls take)
 template <int D>
 __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
@@ -223,8 +226,14 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 // The lists of rows are made once for all passes (block_plan_kernel). A block's keys and values are staged in LDS for all waves,
 // one block ahead. A wave's tiles are a sequence of their own that runs ahead of the visits: while a tile is computed, the rows of the
 // wave's next one are on their way from global memory straight into matrix operands, and the row numbers of the one
-// behind that. (Keys fetched that way too, so that only V needs LDS, arrive late: every wave gathers the whole block by 64-byte
-// pieces; 64x64 forward 134 us against 116.)
+// behind that.
+//
+// What bounds it is the latency of a visit: with 8 of 64 blocks a pool has 4 or 5 tiles a visit, one to a wave, so LDS reads, two
+// products, 16 exponentials a lane, the write-back and a barrier stand one behind the other (of 1.5 us with 64 features: LDS reads of K 0.17,
+// of V and sums 0.16, exponentials 0.15, second product and write-back 0.2, staging and barriers 0.3). 4 x 8 heads of 4096 queries and
+// 64 features, 8 of 64 blocks: 95 us, 0.36 PFLOP/s of tile work, 0.75 TB/s of the bytes. Measured and slower: keys fetched straight into
+// operands, so that only V needs LDS (134 us against 116 then: every wave gathers the block by 64-byte pieces); two tiles of a wave
+// at once (110 against 99: registers, hence fewer waves); 10 or 12 waves a pool (103 .. 105 against 102).
 //
 // Products are formed transposed, S^T = K Q^T: a lane then holds 4 keys x 4 tiles of ONE row (lane & 15), the row's
 // maximum and sum are two lane swaps away, and exp(S^T) is in the register layout that the second product takes as its
@@ -235,7 +244,7 @@ constexpr int POOL = 512, MAX_SLICES = 8;
 // offs[b][hkv][pool][0 .. nblk]: where the rows of a block begin in rows[b][hkv][pool][512 top] (numbers inside the pool,
 // ascending). A set: a block that a query names twice counts once, numbers outside 0 .. nblk-1 name none.
 // A thread is a row. It sets its bit in the words of its blocks; after the counts' prefix sums a row's place in a block's list is the
-// block's start + the bits of earlier words + those of earlier lanes.
+// block's start + the bits of earlier words + those of earlier lanes. Four barriers for 256 blocks: 8 us for 256 pools, 8 of 64 blocks.
 constexpr int PLAN_CHUNK = 256;   // blocks at a time
 __global__ __launch_bounds__(POOL) void block_plan_kernel(const int* __restrict__ blocks, int* __restrict__ offs,
                                                           unsigned short* __restrict__ rows, int Lq, int Hq, int G, int top, int nblk,
@@ -604,7 +613,8 @@ __global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_poo
   }
 }
 
-// The slices of a split pool become one: their sums, brought to a common maximum, in the order of the slices
+// The slices of a split pool become one: their sums, brought to a common maximum, in the order of the slices. (4 or 5 us for 13320 rows
+// of 32 features, 8 slices: 17 MB, 3.4 TB/s.)
 template <int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(Args a) {
   constexpr int PC = D / 8;
@@ -663,7 +673,8 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
   *(bf16x8_t*)(a.dq + b * a.dqb + i * a.dql + h * a.dqh + c * 8) = dm_pack8(f);
 }
 
-// dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end.
+// dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end. Bound as the
+// forward kernel is, with one product more in a visit (the call above: 115 us).
 template <int D>
 __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   using GE = Geo<D>;
@@ -829,6 +840,8 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 // waves in tiles of 32; every wave sums all 64 keys over its own rows in registers, and the four sums are added in wave
 // order. Scores are formed as S = Q K^T here: a lane holds 4 rows x 2 tiles of ONE key, which is the layout that dv =
 // P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
+// Bound by registers with 64 features (the sums of 64 keys take 128; 2 waves a SIMD) and by the gather of 32 rows a tile: 107 us for 4 x 8
+// heads of 4096 queries and keys, 8 of 64 blocks, 0.32 PFLOP/s; 86 us for 8 x 64 heads of 1024 and 8 features, 4 of 16.
 constexpr int LIST = 4096;
 template <int D>
 __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel(Args a) {
