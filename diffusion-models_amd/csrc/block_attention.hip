@@ -454,8 +454,7 @@ __device__ __forceinline__ bool pool_of_block(const Args& a, int& bh, int& pool,
 // where a slice's sums of a row begin (`row` counts the call's rows: (sample, position, head))
 __device__ __forceinline__ long part_row(const Args& a, int slice, long row) { return (long)slice * ((long)a.B * a.Lq * a.Hq) + row; }
 
-// 8 features of a row's output, what their rounding lost and the row's statistic, from its sums f and its maximum, sum of the
-// weights and sum of the weights as rounded
+// 8 features of a row's output, what their rounding lost and the row's statistic, from its sums f and its `stat`
 template <int D>
 __device__ __forceinline__ void write_out(const Args& a, float (&f)[8], const f32x4_t& st, long row, int c, long lrow) {
   const float inv = 1.0f / st[2];
@@ -471,14 +470,18 @@ __device__ __forceinline__ void write_out(const Args& a, float (&f)[8], const f3
   if (a.lse && c == 0) a.lse[lrow] = st[2] == 0.f ? -INFINITY : st[0] * LN2 + logf(st[1]);
 }
 
-template <int D>
+// KEEP: for a backward call. The weights are the matrix instruction's operands in bf16: for an output alone rounded, and the output is
+// divided by the sum of the ROUNDED weights (one more product, with ones), so that it stays an average of values and a rounding
+// counts only with the value's distance from the output. With KEEP as a pair, the rounded weight and what the rounding lost (2^-17),
+// and the output is divided by the weights' own sum: delta is taken from it, and would pass its error on to every ds of the row.
+template <int D, bool KEEP>
 __global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_pool_kernel(Args a) {
   using GE = Geo<D>;
   using PL = Pool<D>;
   constexpr int P = POOL;
   __shared__ __attribute__((aligned(16))) char kv[PL::BUFS][PL::KV];
   __shared__ __attribute__((aligned(16))) float acc[(P + 1) * GE::DV];
-  __shared__ __attribute__((aligned(16))) f32x4_t stat[P + 1];   // maximum, sum of the weights, sum of the weights as rounded
+  __shared__ __attribute__((aligned(16))) f32x4_t stat[P + 1];   // maximum, sum of the weights (KEEP), what the output is divided by
   __shared__ unsigned rowoff[P + 1];
   int bh, pool, slice;
   if (!pool_of_block(a, bh, pool, slice)) return;
@@ -549,18 +552,22 @@ __global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_poo
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * asc - at);
       w.behind(n0, [&](int e) { s[e] = 0.f; });   // (a scale of zero times -infinity is no zero)
       float sum = 0.f;
-      if (a.lse) {   // (only the saved statistic needs it)
+      if (KEEP) {
         float part[4];
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) part[kt] = (s[kt * 4] + s[kt * 4 + 1]) + (s[kt * 4 + 2] + s[kt * 4 + 3]);
-        sum = row_sum((part[0] + part[1]) + (part[2] + part[3]));
+        sum = st[1] * alpha + row_sum((part[0] + part[1]) + (part[2] + part[3]));
       }
-      // The weights are rounded to bf16 as the matrix instruction's operand. The output is divided by the sum of the
-      // ROUNDED weights (one more product, with ones), so that it stays an average of values: a rounding then counts only
-      // with the value's distance from the output. The saved statistic is of the unrounded ones.
-      bf16x8_t p[2];
+      bf16x8_t p[2], lost[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) p[u] = dm_pack8(s + u * 8);
+      for (int u = 0; u < 2; ++u) {
+        p[u] = dm_pack8(s + u * 8);
+        if (KEEP) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[u * 8 + e] -= (float)p[u][e];
+          lost[u] = dm_pack8(s + u * 8);
+        }
+      }
       const float r_old = st[2] * alpha;
       f32x4_t rs = {r_old, r_old, r_old, r_old};
 #pragma unroll
@@ -571,13 +578,16 @@ __global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_poo
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int dt = 0; dt < GE::DT; ++dt)
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join4(vt[dt][2 * u], vt[dt][2 * u + 1]), p[u], o[dt], 0, 0, 0);
-        rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
+        for (int dt = 0; dt < GE::DT; ++dt) {
+          const bf16x8_t values = join4(vt[dt][2 * u], vt[dt][2 * u + 1]);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, p[u], o[dt], 0, 0, 0);
+          if (KEEP) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, lost[u], o[dt], 0, 0, 0);
+        }
+        if (!KEEP) rs = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[u], rs, 0, 0, 0);
       }
 #pragma unroll
       for (int dt = 0; dt < GE::DT; ++dt) *(f32x4_t*)(acc + acc_at<D>(row, dt * 4 + g)) = o[dt];
-      stat[row] = f32x4_t{m_new, st[1] * alpha + sum, rs[0], 0.f};   // (four lanes, the same values)
+      stat[row] = f32x4_t{m_new, sum, KEEP ? sum : rs[0], 0.f};   // (four lanes, the same values)
       it = it1;
       row = row1;
       it1 = it2;
@@ -1133,7 +1143,9 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
       a.part = (float*)ws;
       a.part_stat = (f32x4_t*)(a.part + a.slices * rows * d->D);
     }
-    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD>), dim3(d->B * d->Hkv * a.pools * a.slices), dim3(POOL), 0, st, a))
+    const dim3 grid(d->B * d->Hkv * a.pools * a.slices);
+    if (lse || out_lo) BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, true>), grid, dim3(POOL), 0, st, a))
+    else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_pool_kernel<HD, false>), grid, dim3(POOL), 0, st, a))
     if (a.slices > 1) {
       DM_CHECK_LAUNCH();
       BY_HEAD_DIM(d->D, hipLaunchKernelGGL((attend_join_kernel<HD>), dm_grid((rows * (HD / 8) + 255) / 256), dim3(256), 0, st, a))

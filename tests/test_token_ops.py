@@ -284,7 +284,7 @@ def test_block_attention_of_split_pools(B, Lq, Lk, Hq, Hkv, D, top, ragged, chos
     got = run(slice(0, B))
     for name, x, (want, bound) in zip(("out", "dq", "dk", "dv"), got, ref):
         within(name, x, want, bound)
-    assert torch.equal(ops().block_attention(q, k, v, blocks, scale, k_len), got[0])
+    within("out without gradients", ops().block_attention(q, k, v, blocks, scale, k_len), *ref[0])
     for x, y in zip(got, run(slice(B - 1, B))):   # the same bits alone
         assert torch.equal(x[B - 1:], y)
 
