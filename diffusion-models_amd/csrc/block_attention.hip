@@ -960,40 +960,41 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes, read by its other lanes
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {   // 32 keys at a time (all 64 would not leave registers for the next rows)
-        bf16x8_t pt[2], dst[2];   // p and ds, rounded as the matrix instructions' operands
+      for (int kt = 0; kt < 4; ++kt) {   // 16 keys at a time (more would not leave registers for the next rows)
+        Frag<D> kf, vf;
+        kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
+        vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
+        float p[8], ds[8];
 #pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          const int kt = half * 2 + k2;
-          Frag<D> kf, vf;
-          kf.from_lds(kbuf, kt * 16 + (lane & 15), g);
-          vf.from_lds(vbuf, kt * 16 + (lane & 15), g);
-          float p[8], ds[8];
+        for (int mt = 0; mt < 2; ++mt) {
+          const f32x4_t ls = *(const f32x4_t*)(st_lse + mt * 16 + g * 4), de = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
+          const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf, de);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            const f32x4_t ls = *(const f32x4_t*)(st_lse + mt * 16 + g * 4), de = *(const f32x4_t*)(st_delta + mt * 16 + g * 4);
-            const f32x4_t s = dot_frag<D>(qf[mt], kf), dp = dot_frag<D>(of[mt], vf, de);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - ls[e]);
-              ds[mt * 4 + e] = p[mt * 4 + e] * dp[e];
-            }
+          for (int e = 0; e < 4; ++e) {
+            p[mt * 4 + e] = __builtin_amdgcn_exp2f(s[e] * sc - ls[e]);
+            ds[mt * 4 + e] = p[mt * 4 + e] * dp[e];
           }
-          pt[k2] = dm_pack8(p);
-          dst[k2] = dm_pack8(ds);
         }
-        if (half == 1 && (t + 4) * 32 < count) load(t + 4);   // on its way during the last products
+        if (kt == 3 && (t + 4) * 32 < count) load(t + 4);   // on its way during the last products
+        // p and ds as pairs of operands, rounded to bf16 and what that lost: weights of one size are rounded one way in every row, an error
+        // that their sum over rows would keep
+        const bf16x8_t ph = dm_pack8(p), dh = dm_pack8(ds);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] -= (float)ph[e];
+          ds[e] -= (float)dh[e];
+        }
+        const bf16x8_t pl = dm_pack8(p), dl = dm_pack8(ds);
 #pragma unroll
         for (int dt = 0; dt < GE::DT; ++dt) {
           const bf16x8_t qt = join4(read_tr<D>(qb, 0, dt, lane), read_tr<D>(qb, 16, dt, lane));
           const bf16x8_t ot = join4(read_tr<D>(ob, 0, dt, lane), read_tr<D>(ob, 16, dt, lane));
-#pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            const int kt = half * 2 + k2;
-            dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pt[k2], ot, dv[kt][dt], 0, 0, 0);
-            dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dst[k2], qt, dk[kt][dt], 0, 0, 0);
-          }
+          dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ph, ot, dv[kt][dt], 0, 0, 0);
+          dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dh, qt, dk[kt][dt], 0, 0, 0);
+          dv[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pl, ot, dv[kt][dt], 0, 0, 0);
+          dk[kt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dl, qt, dk[kt][dt], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);   // (the next keys' products would be begun before these are done, and spill)
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
