@@ -7,7 +7,8 @@
 //
 // Query heads share key heads (Hq = G Hkv). The ROWS of a (sample, key head) are its G Lq queries, r = i G + g: they all
 // read the same keys and values. delta is taken from out and what out's rounding lost (out_lo): where a query's weight lies on
-// few keys, ds is a small difference of do . v and delta, and the rounding of out alone would be as large. No kernel adds with float atomics: results do not depend on scheduling.
+// few keys, ds is a small difference of do . v and delta, and the rounding of out alone would be as large. No kernel adds with float
+// atomics: results do not depend on scheduling.
 #include "block_common.h"
 
 namespace {
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
 // What bounds it is the latency of a visit: with 8 of 64 blocks a pool has 4 or 5 tiles a visit, one to a wave, so LDS reads, two
 // products, 16 exponentials a lane, the write-back and a barrier stand one behind the other (of 1.5 us with 64 features: LDS reads of K 0.17,
 // of V and sums 0.16, exponentials 0.15, second product and write-back 0.2, staging and barriers 0.3). 4 x 8 heads of 4096 queries and
-// 64 features, 8 of 64 blocks: 95 us, 0.36 PFLOP/s of tile work, 0.75 TB/s of the bytes. Measured and slower: keys fetched straight into
+// 64 features, 8 of 64 blocks: 95 us, 0.18 PFLOP/s and 0.75 TB/s. Measured and slower: keys fetched straight into
 // operands, so that only V needs LDS (134 us against 116 then: every wave gathers the block by 64-byte pieces); two tiles of a wave
 // at once (110 against 99: registers, hence fewer waves); 10 or 12 waves a pool (103 .. 105 against 102).
 //
@@ -363,7 +364,8 @@ struct Pool {
 
   __device__ __forceinline__ Pool(const Args& a_, int bh_, int pool_, int slice_)
       : a(a_), bh(bh_), b(bh_ / a_.Hkv), hk(bh_ - (bh_ / a_.Hkv) * a_.Hkv), pool(pool_), slice(slice_), n(valid_keys(a_.k_len, bh_ / a_.Hkv, a_.Lk)),
-        lo((int)((long)((n + BLK - 1) / BLK) * slice_ / a_.slices)), nb((int)((long)((n + BLK - 1) / BLK) * (slice_ + 1) / a_.slices)), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
+        lo(share(n, slice_, a_.slices)), nb(share(n, slice_ + 1, a_.slices)), lane(threadIdx.x & 63),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l15(threadIdx.x & 15),
         g((threadIdx.x & 63) >> 4), rows(a_.rows + ((long)bh_ * a_.pools + pool_) * ((long)P * a_.top)),
         mine(offsets(a_, bh_, pool_), lo, nb, threadIdx.x & 63) {
 #pragma unroll
@@ -373,6 +375,9 @@ struct Pool {
       src[u] = r.p + b * r.sb + t * r.sl + hk * r.sh + c * 8;
       step[u] = BLK * r.sl;
     }
+  }
+  static __device__ __forceinline__ int share(int n, int slice, int slices) {   // where a slice's blocks begin
+    return (int)((long)((n + BLK - 1) / BLK) * slice / slices);
   }
   static __device__ __forceinline__ const int* offsets(const Args& a, int bh, int pool) {
     return a.offs + ((long)bh * a.pools + pool) * (a.nblk + 1);
@@ -473,7 +478,8 @@ __device__ __forceinline__ void write_out(const Args& a, float (&f)[8], const f3
 // KEEP: for a backward call. The weights are the matrix instruction's operands in bf16: for an output alone rounded, and the output is
 // divided by the sum of the ROUNDED weights (one more product, with ones), so that it stays an average of values and a rounding
 // counts only with the value's distance from the output. With KEEP as a pair, the rounded weight and what the rounding lost (2^-17),
-// and the output is divided by the weights' own sum: delta is taken from it, and would pass its error on to every ds of the row.
+// and the output is divided by the weights' own sum: delta is taken from it, and would pass its error on to every ds of the row (111 us
+// for the call above).
 template <int D, bool KEEP>
 __global__ __launch_bounds__(POOL, D == 8 ? 5 : D == 16 ? 6 : 2) void attend_pool_kernel(Args a) {
   using GE = Geo<D>;
@@ -850,8 +856,9 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 // waves in tiles of 32; every wave sums all 64 keys over its own rows in registers, and the four sums are added in wave
 // order. Scores are formed as S = Q K^T here: a lane holds 4 rows x 2 tiles of ONE key, which is the layout that dv =
 // P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
-// Bound by registers with 64 features (the sums of 64 keys take 128; 2 waves a SIMD) and by the gather of 32 rows a tile: 107 us for 4 x 8
-// heads of 4096 queries and keys, 8 of 64 blocks, 0.32 PFLOP/s; 86 us for 8 x 64 heads of 1024 and 8 features, 4 of 16.
+// Bound by registers with 64 features (the sums of 64 keys take 128; 2 waves a SIMD) and by the latency of a tile's chain: 121 us for 4 x 8
+// heads of 4096 queries and keys, 8 of 64 blocks, 0.43 PFLOP/s issued; 109 us for 8 x 64 heads of 1024 and 8 features, 4 of 16. (p and
+// ds rounded once: 107 and 87 us. Pairs with 32 keys at a time: 148 and 138, registers spilled.)
 constexpr int LIST = 4096;
 template <int D>
 __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel(Args a) {
