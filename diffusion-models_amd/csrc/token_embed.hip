@@ -368,6 +368,14 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout
   }
 }
 
+// A table of zeros, for rows that no token names
+__global__ __launch_bounds__(256) void clear_kernel(float* __restrict__ to, long n, long vecs) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, step = (long)gridDim.x * 256;
+  for (long i = at; i < vecs; i += step) ((f32x4_t*)to)[i] = zero;
+  for (long i = vecs * 4 + at; i < n; i += step) to[i] = 0.f;
+}
+
 // A run that goes on behind the chunk it began in: its parts, chunk by chunk
 template <int V>
 __global__ __launch_bounds__(256) void run_join_kernel(const unsigned* __restrict__ key, const float* __restrict__ part,
@@ -478,7 +486,9 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   const char* who = "dm_token_embed_bwd";
   int rc = check_embed(who, n, rows, width);
   if (rc) return rc;
-  if (n == 0) return DM_OK;
+  DM_REQUIRE(accumulate >= 0 && accumulate <= 2, DM_ERR_ARG, "%s: accumulate is 0, 1 or 2, not %d", who, accumulate);
+  if (n == 0 && accumulate != 2) return DM_OK;
+  DM_REQUIRE(n > 0, DM_ERR_SHAPE, "%s: no tokens to write a table from", who);
   DM_REQUIRE(dout && tokens && dtable, DM_ERR_ARG, "%s: null pointer", who);
   const Plan p = plan_of(n, rows, width);
   DM_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= p.total, DM_ERR_ARG, "%s: workspace of %zu bytes is too small or misaligned (%zu)", who, ws_bytes, p.total);
@@ -488,6 +498,11 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   float* part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
+  if (accumulate == 2) {
+    const long all = rows * width, vecs = ((uintptr_t)dtable & 15) ? 0 : all / 4, groups = (all / 4 + 255) / 256;
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(groups < 1 ? 1 : groups > 4096 ? 4096 : groups)), block, 0, st, dtable, all, vecs);
+    DM_CHECK_LAUNCH();
+  }
   const int scan = p.tiles > SCAN_TILES;
   // one workgroup up to 8192 tokens (backward with 320 features, in one launch / in two a pass: 4999 tokens 26 / 35 us, 8192 32 / 37)
   if (n <= SMALL) {
@@ -511,7 +526,7 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   const unsigned *sk = key[(p.passes - 1) & 1], *si = idx[(p.passes - 1) & 1];
   const int V = vectors(width, dout, dtable, dout_bf16), tpr = sum_threads(width / V), chunk = chunk_of(n);
   const dim3 grid(dm_cdiv(p.chunks, 256 / tpr), dm_cdiv(width / V, tpr));
-#define GO(T, V) hipLaunchKernelGGL((run_sum_kernel<T, V>), grid, block, 0, st, (const T*)dout, sk, si, dtable, part, n, (unsigned)rows, width, scale, tpr, chunk, accumulate)
+#define GO(T, V) hipLaunchKernelGGL((run_sum_kernel<T, V>), grid, block, 0, st, (const T*)dout, sk, si, dtable, part, n, (unsigned)rows, width, scale, tpr, chunk, accumulate == 1)
   if (dout_bf16) { if (V == 8) GO(bf16_t, 8); else if (V == 4) GO(bf16_t, 4); else GO(bf16_t, 1); }
   else { if (V == 4) GO(float, 4); else GO(float, 1); }
 #undef GO
@@ -519,8 +534,8 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   if (p.chunks > 1) {
     const int W = V == 1 ? 1 : 4, t = sum_threads(width / W);   // (the parts are fp32 whatever dout is)
     const dim3 jgrid(dm_cdiv(p.chunks, 256 / t), dm_cdiv(width / W, t));
-    if (W == 4) hipLaunchKernelGGL((run_join_kernel<4>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate);
-    else hipLaunchKernelGGL((run_join_kernel<1>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate);
+    if (W == 4) hipLaunchKernelGGL((run_join_kernel<4>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate == 1);
+    else hipLaunchKernelGGL((run_join_kernel<1>), jgrid, block, 0, st, sk, part, dtable, n, (unsigned)rows, width, scale, t, chunk, accumulate == 1);
     DM_CHECK_LAUNCH();
   }
   return DM_OK;

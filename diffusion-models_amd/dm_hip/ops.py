@@ -853,6 +853,16 @@ def _on(device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def _once(backward):
+    """A Function's backward that has no derivative of its own: torch's once_differentiable, at its cost only where a second
+    derivative could be asked for."""
+    checked = once_differentiable(backward)
+
+    def once(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return once
+
+
 def _tokens4(t, name, who):
     """A bf16 [B, L, H, D] tensor whose rows of D can be read 16 bytes at a time; copied only if it is not one."""
     _require_device(t, who)
@@ -988,7 +998,7 @@ class _BlockAttentionFn(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         q, k, v, blocks, k_len, out, kept = ctx.saved_tensors
         with _on(q.device):
@@ -1053,7 +1063,7 @@ class _SparseAttentionFn(Function):
         return out.view(B, L, H * D)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         qkv, blocks, out, kept = ctx.saved_tensors
         d = ctx.d
@@ -1102,7 +1112,7 @@ class _TokenEmbedFn(Function):
         return _embed_rows(tokens, f32c(table.detach()), scale, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         (tokens,) = ctx.saved_tensors
         (rows, width), dtype, scale, padding = ctx.cfg
@@ -1111,13 +1121,14 @@ class _TokenEmbedFn(Function):
         dout = dout.contiguous()
         sink = _grad_sink(ctx.param)
         with _on(dout.device):
-            dtable = sink if sink is not None else torch.zeros((rows, width), dtype=torch.float32, device=dout.device)
             n = tokens.numel()
+            new = torch.empty if n and width else torch.zeros
+            dtable = sink if sink is not None else new((rows, width), dtype=torch.float32, device=dout.device)
             if n and width:
                 need = lib.dm_token_embed_bwd_ws_bytes(n, rows, width)
                 ws = _scratch(dout.device, (need + 3) // 4)
                 check(lib.dm_token_embed_bwd(dout.data_ptr(), int(dout.dtype == BF16), tokens.data_ptr(), dtable.data_ptr(), n, rows,
-                                             width, scale, padding, int(sink is not None), ws.data_ptr(), need, _stream()))
+                                             width, scale, padding, 2 if sink is None else 1, ws.data_ptr(), need, _stream()))
         if sink is not None:
             _grad_done(ctx.param)
             return None, None, None, None, None

@@ -341,8 +341,9 @@ int dm_block_attention_bwd(const dm_block_desc* d, const void* q, const void* k,
  * multiples of 4 run faster). */
 int dm_token_embed(const float* table, const int64_t* tokens, void* out, int out_bf16, long n, long rows, int width,
                    float scale, void* stream);
-/* dtable[t] += scale * sum of dout[i] over tokens[i] == t (accumulate != 0), or these rows are written (accumulate == 0);
- * rows without such a token are left alone either way. fp32 sums of neighbours in a sorted order, no float atomics: bitwise
+/* dtable[t] += scale * sum of dout[i] over tokens[i] == t (accumulate 1), or these rows are written (accumulate 0); rows
+ * without such a token are left alone either way. accumulate 2: the whole table is written, rows without one with zeros
+ * (n > 0). fp32 sums of neighbours in a sorted order, no float atomics: bitwise
  * reproducible. Tokens equal to `padding` (-1: none) or outside 0 .. rows-1 have no gradient.
  * ws: dm_token_embed_bwd_ws_bytes, 16-byte aligned, contents irrelevant. */
 size_t dm_token_embed_bwd_ws_bytes(long n, long rows, int width);
