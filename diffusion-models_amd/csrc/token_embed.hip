@@ -368,12 +368,17 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout
   }
 }
 
-// A table of zeros, for rows that no token names
+// A table of zeros, for rows that no token names. Bound by HBM's writes.
+constexpr int CLEAR = 4;   // 16-byte pieces a thread
 __global__ __launch_bounds__(256) void clear_kernel(float* __restrict__ to, long n, long vecs) {
   const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-  const long at = (long)blockIdx.x * 256 + threadIdx.x, step = (long)gridDim.x * 256;
-  for (long i = at; i < vecs; i += step) ((f32x4_t*)to)[i] = zero;
-  for (long i = vecs * 4 + at; i < n; i += step) to[i] = 0.f;
+  const long group = dm_block_index(), groups = (long)gridDim.x * gridDim.y;
+#pragma unroll
+  for (int u = 0; u < CLEAR; ++u) {
+    const long i = (group * CLEAR + u) * 256 + threadIdx.x;
+    if (i < vecs) ((f32x4_t*)to)[i] = zero;
+  }
+  for (long i = vecs * 4 + group * 256 + threadIdx.x; i < n; i += groups * 256) to[i] = 0.f;
 }
 
 // A run that goes on behind the chunk it began in: its parts, chunk by chunk
@@ -499,8 +504,8 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
   if (accumulate == 2) {
-    const long all = rows * width, vecs = ((uintptr_t)dtable & 15) ? 0 : all / 4, groups = (all / 4 + 255) / 256;
-    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(groups < 1 ? 1 : groups > 4096 ? 4096 : groups)), block, 0, st, dtable, all, vecs);
+    const long all = rows * width, vecs = ((uintptr_t)dtable & 15) ? 0 : all / 4;
+    hipLaunchKernelGGL(clear_kernel, dm_grid(all / (4 * 256 * CLEAR) + 1), block, 0, st, dtable, all, vecs);
     DM_CHECK_LAUNCH();
   }
   const int scan = p.tiles > SCAN_TILES;
