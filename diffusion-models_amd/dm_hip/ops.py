@@ -218,7 +218,7 @@ def _stream():
     that the consumer of the gradients has to wait for."""
     global LAUNCHES
     LAUNCHES += 1
-    raw = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())   # (current_stream().cuda_stream without the object)
+    raw = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())   # (current_stream().cuda_stream without the object)
     if _AUX:
         s = _AUX.get(raw)
         if s is not None:
@@ -850,7 +850,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device):
     """Context in which launches and scratch go to `device` (torch's current device may be another one)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _once(backward):
@@ -1095,11 +1095,12 @@ def sparse_attention(qkv, n_heads, head_dim, top, scale=None):
 
 # ------------------------------------------------------------------------------------------------------------
 def _embed_rows(tokens, table, scale, dtype):
+    rows, width = table.shape
+    n = tokens.numel()
     with _on(table.device):
-        out = torch.empty(tokens.shape + table.shape[1:], dtype=dtype, device=table.device)
-        if out.numel():
-            check(lib.dm_token_embed(table.data_ptr(), tokens.data_ptr(), out.data_ptr(), int(dtype == BF16), tokens.numel(),
-                                     table.shape[0], table.shape[1], scale, _stream()))
+        out = torch.empty((*tokens.shape, width), dtype=dtype, device=table.device)
+        if n and width:
+            check(lib.dm_token_embed(table.data_ptr(), tokens.data_ptr(), out.data_ptr(), dtype is BF16, n, rows, width, scale, _stream()))
     return out
 
 
@@ -1109,7 +1110,7 @@ class _TokenEmbedFn(Function):
         ctx.save_for_backward(tokens)
         ctx.param = table
         ctx.cfg = (tuple(table.shape), table.dtype, scale, padding)
-        return _embed_rows(tokens, f32c(table.detach()), scale, dtype)
+        return _embed_rows(tokens, f32c(table), scale, dtype)
 
     @staticmethod
     @_once
@@ -1156,7 +1157,7 @@ def token_embed(tokens, table, scale=1.0, padding_idx=None, dtype=BF16):
         tokens = tokens.to(torch.int64).contiguous()
     if torch.is_grad_enabled() and table.requires_grad:
         return _TokenEmbedFn.apply(table, tokens, float(scale), padding, dtype)
-    return _embed_rows(tokens, f32c(table.detach()), float(scale), dtype)
+    return _embed_rows(tokens, f32c(table.detach() if table.requires_grad else table), float(scale), dtype)
 
 
 # ------------------------------------------------------------------------------------------------------------
