@@ -659,6 +659,58 @@ def test_two_captured_graphs_do_not_share_scratch():
 
 
 @gpu
+def test_graph_of_split_pools():
+    def inputs(seed):
+        g = gen(seed)
+        x = {"q": randn(g, 3, 333, 8, 32), "k": randn(g, 3, 4111, 2, 32), "v": randn(g, 3, 4111, 2, 32)}
+        x = {n: t.requires_grad_(True) for n, t in x.items()}
+        x["blocks"], x["do"] = some_blocks(g, 3, 8, 333, 65, 7), randn(g, 3, 333, 8, 32)
+        return x
+
+    def step(x):
+        leaves = [x[n] for n in "qkv"]
+        out = ops().block_attention(*leaves, x["blocks"])
+        return [out.detach(), *torch.autograd.grad(out, leaves, x["do"])]
+    want = [[t.clone() for t in step(inputs(s))] for s in (1, 2)]
+    static = inputs(1)
+    graph = ops().new_graph()
+    with torch.cuda.graph(graph):
+        got = step(static)
+    for s in (2, 1, 2):
+        fresh = inputs(s)
+        with torch.no_grad():
+            for n in static:
+                static[n].copy_(fresh[n])
+        graph.replay()
+        for a, b in zip(got, want[s - 1]):
+            assert torch.equal(a, b)
+        torch.randn(1 << 20, device="cuda").sum().item()
+
+
+@gpu
+def test_more_workgroups_than_one_dimension_holds():
+    """Over 2^20 workgroups: queries taken one by one, and token rows. The end of the call equals a call for the end."""
+    rows_together(1)
+    g = gen(17)
+    L, tail = (1 << 22) + 4099, 5000
+    q, k, v, do = randn(g, 1, L, 1, 8), randn(g, 1, 130, 1, 8), randn(g, 1, 130, 1, 8), randn(g, 1, L, 1, 8)
+    keys = ops().block_keys(k)
+    blocks = ops().block_select(q, keys, 2)
+    end = slice(L - tail, L)
+    assert torch.equal(blocks[:, :, end], ops().block_select(q[:, end], keys, 2))
+    leaf, part = q.requires_grad_(True), q[:, end].detach().clone().requires_grad_(True)
+    out = ops().block_attention(leaf, k, v, blocks)
+    small = ops().block_attention(part, k, v, blocks[:, :, end])
+    assert torch.equal(out[:, end], small)
+    (dq,), (dp,) = torch.autograd.grad(out, leaf, do), torch.autograd.grad(small, part, do[:, end])
+    assert torch.equal(dq[:, end], dp)
+    table = torch.randn(3, 257, generator=g, device="cuda")
+    tokens = torch.randint(0, 3, (L,), generator=g, device="cuda")
+    rows = ops().token_embed(tokens, table)
+    assert torch.equal(rows[-tail:], table[tokens[-tail:]].to(torch.bfloat16)) and torch.equal(rows[:tail], table[tokens[:tail]].to(torch.bfloat16))
+
+
+@gpu
 def test_on_a_stream_of_the_callers():
     want = _everything(_inputs(6))
     s = torch.cuda.Stream()
