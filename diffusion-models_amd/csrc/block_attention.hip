@@ -27,7 +27,7 @@ struct Args {
   const unsigned short* rows;
   float* part;                 // of a pool whose blocks are split: its slices' sums, [slice][row of the call][D], and statistics behind
   f32x4_t* part_stat;
-  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools, slices;
+  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools, slices, near;
   float scale;
 };
 
@@ -448,13 +448,29 @@ struct Pool {
   }
 };
 
+// Workgroup `id` of `each` to a (sample, key head): which one, and which of its `each`. The workgroups of a head go to one XCD, whose L2
+// then holds its keys and values, and so do those of `near` neighbouring heads, side by side: narrow heads share cache lines (8 of
+// 8 features in 128 bytes), which 8 XCDs would otherwise fetch once each.
+__device__ __forceinline__ bool head_of_block(const Args& a, long id, int each, int& bh, int& part) {
+  const int nbh = a.B * a.Hkv, units = nbh / a.near, wide = each * a.near;
+  long unit, in;
+  if ((units & 7) == 0) {
+    const long local = id >> 3;
+    unit = local / wide * 8 + (id & 7);
+    in = local % wide;
+  } else {
+    unit = id / wide;
+    in = id % wide;
+  }
+  part = (int)(in / a.near);
+  bh = (int)(unit * a.near + in % a.near);
+  return unit < units;
+}
 __device__ __forceinline__ bool pool_of_block(const Args& a, int& bh, int& pool, int& slice) {
-  const int nbh = a.B * a.Hkv, each = a.pools * a.slices;
-  if ((nbh & 7) == 0) dm_xcd_tile(blockIdx.x, each, bh, pool);   // one head's pools on one XCD: its keys and values stay in that L2
-  else { bh = blockIdx.x / each; pool = blockIdx.x % each; }
+  if (!head_of_block(a, blockIdx.x, a.pools * a.slices, bh, pool)) return false;
   slice = a.slices == 1 ? 0 : pool / a.pools;
   pool -= slice * a.pools;
-  return bh < nbh;
+  return true;
 }
 // where a slice's sums of a row begin (`row` counts the call's rows: (sample, position, head))
 __device__ __forceinline__ long part_row(const Args& a, int slice, long row) { return (long)slice * ((long)a.B * a.Lq * a.Hq) + row; }
@@ -869,7 +885,9 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
   __shared__ __attribute__((aligned(16))) float stat[4][2][32];           // lse, -delta
   __shared__ unsigned short list[LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-  const int j = blockIdx.x, bh = blockIdx.y, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  int j, bh;
+  if (!head_of_block(a, dm_block_index(), a.nblk, bh, j)) return;
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int n0 = valid_keys(a.k_len, b, a.Lk) - j * BLK;
   const float sc = a.scale * LOG2E;
   // The chain of loads at the start (where the block's rows lie in the lists, the rows, their q and do) and the keys and values
@@ -1100,6 +1118,8 @@ Args args_of(const dm_block_desc* d) {
   a.pools = plan_of(d).pools;
   a.scale = d->scale;
   a.slices = 1;
+  // neighbouring heads that share cache lines, as many as leave every XCD some
+  for (a.near = 64 / d->D; a.near > 1 && (d->Hkv % a.near || (long)d->B * d->Hkv / a.near % 8); a.near /= 2) {}
   return a;
 }
 
@@ -1214,7 +1234,7 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   }
   else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dim3(a.nblk, d->B * d->Hkv), dim3(256), 0, st, a));
+  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dm_grid((long)a.nblk * d->B * d->Hkv), dim3(256), 0, st, a));
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
