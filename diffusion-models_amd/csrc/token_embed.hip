@@ -215,10 +215,31 @@ __global__ __launch_bounds__(256) void sort_pass_kernel(const int64_t* __restric
   }
 }
 
-// The whole sort of a small call in one launch: the same passes, by one workgroup in LDS
+// A table of zeros, for rows that no token names: workgroup `group` of `groups` with T threads. Bound by HBM's writes.
+constexpr int CLEAR = 4;   // 16-byte pieces a thread
+template <int T>
+__device__ __forceinline__ void clear(float* __restrict__ to, long n, long vecs, long group, long groups) {
+  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < CLEAR; ++u) {
+    const long i = (group * CLEAR + u) * T + threadIdx.x;
+    if (i < vecs) ((f32x4_t*)to)[i] = zero;
+  }
+  for (long i = vecs * 4 + group * T + threadIdx.x; i < n; i += groups * T) to[i] = 0.f;
+}
+__global__ __launch_bounds__(256) void clear_kernel(float* __restrict__ to, long n, long vecs) {
+  clear<256>(to, n, vecs, dm_block_index(), (long)gridDim.x * gridDim.y);
+}
+
+// The whole sort of a small call in one launch: the same passes, by one workgroup in LDS. The others clear the table meanwhile.
 constexpr int SMALL = 8192;
 __global__ __launch_bounds__(1024) void sort_small_kernel(const int64_t* __restrict__ tokens, unsigned* __restrict__ key_out,
-                                                          unsigned* __restrict__ idx_out, int n, long rows, long padding, int passes) {
+                                                          unsigned* __restrict__ idx_out, int n, long rows, long padding, int passes,
+                                                          float* __restrict__ table, long floats, long vecs) {
+  if (dm_block_index() > 0) {
+    clear<1024>(table, floats, vecs, dm_block_index() - 1, (long)gridDim.x * gridDim.y - 1);
+    return;
+  }
   __shared__ unsigned skey[SMALL];
   __shared__ unsigned short sidx[SMALL], wcount[16][RADIX];
   __shared__ unsigned wsum[4];
@@ -368,19 +389,6 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const T* __restrict__ dout
   }
 }
 
-// A table of zeros, for rows that no token names. Bound by HBM's writes.
-constexpr int CLEAR = 4;   // 16-byte pieces a thread
-__global__ __launch_bounds__(256) void clear_kernel(float* __restrict__ to, long n, long vecs) {
-  const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
-  const long group = dm_block_index(), groups = (long)gridDim.x * gridDim.y;
-#pragma unroll
-  for (int u = 0; u < CLEAR; ++u) {
-    const long i = (group * CLEAR + u) * 256 + threadIdx.x;
-    if (i < vecs) ((f32x4_t*)to)[i] = zero;
-  }
-  for (long i = vecs * 4 + group * 256 + threadIdx.x; i < n; i += groups * 256) to[i] = 0.f;
-}
-
 // A run that goes on behind the chunk it began in: its parts, chunk by chunk
 template <int V>
 __global__ __launch_bounds__(256) void run_join_kernel(const unsigned* __restrict__ key, const float* __restrict__ part,
@@ -503,15 +511,16 @@ extern "C" int dm_token_embed_bwd(const void* dout, int dout_bf16, const int64_t
   float* part = (float*)(w + p.part);
   hipStream_t st = (hipStream_t)stream;
   const dim3 block(256), tiles(p.tiles);
-  if (accumulate == 2) {
-    const long all = rows * width, vecs = ((uintptr_t)dtable & 15) ? 0 : all / 4;
-    hipLaunchKernelGGL(clear_kernel, dm_grid(all / (4 * 256 * CLEAR) + 1), block, 0, st, dtable, all, vecs);
+  const int scan = p.tiles > SCAN_TILES;
+  const long floats = accumulate == 2 ? rows * width : 0, vecs = ((uintptr_t)dtable & 15) ? 0 : floats / 4;
+  if (floats && n > SMALL) {
+    hipLaunchKernelGGL(clear_kernel, dm_grid(floats / (4 * 256 * CLEAR) + 1), block, 0, st, dtable, floats, vecs);
     DM_CHECK_LAUNCH();
   }
-  const int scan = p.tiles > SCAN_TILES;
   // one workgroup up to 8192 tokens (backward with 320 features, in one launch / in two a pass: 4999 tokens 26 / 35 us, 8192 32 / 37)
   if (n <= SMALL) {
-    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(1024), 0, st, tokens, key[(p.passes - 1) & 1], idx[(p.passes - 1) & 1], (int)n, rows, padding, p.passes);
+    hipLaunchKernelGGL(sort_small_kernel, dm_grid(floats ? floats / (4 * 1024 * CLEAR) + 2 : 1), dim3(1024), 0, st, tokens,
+                       key[(p.passes - 1) & 1], idx[(p.passes - 1) & 1], (int)n, rows, padding, p.passes, dtable, floats, vecs);
     DM_CHECK_LAUNCH();
   }
   for (int i = 0; i < p.passes && n > SMALL; ++i) {
