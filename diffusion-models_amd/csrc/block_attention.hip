@@ -873,7 +873,7 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
 // order. Scores are formed as S = Q K^T here: a lane holds 4 rows x 2 tiles of ONE key, which is the layout that dv =
 // P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
 // Bound by registers with 64 features (the sums of 64 keys take 128; 2 waves a SIMD) and by the latency of a tile's chain: 121 us for 4 x 8
-// heads of 4096 queries and keys, 8 of 64 blocks, 0.43 PFLOP/s issued; 109 us for 8 x 64 heads of 1024 and 8 features, 4 of 16. (p and
+// heads of 4096 queries and keys, 8 of 64 blocks, 0.43 PFLOP/s issued; 107 us for 8 x 64 heads of 1024 and 8 features, 4 of 16. (p and
 // ds rounded once: 107 and 87 us. Pairs with 32 keys at a time: 148 and 138, registers spilled.)
 constexpr int LIST = 4096;
 template <int D>
