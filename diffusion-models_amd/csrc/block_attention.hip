@@ -1084,20 +1084,22 @@ int check_span(const char* who, const dm_block_desc* d) {
 // (Pools of 128 and 256 rows, which occupy more CUs where there are few rows, were never faster by more than 5 %.)
 struct Form { bool pool; int slices; };
 Form form_of(const dm_block_desc* d) {
-  // The two round differently, and a sample's result must not depend on the batch it is in: the choice is priced for 4 samples.
-  const double rows = (double)d->Lq * (d->Hq / d->Hkv), heads = 4.0 * d->Hkv;
-  const double at_once = d->D <= 16 ? 512 : 256, visit = d->D <= 16 ? 900 : d->D == 32 ? 1050 : 1500;
-  const double pools = heads * dm_cdiv((long)rows, POOL), most = (rows < POOL ? rows : POOL) * d->top;
-  const double visits = most < blocks_of(d) ? most : blocks_of(d);
-  Form f = {true, 1};
-  double best = 0;
-  for (int s = 1; s <= MAX_SLICES; s *= 2) {
-    const double rounds = (double)(long)((pools * s + at_once - 1) / at_once), moved = s > 1 ? heads * rows * s * (d->D * 4 + 16) * 2 : 0;
-    const double ns = (s > 1 ? 14000.0 : 8000.0) + rounds * visits / s * visit + moved / 3000;
-    if (s == 1 || ns < best) { best = ns; f.slices = s; }
-  }
   if (d->pool) return Form{d->pool == POOL, 1};
-  f.pool = heads * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 1.25 * best;
+  // The forms round differently, and a sample's result must not depend on the batch it is in: they are priced for a batch that is
+  // assumed, slices for 4 samples and single queries for 8. (What that costs other batches, us, as chosen / the best form: 8 heads x 256
+  // queries, 8 of 64 blocks of 64 features, 1 sample 28 / 25, 64 samples 342 / 176; 2 heads of 4 x 333, 7 of 65 of 32 features, 80 samples 247 / 134.)
+  const double rows = (double)d->Lq * (d->Hq / d->Hkv), most = (rows < POOL ? rows : POOL) * d->top;
+  const double at_once = d->D <= 16 ? 512 : 256, visit = d->D <= 16 ? 900 : d->D == 32 ? 1050 : 1500;
+  const double visits = most < blocks_of(d) ? most : blocks_of(d);
+  auto pool_ns = [&](double samples, int s) {
+    const double heads = samples * d->Hkv, pools = heads * dm_cdiv((long)rows, POOL);
+    const double rounds = (double)(long)((pools * s + at_once - 1) / at_once), moved = s > 1 ? heads * rows * s * (d->D * 4 + 16) * 2 : 0;
+    return (s > 1 ? 14000.0 : 8000.0) + rounds * visits / s * visit + moved / 3000;
+  };
+  Form f = {true, 1};
+  for (int s = 2; s <= MAX_SLICES; s *= 2)
+    if (pool_ns(4, s) < pool_ns(4, f.slices)) f.slices = s;
+  f.pool = 8 * d->Hkv * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 1.25 * pool_ns(8, f.slices);
   return f;
 }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
