@@ -161,8 +161,8 @@ __global__ __launch_bounds__(256) void attend_row_kernel(Args a, long rows) {
   }
 }
 
-// dq of one query a wave, and delta for the kernel behind: blocks are read once more from the caches (2 x 4 heads x 200 queries, 16 of
-// 256 blocks of 64 features: the whole backward pass takes what its host calls take)
+// dq of one query a wave, and delta for the kernel behind. Bound by the caches, which every query reads its blocks from (2 x 4 heads x 200
+// queries, 16 of 256 blocks of 64 features: 61 us for 419 MB, 6.9 TB/s)
 template <int D>
 __global__ __launch_bounds__(256) void dq_row_kernel(Args a, long rows) {
   constexpr int LPR = D / 8, KPI = 64 / LPR, NI = BLK / KPI;
@@ -450,7 +450,7 @@ struct Pool {
 
 // Workgroup `id` of `each` to a (sample, key head): which one, and which of its `each`. The workgroups of a head go to one XCD, whose L2
 // then holds its keys and values, and so do those of `near` neighbouring heads, side by side: narrow heads share cache lines (8 of
-// 8 features in 128 bytes), which 8 XCDs would otherwise fetch once each.
+// 8 features in 128 bytes), which 8 XCDs would otherwise fetch once each (8 x 64 heads of 1024 queries and 8 features: dq 125 -> 87 us).
 __device__ __forceinline__ bool head_of_block(const Args& a, long id, int each, int& bh, int& part) {
   const int nbh = a.B * a.Hkv, units = nbh / a.near, wide = each * a.near;
   long unit, in;
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
 }
 
 // dq of a pool, and delta for the kernel behind. dq gathers p (dp - delta) k; the scale is applied once at the end. Bound as the
-// forward kernel is, with one product more in a visit (the call above: 115 us).
+// forward kernel is, with one product more in a visit (the call above: 117 us).
 template <int D>
 __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   using GE = Geo<D>;
