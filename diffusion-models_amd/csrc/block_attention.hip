@@ -27,7 +27,8 @@ struct Args {
   const unsigned short* rows;
   float* part;                 // of a pool whose blocks are split: its slices' sums, [slice][row of the call][D], and statistics behind
   f32x4_t* part_stat;
-  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools, slices, near;
+  float* key_part;             // of blocks whose rows are split: the slices' dk and dv, [slice][sample, key head][block][2][64][D]
+  int B, Lq, Lk, Hq, Hkv, G, top, nblk, pools, slices, row_slices, near;
   float scale;
 };
 
@@ -868,13 +869,21 @@ __global__ __launch_bounds__(POOL) void dq_pool_kernel(Args a) {
   }
 }
 
+__device__ __forceinline__ void write_keys(const Args& a, float (&dk)[8], const float (&dv)[8], int b, int hk, long pos, int d) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) dk[x] *= a.scale;
+  *(bf16x8_t*)(a.dk + b * a.dkb + pos * a.dkl + hk * a.dkh + d) = dm_pack8(dk);
+  *(bf16x8_t*)(a.dv + b * a.dvb + pos * a.dvl + hk * a.dvh + d) = dm_pack8(dv);
+}
+
 // dk and dv of one block, four waves. The rows that chose it are packed into a list, 4096 rows at a time, and dealt to the
 // waves in tiles of 32; every wave sums all 64 keys over its own rows in registers, and the four sums are added in wave
 // order. Scores are formed as S = Q K^T here: a lane holds 4 rows x 2 tiles of ONE key, which is the layout that dv =
 // P^T dO and dk = dS^T Q take as their left operand; the right operands are the tile's rows, read transposed from the wave's own LDS.
 // Bound by registers with 64 features (the sums of 64 keys take 128; 2 waves a SIMD) and by the latency of a tile's chain: 121 us for 4 x 8
 // heads of 4096 queries and keys, 8 of 64 blocks, 0.43 PFLOP/s issued; 107 us for 8 x 64 heads of 1024 and 8 features, 4 of 16. (p and
-// ds rounded once: 107 and 87 us. Pairs with 32 keys at a time: 148 and 138, registers spilled.)
+// ds rounded once: 107 and 87 us. Pairs with 32 keys at a time: 148 and 138, registers spilled.) Where blocks are few, their rows are dealt
+// to up to 8 workgroups, pool by pool, and joined by dkv_join_kernel (row_slices_of).
 constexpr int LIST = 4096;
 template <int D>
 __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel(Args a) {
@@ -886,7 +895,9 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
   __shared__ unsigned short list[LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
   int j, bh;
-  if (!head_of_block(a, dm_block_index(), a.nblk, bh, j)) return;
+  if (!head_of_block(a, dm_block_index(), a.nblk * a.row_slices, bh, j)) return;
+  const int slice = j / a.nblk, p_first = (int)((long)a.pools * slice / a.row_slices), p_end = (int)((long)a.pools * (slice + 1) / a.row_slices);
+  j -= slice * a.nblk;
   const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int n0 = valid_keys(a.k_len, b, a.Lk) - j * BLK;
   const float sc = a.scale * LOG2E;
@@ -895,13 +906,13 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
   constexpr int per = LIST / POOL;    // pools whose rows fit the list
   int start = 0, own = 0;
   auto find = [&](int p0) {           // lane x: the rows of pool p0 + x
-    const bool has = lane < per && p0 + lane < a.pools;
+    const bool has = lane < per && p0 + lane < p_end;
     const int* at = a.offs + ((long)bh * a.pools + p0 + lane) * (a.nblk + 1) + j;
     start = has ? at[0] : 0;
     own = has ? at[1] - start : 0;
   };
   if (n0 > 0) {
-    find(0);
+    find(p_first);
     constexpr int PER = (2 * BLK * D / 8 + 255) / 256;
     const bf16x8_t none = {};
     bf16x8_t x[PER];
@@ -931,8 +942,8 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
   const float *const lbase = a.lse + (long)b * a.Hq * a.Lq, *const dbase = a.delta + (long)b * a.Hq * a.Lq;
   char *qb = rows[wave][0], *ob = rows[wave][1];
   float *st_lse = stat[wave][0], *st_delta = stat[wave][1];
-  for (int p0 = 0; p0 < a.pools && n0 > 0; p0 += per) {
-    if (p0) find(p0);
+  for (int p0 = p_first; p0 < p_end && n0 > 0; p0 += per) {
+    if (p0 > p_first) find(p0);
     int inc = own;
 #pragma unroll
     for (int o = 1; o < per; o <<= 1) {
@@ -941,7 +952,7 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
     }
     const int count = __builtin_amdgcn_readlane(inc, per - 1), before = inc - own;
     __syncthreads();   // the list's last use is over
-    for (int x = wave; x < per && p0 + x < a.pools; x += 4) {
+    for (int x = wave; x < per && p0 + x < p_end; x += 4) {
       const int s = __builtin_amdgcn_readlane(start, x), m = __builtin_amdgcn_readlane(own, x), to = __builtin_amdgcn_readlane(before, x);
       const unsigned short* from = a.rows + ((long)bh * a.pools + p0 + x) * ((long)POOL * a.top) + s;
       for (int e = lane; e < m; e += 64) list[to + e] = (unsigned short)(x * POOL + from[e]);
@@ -1051,14 +1062,44 @@ __global__ __launch_bounds__(256, D <= 16 ? 4 : D == 32 ? 3 : 2) void dkv_kernel
     const long pos = (long)j * BLK + t;
     const bool live = t < n0;   // positions behind the last valid key: zero
     const int place = (((t >> 4) * GE::DT + (d >> 4)) * 64 + ((t >> 2) & 3) * 16 + (d & 15)) * 4 + (t & 3);
-    float f[8];
+    float f[8], h[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? sum[place + x * 4] * a.scale : 0.f;
-    *(bf16x8_t*)(a.dk + b * a.dkb + pos * a.dkl + hk * a.dkh + d) = dm_pack8(f);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = live ? sum[HALF + place + x * 4] : 0.f;
-    *(bf16x8_t*)(a.dv + b * a.dvb + pos * a.dvl + hk * a.dvh + d) = dm_pack8(f);
+    for (int x = 0; x < 8; ++x) {
+      f[x] = live ? sum[place + x * 4] : 0.f;
+      h[x] = live ? sum[HALF + place + x * 4] : 0.f;
+    }
+    if (a.row_slices == 1) {
+      write_keys(a, f, h, b, hk, pos, d);
+    } else {
+      float* to = a.key_part + ((((long)slice * a.B * a.Hkv + bh) * a.nblk + j) * 2 * BLK + t) * D + d;
+      *(f32x4_t*)to = *(const f32x4_t*)f;
+      *(f32x4_t*)(to + 4) = *(const f32x4_t*)(f + 4);
+      *(f32x4_t*)(to + BLK * D) = *(const f32x4_t*)h;
+      *(f32x4_t*)(to + BLK * D + 4) = *(const f32x4_t*)(h + 4);
+    }
   }
+}
+
+// dk and dv of blocks whose rows were split, in the order of the slices
+template <int D>
+__global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
+  constexpr int PC = D / 8;
+  const long e = dm_block_index() * 256 + threadIdx.x, at = e / PC;   // (sample, key head), key
+  const int d = (int)(e % PC) * 8;
+  const long bh = at / a.Lk, pos = at - bh * a.Lk;
+  if (bh >= (long)a.B * a.Hkv) return;
+  float f[8] = {0, 0, 0, 0, 0, 0, 0, 0}, h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < MAX_SLICES; ++s)
+    if (s < a.row_slices) {
+      const float* p = a.key_part + ((((long)s * a.B * a.Hkv + bh) * a.nblk + pos / BLK) * 2 * BLK + pos % BLK) * D + d;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        f[k] += p[k];
+        h[k] += p[BLK * D + k];
+      }
+    }
+  write_keys(a, f, h, (int)(bh / a.Hkv), (int)(bh % a.Hkv), pos, d);
 }
 
 // rows are addressed inside a sample by 32-bit numbers of 8 features
@@ -1102,6 +1143,23 @@ Form form_of(const dm_block_desc* d) {
   f.pool = 8 * d->Hkv * rows * (0.3 + d->top * (0.46 + 0.005 * d->D)) > 1.25 * pool_ns(8, f.slices);
   return f;
 }
+// In how many slices the rows of a block are dealt to workgroups for dk and dv, priced for 4 samples as above: 256 CUs hold 2 workgroups
+// with 64 features, 3 with 32, 4 with fewer; one takes 5 us + 2.5 us for 128 rows. (A training call, unsplit / split, us, host included: 8 heads
+// of 16384 queries and 77 keys of 64 features 370 / 144; 32 such samples of 4096 queries, for which a split is not needed, 625 / 691.)
+int row_slices_of(const dm_block_desc* d) {
+  const double rows = (double)d->Lq * (d->Hq / d->Hkv), named = rows * d->top / blocks_of(d), each = named < rows ? named : rows;
+  const double groups = 4.0 * d->Hkv * blocks_of(d), at_once = 256 * (d->D == 64 ? 2 : d->D == 32 ? 3 : 4);
+  const int pools = dm_cdiv((long)rows, POOL);
+  auto ns = [&](int s) {
+    const double rounds = (double)(long)((groups * s + at_once - 1) / at_once);
+    return rounds * (5000 + each / s / 128 * 2500) + (s > 1 ? 6000 + groups * s * BLK * d->D * 16 / 3000 : 0);
+  };
+  int best = 1;
+  for (int s = 2; s <= MAX_SLICES && s <= pools; s *= 2)
+    if (ns(s) < ns(best)) best = s;
+  return best;
+}
+size_t key_part_bytes(const dm_block_desc* d, int slices) { return (size_t)slices * d->B * d->Hkv * blocks_of(d) * 2 * BLK * d->D * 4; }
 // The plan's pools (made for the backward pass also where the forward takes one query a workgroup), and its parts
 struct PlanLayout { int pools; size_t offs, bytes; };
 PlanLayout plan_of(const dm_block_desc* d) {
@@ -1119,7 +1177,7 @@ Args args_of(const dm_block_desc* d) {
   a.nblk = blocks_of(d);
   a.pools = plan_of(d).pools;
   a.scale = d->scale;
-  a.slices = 1;
+  a.slices = a.row_slices = 1;
   // neighbouring heads that share cache lines, as many as leave every XCD some
   for (a.near = 64 / d->D; a.near > 1 && (d->Hkv % a.near || (long)d->B * d->Hkv / a.near % 8); a.near /= 2) {}
   return a;
@@ -1187,7 +1245,7 @@ extern "C" int dm_block_attention_fwd(const dm_block_desc* d, const void* q, con
   return DM_OK;
 }
 
-// (delta first in the workspace, the slices' sums behind it)
+// (delta first in the workspace, slices' sums behind it)
 static size_t delta_bytes(size_t rows) { return (rows * 4 + 15) / 16 * 16; }
 
 extern "C" size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d) {
@@ -1195,7 +1253,9 @@ extern "C" size_t dm_block_attention_bwd_ws_bytes(const dm_block_desc* d) {
   if (check_desc(who, d) || check_pool(who, d)) return 0;
   const Form f = form_of(d);
   const size_t rows = (size_t)d->B * d->Hq * d->Lq;
-  return delta_bytes(rows) + (f.pool && f.slices > 1 ? f.slices * rows * d->D * 4 : 0);
+  const int k = row_slices_of(d);
+  const size_t queries = f.pool && f.slices > 1 ? f.slices * rows * d->D * 4 : 0, keys = k > 1 ? key_part_bytes(d, k) : 0;
+  return delta_bytes(rows) + (queries > keys ? queries : keys);   // (one after the other in the same memory)
 }
 
 extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, const void* k, const void* v, const int* blocks,
@@ -1236,7 +1296,13 @@ extern "C" int dm_block_attention_bwd(const dm_block_desc* d, const void* q, con
   }
   else BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dq_row_kernel<HD>), dm_grid(dm_cdiv(rows, 4)), dim3(256), 0, st, a, rows))
   DM_CHECK_LAUNCH();
-  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dm_grid((long)a.nblk * d->B * d->Hkv), dim3(256), 0, st, a));
+  a.row_slices = row_slices_of(d);
+  a.key_part = (float*)((char*)ws + delta_bytes(rows));
+  BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_kernel<HD>), dm_grid((long)a.nblk * a.row_slices * d->B * d->Hkv), dim3(256), 0, st, a));
+  if (a.row_slices > 1) {
+    DM_CHECK_LAUNCH();
+    BY_HEAD_DIM(d->D, hipLaunchKernelGGL((dkv_join_kernel<HD>), dm_grid(((long)d->B * d->Hkv * d->Lk * (HD / 8) + 255) / 256), dim3(256), 0, st, a));
+  }
   DM_CHECK_LAUNCH();
   return DM_OK;
 }

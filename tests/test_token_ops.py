@@ -290,6 +290,40 @@ def test_block_attention_of_split_pools(B, Lq, Lk, Hq, Hkv, D, top, ragged, chos
 
 
 @gpu
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,top,ragged", [
+    (2, 4500, 300, 2, 2, 8, 3, False),
+    (3, 3000, 100, 4, 2, 16, 2, True),
+    (2, 2100, 130, 4, 1, 32, 2, True),
+    (1, 5000, 64, 2, 1, 64, 1, False),
+])
+def test_block_attention_of_few_keys_and_many_queries(B, Lq, Lk, Hq, Hkv, D, top, ragged):
+    """Few blocks that many rows chose: the rows are dealt to several workgroups for dk and dv."""
+    import ctypes
+    from dm_hip import lib
+    g = gen(18)
+    q, k, v, do = randn(g, B, Lq, Hq, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lk, Hkv, D), randn(g, B, Lq, Hq, D)
+    k_len = torch.tensor([Lk - 1, 0, Lk // 3], dtype=torch.int32, device="cuda")[:B] if ragged else None
+    if ragged:
+        for b in range(B):
+            k[b, int(k_len[b]):], v[b, int(k_len[b]):] = float("nan"), float("inf")
+    blocks = some_blocks(g, B, Hq, Lq, -(-Lk // BLOCK), top)
+    desc = ops()._block_desc(B, Lq, Lk, Hq, Hkv, D, top, 1.0, q, k, v)
+    assert lib.dm_block_attention_bwd_ws_bytes(ctypes.byref(desc)) > B * Lq * Hq * 4 + 16
+    scale = 1.3 * D ** -0.5
+    ref = ref_attention(q, k, v, blocks, scale, k_len, do)
+
+    def run(sl):
+        leaves = [x[sl].clone().requires_grad_(True) for x in (q, k, v)]
+        out = ops().block_attention(*leaves, blocks[sl], scale, None if k_len is None else k_len[sl])
+        return [out.detach(), *torch.autograd.grad(out, leaves, do[sl])]
+    got = run(slice(0, B))
+    for name, x, (want, bound) in zip(("out", "dq", "dk", "dv"), got, ref):
+        within(name, x, want, bound)
+    for x, y in zip(got, run(slice(B - 1, B))):
+        assert torch.equal(x[B - 1:], y)
+
+
+@gpu
 @pytest.mark.parametrize("pool", [1, 512])
 def test_block_attention_of_one_sharp_weight(pool):
     """One key takes (almost) all the weight: ds is a small difference of large numbers."""
