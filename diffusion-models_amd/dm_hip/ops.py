@@ -974,16 +974,26 @@ def _block_kept(d, plan_bytes):
     return out_lo, lse, lse + rows * 4
 
 
-def _block_backward(desc, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
-    d = BlockDesc.from_buffer_copy(desc)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+def _block_setup(ctx, d, q, k, v, dq_strides, dk_strides):
+    """What the backward call needs besides tensors, made while the forward call's thread has it at hand"""
+    d.dq_stride[:], d.dk_stride[:], d.dv_stride[:] = dq_strides, dk_strides, dk_strides
     ref = ctypes.byref(d)
-    n = lib.dm_block_attention_bwd_ws_bytes(ref)
-    ws = _scratch(q.device, (n + 3) // 4)
-    out_lo, lse, _ = _block_kept(d, lib.dm_block_attention_plan_bytes(ref, 1))
+    ctx.d = d
+    ctx.strides = (q.stride(), k.stride(), v.stride())
+    ctx.sizes = (lib.dm_block_attention_bwd_ws_bytes(ref), *_block_kept(d, lib.dm_block_attention_plan_bytes(ref, 1))[:2])
+
+
+def _block_backward(ctx, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv):
+    d = ctx.d
+    if (q.stride(), k.stride(), v.stride()) != ctx.strides:   # (saved tensors came back laid out otherwise)
+        d = BlockDesc.from_buffer_copy(d)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    n, out_lo, lse = ctx.sizes
+    if dout.dtype is not BF16 or not dout.is_contiguous() or dout.data_ptr() & 15:
+        dout = _aligned(dout)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
     at = kept.data_ptr()
-    check(lib.dm_block_attention_bwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len), at,
+    check(lib.dm_block_attention_bwd(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), blocks.data_ptr(), _p(k_len), at,
                                      out.data_ptr(), at + out_lo, at + lse, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                                      dv.data_ptr(), ws.data_ptr(), n, _stream()))
 
@@ -994,7 +1004,7 @@ class _BlockAttentionFn(Function):
         with _on(q.device):
             out, kept = _block_forward(d, q, k, v, blocks, k_len, True)
         ctx.save_for_backward(q, k, v, blocks, k_len, out, kept)
-        ctx.d = d
+        _block_setup(ctx, d, q, k, v, (d.Lq * d.Hq * d.D, d.Hq * d.D, d.D), (d.Lk * d.Hkv * d.D, d.Hkv * d.D, d.D))
         return out
 
     @staticmethod
@@ -1002,8 +1012,8 @@ class _BlockAttentionFn(Function):
     def backward(ctx, dout):
         q, k, v, blocks, k_len, out, kept = ctx.saved_tensors
         with _on(q.device):
-            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-            _block_backward(ctx.d, q, k, v, blocks, k_len, out, kept, _aligned(dout), dq, dk, dv)
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)   # (contiguous: _block_setup)
+            _block_backward(ctx, q, k, v, blocks, k_len, out, kept, dout, dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -1059,7 +1069,7 @@ class _SparseAttentionFn(Function):
             out, kept = _block_forward(d, q, k, v, blocks, None, training)
         if training:
             ctx.save_for_backward(qkv, blocks, out, kept)
-            ctx.d = d
+            _block_setup(ctx, d, q, k, v, q.stride()[:3], k.stride()[:3])
         return out.view(B, L, H * D)
 
     @staticmethod
@@ -1069,8 +1079,8 @@ class _SparseAttentionFn(Function):
         d = ctx.d
         parts = (d.B, d.Lq, 3, d.Hq, d.D)
         with _on(qkv.device):
-            dqkv = torch.empty_like(qkv)
-            _block_backward(d, *qkv.view(parts).unbind(2), blocks, None, out, kept, _aligned(dout), *dqkv.view(parts).unbind(2))
+            dqkv = qkv.new_empty(qkv.shape)   # (contiguous, as qkv was in the forward call)
+            _block_backward(ctx, *qkv.view(parts).unbind(2), blocks, None, out, kept, dout, *dqkv.view(parts).unbind(2))
         return dqkv, None, None, None, None, None
 
 

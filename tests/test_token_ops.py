@@ -745,6 +745,28 @@ def test_more_workgroups_than_one_dimension_holds():
 
 
 @gpu
+def test_saved_tensors_that_come_back_from_elsewhere():
+    g = gen(19)
+    q, k, v, do = (randn(g, 2, 130, 4, 16) for _ in range(4))
+    blocks = some_blocks(g, 2, 4, 130, 3, 2)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    want = torch.autograd.grad(ops().block_attention(*leaves, blocks), leaves, do)
+
+    def heads_first(t):   # the same values, laid out otherwise
+        t = t.cuda()
+        return t.transpose(1, 2).contiguous().transpose(1, 2) if t.shape == q.shape and any(torch.equal(t, x) for x in leaves) else t
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), heads_first):
+        out = ops().block_attention(*leaves, blocks)
+    for a, b in zip(torch.autograd.grad(out, leaves, do), want):
+        assert torch.equal(a, b)
+    qkv, dp = randn(g, 2, 260, 3 * 64).requires_grad_(True), randn(g, 2, 260, 64)
+    want = torch.autograd.grad(ops().sparse_attention(qkv, 4, 16, 2), qkv, dp)
+    with torch.autograd.graph.save_on_cpu():
+        out = ops().sparse_attention(qkv, 4, 16, 2)
+    assert torch.equal(torch.autograd.grad(out, qkv, dp)[0], want[0])
+
+
+@gpu
 def test_on_a_stream_of_the_callers():
     want = _everything(_inputs(6))
     s = torch.cuda.Stream()
